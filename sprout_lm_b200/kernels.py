@@ -21,7 +21,7 @@ F32, BF16 = 0, 1
 LAUNCHES = 0          # kernels launched through this module (one per call); benchmarks read the difference
 STATUS_BITS = {1: "a block-table entry outside the page pool", 2: "a token id outside the vocabulary",
                4: "non-finite logits", 8: "a bounded device-side wait ran out", 16: "a position outside the rotary table",
-               32: "a kernel's shared memory was not aligned for its tiles"}
+               32: "a kernel's shared memory was not aligned for its tiles", 64: "a request's rows outside the step's"}
 
 
 class KernelError(RuntimeError):
@@ -39,6 +39,7 @@ _SIGNATURES = {
     "sprout_attention_simple": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
+    "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
     "sprout_feed_tokens": [_P, _P, _P, _I, _I, _I, _P],
     "sprout_attention_decode": [_P, _I, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
@@ -128,6 +129,8 @@ def load_library(verbose: bool = True):
             lib.sprout_abi_version.restype = c_int
             lib.sprout_sample_scratch_bytes.restype = ctypes.c_longlong
             lib.sprout_sample_scratch_bytes.argtypes = [c_int]
+            lib.sprout_verify_scratch_bytes.restype = ctypes.c_longlong
+            lib.sprout_verify_scratch_bytes.argtypes = [c_int, c_int]
             lib.sprout_delta_scratch_floats.restype = ctypes.c_longlong
             lib.sprout_maps_attention_tc_scratch_floats.restype = ctypes.c_longlong
             lib.sprout_maps_attention_tc_scratch_floats.argtypes = [c_int] * 6
@@ -968,6 +971,81 @@ def sample(logits, out, status, temperature=None, uniform=None):
     _run("sprout_sample", _ptr(logits, "logits", torch.float32), logits.stride(0),
          _ptr(temperature, "temperature", torch.float32, True), _ptr(uniform, "uniform", torch.float32, True),
          _ptr(out, "out", torch.int32), _ptr(scratch, "scratch"), R, V, _ptr(status, "status", torch.int32), _stream())
+
+
+def _one_device(name, **tensors):
+    """All tensors (None: not given) on one CUDA device, the current one."""
+    current = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for what, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{name}: {what} must be a CUDA tensor; there is no CPU path")
+        if t.device.index != current:
+            raise KernelError(f"{name}: {what} is on {t.device}, the current device is cuda:{current}")
+
+
+def _overlap(a, b) -> bool:
+    """Whether two tensors' memory (from the first to the last element) meets."""
+    def span(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def verify_drafts(logits, drafts, row_start, out, accepted, status, draft_logits=None, temperatures=None, accept=None, draw=None):
+    """Which drafted tokens stand against the target's probabilities, and the token after the last that does.
+
+    Request r has rows ``row_start[r]`` to ``row_start[r + 1] - 1`` (int32 [requests + 1]) of ``logits`` (float32 [rows, vocab]), one more
+    than it has drafts: row i is what the target says at the place of its i-th draft, the last what it says behind all of them.
+    ``drafts`` (int32 [rows]) holds the tokens in the same places (a request's last entry is not read).  ``draft_logits`` (float32
+    [rows - requests, vocab]): the draft model's rows, one a draft, request by request; without it a draft counts as drawn with
+    probability 1 (looked up).  ``temperatures`` (float32 [requests]), ``accept`` and ``draw`` (float32 [rows], uniform in [0, 1)):
+    a request with a temperature T > 0 keeps draft x of row i with probability min(1, p(x) / q(x)), p and q the softmax of the two logits
+    over T: where ``accept[i] * q(x) < p(x)``; at the first that is not kept the token is drawn at ``draw[i]`` from max(p - q, 0),
+    behind the last one from p.  Temperature 0 (or no temperatures): drafts stand while they are the row's argmax (the lowest index among
+    ties), then the argmax follows.
+
+    ``out`` (int32 [rows]): the drafts that stand, the token after them, and -1 in the rest of the request's rows; ``accepted`` (int32
+    [requests]): how many stand.  A row that is reached and holds a non-finite logit, or a draft outside the vocabulary, sets a status bit
+    and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
+    name = "verify_drafts"
+    _one_device(name, logits=logits, drafts=drafts, row_start=row_start, out=out, accepted=accepted, status=status, draft_logits=draft_logits,
+                temperatures=temperatures, accept=accept, draw=draw)
+    _rows_contiguous(logits, "logits")
+    rows, vocab = logits.shape
+    requests = row_start.numel() - 1
+    if rows < 1 or vocab < 1 or not 1 <= requests <= rows:
+        raise KernelError(f"{name}: at least one request and a row for each (got {rows} rows of {vocab} logits for {requests} requests)")
+    for what, t, n in (("drafts", drafts, rows), ("row_start", row_start, requests + 1), ("out", out, rows), ("accepted", accepted, requests)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+            raise KernelError(f"{name}: {what} must be contiguous int32 [{n}]")
+    if (temperatures is None) != (accept is None) or (accept is None) != (draw is None):
+        raise KernelError(f"{name}: temperatures, accept and draw go together")
+    for what, t, n in (("temperatures", temperatures, requests), ("accept", accept, rows), ("draw", draw, rows)):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous()):
+            raise KernelError(f"{name}: {what} must be contiguous float32 [{n}]")
+    if draft_logits is not None:
+        _rows_contiguous(draft_logits, "draft_logits")
+        if tuple(draft_logits.shape) != (rows - requests, vocab):
+            raise KernelError(f"{name}: draft_logits must be [{rows - requests}, {vocab}], a row per draft (got {tuple(draft_logits.shape)})")
+        if rows == requests:
+            draft_logits = None                # nobody drafted anything
+    for what, t in (("out", out), ("accepted", accepted)):
+        for other, s in (("logits", logits), ("drafts", drafts), ("row_start", row_start), ("draft_logits", draft_logits), ("temperatures", temperatures),
+                         ("accept", accept), ("draw", draw), ("status", status)):
+            if s is not None and _overlap(t, s):
+                raise KernelError(f"{name}: {what} and {other} share memory")
+    if _overlap(out, accepted):
+        raise KernelError(f"{name}: out and accepted share memory")
+    draft_rows = rows - requests if draft_logits is not None else 0
+    scratch = torch.empty(load_library().sprout_verify_scratch_bytes(rows + draft_rows, vocab), dtype=torch.uint8, device=logits.device)
+    _run("sprout_verify", _ptr(logits, "logits", torch.float32), logits.stride(0), _ptr(draft_logits, "draft_logits", torch.float32, True),
+         draft_logits.stride(0) if draft_logits is not None else 0, _ptr(drafts, "drafts"), _ptr(row_start, "row_start"),
+         _ptr(temperatures, "temperatures", torch.float32, True), _ptr(accept, "accept", torch.float32, True), _ptr(draw, "draw", torch.float32, True),
+         _ptr(out, "out"), _ptr(accepted, "accepted"), _ptr(scratch, "scratch"), rows, draft_rows, requests, vocab,
+         _ptr(status, "status", torch.int32), _stream())
 
 
 def advance_decode(token_ids, positions, context_lens, sampled, history, step_counter):
@@ -2244,4 +2322,4 @@ def describe_status(word: int) -> str:
 
 __all__ = ["KernelError", "BuildError", "load_library", "library_file", "embed", "rmsnorm", "swiglu",
            "rope_append", "gemm_simple", "gemm_bf16", "attention_simple", "attention_tile", "attention_decode", "attention_decode_fused", "attention_decode_resident", "decode_attention_plan", "decode_fusable", "attention_prefill",
-           "paged_attention", "sample", "advance_decode", "feed_tokens", "describe_status"]
+           "paged_attention", "sample", "verify_drafts", "advance_decode", "feed_tokens", "describe_status"]

@@ -39,3 +39,16 @@ def sample(logits: torch.Tensor, status: torch.Tensor, temperatures: torch.Tenso
 
 
 __all__ = ["sample", "uniform_for"]
+
+
+def verify(logits: torch.Tensor, drafts: torch.Tensor, row_start: torch.Tensor, status: torch.Tensor, draft_logits: torch.Tensor | None = None,
+           temperatures: torch.Tensor | None = None, accept: torch.Tensor | None = None, draw: torch.Tensor | None = None):
+    """Drafted tokens against the target's probabilities: ``(tokens, accepted)``, int32 on the device.
+
+    ``tokens`` has a place per row of ``logits``: a request's drafts that stand, the token drawn after them, then -1; ``accepted`` says
+    how many stand.  What is emitted is distributed as if drawn from the target alone; a greedy request (temperature 0, or none given)
+    gets the target's argmax at every place.  The arguments are those of ``kernels.verify_drafts`` (csrc/verify.cu), which this launches."""
+    tokens = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
+    accepted = torch.empty(max(row_start.numel() - 1, 0), dtype=torch.int32, device=logits.device)
+    kernels.verify_drafts(logits, drafts, row_start, tokens, accepted, status, draft_logits, temperatures, accept, draw)
+    return tokens, accepted
