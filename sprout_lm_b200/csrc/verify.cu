@@ -12,28 +12,33 @@
 // maximum; the token is the first row's argmax that was not drafted.
 //
 // A draw decides between neighbouring tokens by a sum over the vocabulary, and neighbours with probabilities of 1e-6 lie next to one
-// another: float32 exponentials leave the running sum off by 1e-8 and would pick the neighbour once in a few hundred draws.  So
-// exponentials and sums are 64-bit (`pow2`: 1e-12).
+// another: float32 exponentials leave the running sum off by 1e-8 and would pick the neighbour once in a few hundred draws.  So the
+// sums a draw is made from are 64-bit sums of 64-bit exponentials (`pow2`: 1e-12).  Those take 33 cycles of an SM's quarter a warp of
+// logits (some 15 64-bit operations, two cycles each), 1.09 T a second, while memory delivers 1.6 T logits a second: only the row that is
+// drawn from takes them.  Whether a draft stands is decided by float32 exponentials, whose sums are good to 1e-8.
 //
-// Two launches.  verify_rows_kernel: a block per (row, run of RUN logits) holds the run in registers: its maximum, first index,
-// sum of exponentials.  verify_pick_kernel: a cluster of CTAs per request merges the runs of its rows, finds the first row that does
-// not stand, and draws: where nothing is taken away from p, from the sums of the runs there are and one run's logits; else the CTAs add
-// up max(p - q, 0) over a share of the runs each and exchange the sums, and the one in whose share the draw falls looks through it.
-#include <cooperative_groups.h>
-
+// Four launches.  verify_rows_kernel: every row in runs of RUN logits, their maxima and sums of exponentials (greedy: the maximum's
+// first index), a block walking a stretch of the rows' runs with the next run on its way.  verify_decide_kernel: a block per request
+// merges its rows' runs, a warp a row, and finds the first row that does not stand.  verify_sums_kernel: the 64-bit sums of that row's
+// runs, a block each.  verify_draw_kernel: a block per request finds the run in which the draw falls and looks through it.
+//
+// The difference in one pass: max(p - q, 0) needs both rows' sums before a single element of it is known.  With a_j, b_j the
+// exponentials and Za, Zb their sums, (p_j - q_j) Zb = a_j rho - b_j, rho = Zb / Za.  The float32 sums give rho to 1e-8, and so the set
+// of tokens where the difference is positive but for those within 1e-8 of zero, which do not matter (1e-8 of them, off by
+// 1e-8): the pass adds up a, b and, over that set, a and b again, from which the exact rho makes the difference's sums.
 #include "common.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int THREADS = 256, PER_THREAD = 16, RUN = THREADS * PER_THREAD;     // logits of a run
-constexpr int WARPS = THREADS / 32;
-constexpr int CTAS = 8;                    // of a request's cluster
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int PER_THREAD = 16, RUN = THREADS * PER_THREAD;       // logits of a run
+constexpr int ROW_BLOCKS = 4;              // of the first kernel, an SM
+constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_LOGITS = RUN / DRAW_THREADS;
 
 struct RunSum { double sum; float max; int index; int bad; int pad; };       // sum: of 2^((v - max) log2(e) / T)
 
 // 2^y for y <= 0 to 1e-12: y = k + f with |f| <= 1/2, 2^f by a polynomial through the Chebyshev nodes, k into the exponent.
+// Below 2^-1000 it is zero.
 __device__ __forceinline__ double pow2(double y) {
   const double magic = 6755399441055744.0;             // 1.5 * 2^52: the sum's low bits are y rounded to a whole number
   const double t = y + magic;
@@ -49,7 +54,7 @@ __device__ __forceinline__ double pow2(double y) {
   p = fma(p, f, 1.0);
   const int k = __double2loint(t);
   const double r = __hiloint2double(__double2hiint(p) + (k << 20), __double2loint(p));
-  return y < -1000.0 ? 0.0 : r;
+  return y >= -1000.0 ? r : 0.0;
 }
 
 __device__ __forceinline__ double warp_sum_d(double v) {
@@ -61,97 +66,150 @@ __device__ __forceinline__ void better(float& v, int& i, float ov, int oi) {
   if (ov > v || (ov == v && oi < i)) { v = ov; i = oi; }
 }
 
-// The logit of a run that a thread's place i holds: side by side in fours over the threads, so that a warp reads whole lines, or
-// (IN_ORDER) PER_THREAD side by side in every thread, for running sums.
-template <bool IN_ORDER> __device__ __forceinline__ int place_of(int i) {
-  return IN_ORDER ? (int)threadIdx.x * PER_THREAD + i : (i >> 2) * (THREADS * 4) + (int)threadIdx.x * 4 + (i & 3);
+// The run's place of a thread's logit i: side by side in fours over the threads, so that a warp reads whole lines.
+__device__ __forceinline__ int place_of(int i) { return (i >> 2) * (THREADS * 4) + (int)threadIdx.x * 4 + (i & 3); }
+// Four logits from `at` on, -inf from `end` on.
+__device__ __forceinline__ float4 load_four(const float* row, int at, int end, bool aligned) {
+  if (aligned && at + 4 <= end) return *(const float4*)(row + at);
+  return make_float4(at < end ? row[at] : -INFINITY, at + 1 < end ? row[at + 1] : -INFINITY, at + 2 < end ? row[at + 2] : -INFINITY,
+                     at + 3 < end ? row[at + 3] : -INFINITY);
 }
-// PER_THREAD logits of a run of `count`; -inf beyond them.
-template <bool IN_ORDER>
+// 2^x, the hardware approximation
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A run's logits of this thread.
 __device__ __forceinline__ void load_run(const float* run, int count, float (&v)[PER_THREAD]) {
   const bool aligned = ((uintptr_t)run & 15) == 0;
 #pragma unroll
   for (int i = 0; i < PER_THREAD; i += 4) {
-    const int at = place_of<IN_ORDER>(i);
-    if (aligned && at + 4 <= count) {
-      const float4 t = *(const float4*)(run + at);
-      v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; k++) v[i + k] = at + k < count ? run[at + k] : -INFINITY;
-    }
+    const float4 t = load_four(run, place_of(i), count, aligned);
+    v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
   }
 }
 
-struct Rows {
+// What verify_decide_kernel leaves for a request's draw.
+struct Chosen {
+  int row;                                             // of the logits, -1: nothing is drawn
+  int draft_row;                                       // whose probabilities are taken away, -1: none
+  int without;                                         // a token that is left out, -1: none
+  float top, top_q;                                    // the rows' maxima
+  int pad;
+  double c, rho;                                       // log2(e) / T; the ratio of the rows' sums, from the float32 ones
+};
+
+// 64-bit sums of a run of the row that is drawn from: the exponentials of the target's and the draft's logits, and both again over the
+// tokens where the difference is positive.
+struct Sums { double a, b, above_a, above_b; };
+
+struct Args {
   const float* logits; const float* draft_logits;      // [rows, vocab], [draft_rows, vocab]
   long long ld, draft_ld;
   const int* row_start; const float* temperature;      // [requests + 1], [requests] (null: 0)
-  RunSum* sums;                                        // [rows + draft_rows, runs]
-  int rows, draft_rows, requests, vocab, runs;
+  const int* drafts; const float* accept; const float* draw;      // [rows]
+  int* out; int* accepted; int* status;                // [rows], [requests]
+  RunSum* runs;                                        // [rows + draft_rows, per_row]
+  Chosen* chosen; Sums* sums;                          // [requests], [requests, per_row]
+  int rows, draft_rows, requests, vocab, per_row;      // per_row: runs of a row
+  int items;                                           // runs that a block of the first kernel takes
 };
 
-__global__ void __launch_bounds__(THREADS)
-verify_rows_kernel(const Rows p) {
+__global__ void __launch_bounds__(THREADS, ROW_BLOCKS)
+verify_rows_kernel(const Args p) {
   __shared__ float s_val[WARPS];
   __shared__ int s_idx[WARPS];
   __shared__ double s_sum[WARPS];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / p.runs, run = blockIdx.x % p.runs;
-  const bool draft = row >= p.rows;
-  const int own = draft ? row - p.rows : row;
-  const float* base = draft ? p.draft_logits + (size_t)own * p.draft_ld : p.logits + (size_t)own * p.ld;
-  // the row's request: the last whose rows (draft rows: one fewer per request before) begin at or before it
-  int lo = 0, hi = p.requests - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.row_start[mid] - (draft ? mid : 0) <= own) lo = mid; else hi = mid - 1;
-  }
-  const float temp = p.temperature ? p.temperature[lo] : 0.f;
-  if (draft && !(temp > 0.f)) return;                  // a greedy request's draft probabilities are not asked for
-  const int begin = run * RUN, count = min(RUN, p.vocab - begin);
-  float v[PER_THREAD];
-  load_run<false>(base + begin, count, v);
-  float best = -INFINITY;
-  int best_i = 0x7fffffff, bad = 0;
+  const long long all = (long long)(p.rows + p.draft_rows) * p.per_row, first = (long long)blockIdx.x * p.items, end = min(first + p.items, all);
+  int row = (int)(first / p.per_row), run = (int)(first % p.per_row), known = -1;
+  auto fetch = [&](int row, int run, float (&v)[PER_THREAD]) {
+    const float* base = row >= p.rows ? p.draft_logits + (size_t)(row - p.rows) * p.draft_ld : p.logits + (size_t)row * p.ld;
+    load_run(base + run * RUN, min(RUN, p.vocab - run * RUN), v);
+  };
+  float next[PER_THREAD];
+  if (first < end) fetch(row, run, next);
+  float temp = 0.f;
+  for (long long item = first; item < end; item++) {
+    float v[PER_THREAD];
 #pragma unroll
-  for (int i = 0; i < PER_THREAD; i++) {
-    const int at = place_of<false>(i);
-    if (at < count && !isfinite(v[i])) bad = 1;
-    if (v[i] > best) { best = v[i]; best_i = begin + at; }         // places rise with i: the first maximum stays
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) better(best, best_i, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_i, o));
-  if (lane == 0) { s_val[warp] = best; s_idx[warp] = best_i; }
-  bad = __syncthreads_or(bad);
-  best = s_val[0]; best_i = s_idx[0];
-#pragma unroll
-  for (int w = 1; w < WARPS; w++) better(best, best_i, s_val[w], s_idx[w]);
-  double sum = 0.0;
-  if (temp > 0.f && !bad) {
-    const double c = 1.4426950408889634 / (double)temp, top = (double)best;
+    for (int i = 0; i < PER_THREAD; i++) v[i] = next[i];
+    const int at_row = row, at_run = run, begin = run * RUN, count = min(RUN, p.vocab - begin);
+    const bool draft = row >= p.rows;
+    if (++run == p.per_row) { run = 0; row++; }
+    if (item + 1 < end) fetch(row, run, next);         // on its way while this run is added up
+    if (at_row != known) {
+      // the row's request: the last whose rows (draft rows: one fewer per request before) begin at or before it; a warp asks 32
+      // places at once
+      const int own = draft ? at_row - p.rows : at_row;
+      int lo = 0;
+      for (int n = p.requests; n > 1;) {
+        const int step = (n + 31) / 32, i = lo + lane * step;
+        const bool before = lane * step < n && p.row_start[i] - (draft ? i : 0) <= own;
+        const int last = max(0, 31 - __clz(__ballot_sync(0xffffffffu, before)));
+        n = min(step, n - last * step);
+        lo += last * step;
+      }
+      temp = p.temperature ? p.temperature[lo] : 0.f;
+      known = at_row;
+    }
+    const bool greedy = !(temp > 0.f);
+    if (draft && greedy) continue;                     // a greedy request's draft probabilities are not asked for
+    float best = -INFINITY;
+    bool bad = false;
 #pragma unroll
     for (int i = 0; i < PER_THREAD; i++) {
-      const double e = pow2(((double)v[i] - top) * c);             // the difference first: it is exact next to the maximum, whatever T
-      if (place_of<false>(i) < count) sum += e;
+      best = fmaxf(best, v[i]);
+      bad |= !(fabsf(v[i]) < INFINITY);
     }
-    sum = warp_sum_d(sum);
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    sum = s_sum[0];
+    if (count < RUN) {                                 // beyond the vocabulary: not what was read
+      bad = false;
 #pragma unroll
-    for (int w = 1; w < WARPS; w++) sum += s_sum[w];
+      for (int i = 0; i < PER_THREAD; i++) bad |= place_of(i) < count && !(fabsf(v[i]) < INFINITY);
+    }
+    best = warp_max(best);
+    if (lane == 0) s_val[warp] = best;
+    bad = __syncthreads_or(bad);
+    best = s_val[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) best = fmaxf(best, s_val[w]);
+    int index = 0x7fffffff;
+    double sum = 0.0;
+    if (greedy) {
+#pragma unroll
+      for (int i = PER_THREAD - 1; i >= 0; i--) if (v[i] == best) index = begin + place_of(i);      // places rise with i
+      index = __reduce_min_sync(0xffffffffu, index);
+      if (lane == 0) s_idx[warp] = index;
+    } else if (!bad) {
+      // a product in two floats: the rounding of log2(e) / T would shift all weights alike, by 1e-7
+      const double c = 1.4426950408889634 / (double)temp;
+      const float c_hi = (float)c, c_lo = isinf(c_hi) ? 0.f : (float)(c - (double)c_hi);
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < PER_THREAD; i++) {
+        const float d = v[i] - best, y = fmaxf(fmaf(d, c_hi, d * c_lo), -200.f);      // -200: also where infinities meet
+        const float e = d == 0.f ? 1.f : exp2_fast(y);                       // 0 times an infinite 1 / T
+        sums[i & 3] += count == RUN || place_of(i) < count ? e : 0.f;
+      }
+      sum = warp_sum_d(((double)sums[0] + (double)sums[1]) + ((double)sums[2] + (double)sums[3]));
+      if (lane == 0) s_sum[warp] = sum;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      if (greedy) {
+        for (int w = 0; w < WARPS; w++) index = min(index, s_idx[w]);
+      } else if (!bad) {
+        sum = s_sum[0];
+        for (int w = 1; w < WARPS; w++) sum += s_sum[w];
+      }
+      p.runs[(size_t)at_row * p.per_row + at_run] = RunSum{sum, best, index, bad, 0};
+    }
   }
-  if (tid == 0) p.sums[(size_t)row * p.runs + run] = RunSum{sum, best, best_i, bad, 0};
 }
-
-struct Pick {
-  Rows rows;
-  const int* drafts; const float* accept; const float* draw;      // [rows]
-  int* out; int* accepted; int* status;                           // [rows], [requests]
-};
 
 // What a row's runs add up to: its maximum, first index and (with `sums`) sum relative to the maximum, in every lane of the warp.
 struct RowSum { double sum; float max; int index; int bad; };
@@ -172,89 +230,50 @@ __device__ __forceinline__ RowSum merge_runs(const RunSum* runs, int count, bool
   return RowSum{warp_sum_d(sum), best, best_i, bad};
 }
 
-// The lowest place of a block's weights (PER_THREAD a thread, side by side) whose running sum, counted from `before`, exceeds `target`;
-// the last with any weight where rounding left none.  -1 where nothing has weight.  `s_sum` [WARPS], `s_pick` [2] are shared.
-__device__ __forceinline__ int pick_place(const double (&w)[PER_THREAD], double before, double target, double* s_sum, int* s_pick) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  double own = 0.0;
-#pragma unroll
-  for (int i = 0; i < PER_THREAD; i++) own += w[i];
-  double upto = own;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double other = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += other;
-  }
-  __syncthreads();                                     // what these held has been read
-  if (lane == 31) s_sum[warp] = upto;
-  if (tid == 0) { s_pick[0] = 0x7fffffff; s_pick[1] = -1; }
-  __syncthreads();
-  double running = before;
-  for (int i = 0; i < warp; i++) running += s_sum[i];
-  running += upto - own;
-  int first = 0x7fffffff, last = -1;
-#pragma unroll
-  for (int i = 0; i < PER_THREAD; i++) {
-    running += w[i];
-    if (w[i] > 0.0) {
-      last = tid * PER_THREAD + i;
-      if (running > target && first == 0x7fffffff) first = last;
-    }
-  }
-  if (first != 0x7fffffff) atomicMin(&s_pick[0], first);
-  if (last >= 0) atomicMax(&s_pick[1], last);
-  __syncthreads();
-  return s_pick[0] != 0x7fffffff ? s_pick[0] : s_pick[1];
-}
-
-__global__ void __cluster_dims__(CTAS, 1, 1) __launch_bounds__(THREADS)
-verify_pick_kernel(const Pick p) {
+__global__ void __launch_bounds__(THREADS)
+verify_decide_kernel(const Args p) {
   __shared__ double s_z[WARPS], s_zq[WARPS];
   __shared__ float s_m[WARPS], s_mq[WARPS];
   __shared__ int s_best[WARPS], s_code[WARPS];         // per row of a batch: 0 stands, 1 does not, 2 and more: flagged
-  __shared__ double s_sum[WARPS], s_total[CTAS];
-  __shared__ int s_pick[2], s_choice;
-  __shared__ double s_before, s_target;
   pdl_launch_dependents();
   pdl_wait();
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), r = blockIdx.x / CTAS;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Rows& a = p.rows;
-  const int first = a.row_start[r], end = a.row_start[r + 1], count = end - first;
-  // every CTA of the cluster takes the same decisions from the same numbers, up to where the cluster's CTAs part
-  if (first < 0 || end > a.rows || count < 1 || (a.draft_rows > 0 && (first - r < 0 || end - r - 1 > a.draft_rows))) {
-    if (rank == 0 && tid == 0) { atomicOr(p.status, SPROUT_STATUS_BAD_ROWS); p.accepted[r] = -1; }
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int first = p.row_start[r], end = p.row_start[r + 1], count = end - first;
+  if (first < 0 || end > p.rows || end <= first || (p.draft_rows > 0 && (first - r < 0 || end - r - 1 > p.draft_rows))) {
+    if (tid == 0) { atomicOr(p.status, SPROUT_STATUS_BAD_ROWS); p.accepted[r] = -1; p.chosen[r].row = -1; }
     return;
   }
-  const float temp = a.temperature ? a.temperature[r] : 0.f;
+  const float temp = p.temperature ? p.temperature[r] : 0.f;
   const bool greedy = !(temp > 0.f);
   const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temp;
   int row = 0, code = 0;
   for (int base = 0; base < count; base += WARPS) {
     const int i = base + warp;
     if (i < count) {
-      const RowSum s = merge_runs(a.sums + (size_t)(first + i) * a.runs, a.runs, !greedy, c);
+      const int x = i < count - 1 ? p.drafts[first + i] : 0, d = first - r + i;
+      const bool token = x >= 0 && x < p.vocab, model = p.draft_rows > 0 && i < count - 1;
+      const float u = greedy ? 0.f : p.accept[first + i];
+      // asked for before the runs are merged: a read that waits for another
+      const float lx = token ? p.logits[(size_t)(first + i) * p.ld + x] : 0.f, dx = token && model && !greedy ? p.draft_logits[(size_t)d * p.draft_ld + x] : 0.f;
+      const RowSum s = merge_runs(p.runs + (size_t)(first + i) * p.per_row, p.per_row, !greedy, c);
       int verdict = s.bad ? SPROUT_STATUS_NONFINITE : 1;           // the last row never "stands": the draw is made there
       double zq = 0.0;
       float mq = 0.f;
       if (i < count - 1 && !s.bad) {
-        const int x = p.drafts[first + i];
-        if (x < 0 || x >= a.vocab) {
+        if (!token) {
           verdict = SPROUT_STATUS_BAD_TOKEN;
         } else if (greedy) {
           verdict = x == s.index ? 0 : 1;
         } else {
-          const double px = pow2(((double)a.logits[(size_t)(first + i) * a.ld + x] - (double)s.max) * c) / s.sum;
+          const double px = pow2(((double)lx - (double)s.max) * c) / s.sum;
           double qx = 1.0;
-          if (a.draft_rows > 0) {
-            const int d = first - r + i;
-            const RowSum t = merge_runs(a.sums + (size_t)(a.rows + d) * a.runs, a.runs, !greedy, c);
+          if (model) {
+            const RowSum t = merge_runs(p.runs + (size_t)(p.rows + d) * p.per_row, p.per_row, true, c);
             if (t.bad) verdict = SPROUT_STATUS_NONFINITE;
             zq = t.sum; mq = t.max;
-            qx = pow2(((double)a.draft_logits[(size_t)d * a.draft_ld + x] - (double)mq) * c) / zq;
+            qx = pow2(((double)dx - (double)mq) * c) / zq;
           }
-          if (verdict == 1) verdict = (double)p.accept[first + i] * qx < px ? 0 : 1;
+          if (verdict == 1) verdict = (double)u * qx < px ? 0 : 1;
         }
       }
       if (lane == 0) { s_z[warp] = s.sum; s_m[warp] = s.max; s_best[warp] = s.index; s_zq[warp] = zq; s_mq[warp] = mq; s_code[warp] = verdict; }
@@ -267,159 +286,182 @@ verify_pick_kernel(const Pick p) {
     __syncthreads();
   }
   const int slot = row % WARPS;                        // batches start at multiples of WARPS
-  if (rank == 0) {
-    for (int i = tid; i < count; i += THREADS)
-      if (i != row || code > 1) p.out[first + i] = i < row ? p.drafts[first + i] : -1;
-    if (tid == 0) {
-      p.accepted[r] = row;
-      if (code > 1) atomicOr(p.status, code);
-    }
+  const bool draws = code <= 1 && !greedy, fell = row < count - 1;
+  for (int i = tid; i < count; i += THREADS)
+    if (i != row || !draws) p.out[first + i] = i < row ? p.drafts[first + i] : i == row && code <= 1 ? s_best[slot] : -1;
+  if (tid == 0) {
+    p.accepted[r] = row;
+    if (code > 1) atomicOr(p.status, code);
+    const bool difference = fell && p.draft_rows > 0;
+    p.chosen[r] = Chosen{draws ? first + row : -1, difference ? first - r + row : -1, fell && !difference ? p.drafts[first + row] : -1,
+                         s_m[slot], s_mq[slot], 0, c, difference ? s_zq[slot] / s_z[slot] : 0.0};
   }
-  if (code > 1) return;
-  if (greedy) {
-    if (rank == 0 && tid == 0) p.out[first + row] = s_best[slot];
-    return;
-  }
-  const float* logits = a.logits + (size_t)(first + row) * a.ld;
-  const float max_p = s_m[slot];
-  const double z = s_z[slot], top = (double)max_p, draw = (double)p.draw[first + row];
-  const bool take_away = row < count - 1;              // max(p - q, 0) instead of p
-  double w[PER_THREAD];
-  if (take_away && a.draft_rows > 0) {
-    // the difference, over a share of the runs in every CTA
-    const float* draft = a.draft_logits + (size_t)(first - r + row) * a.draft_ld;
-    const double top_q = (double)s_mq[slot], inv_z = 1.0 / z, inv_zq = 1.0 / s_zq[slot];
-    const int share = (a.runs + CTAS - 1) / CTAS, run0 = min(rank * share, a.runs), run1 = min(run0 + share, a.runs);
-    auto difference = [&](int run) {
-      float v[PER_THREAD], d[PER_THREAD];
-      const int begin = run * RUN, n = min(RUN, a.vocab - begin);
-      load_run<true>(logits + begin, n, v);
-      load_run<true>(draft + begin, n, d);
-      double sum = 0.0;
+}
+
+__global__ void __launch_bounds__(THREADS)
+verify_sums_kernel(const Args p) {
+  __shared__ Sums s_sums[WARPS];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = blockIdx.x / p.per_row, run = blockIdx.x % p.per_row;
+  const Chosen at = p.chosen[r];
+  if (at.row < 0) return;
+  const int begin = run * RUN, count = min(RUN, p.vocab - begin);
+  const bool difference = at.draft_row >= 0;
+  float v[PER_THREAD], d[PER_THREAD];
+  load_run(p.logits + (size_t)at.row * p.ld + begin, count, v);
+  if (difference) load_run(p.draft_logits + (size_t)at.draft_row * p.draft_ld + begin, count, d);
+  const double top = (double)at.top, top_q = (double)at.top_q;
+  Sums sum = {0.0, 0.0, 0.0, 0.0};
+  if (difference) {
 #pragma unroll
-      for (int i = 0; i < PER_THREAD; i++) {
-        const double e = pow2(((double)v[i] - top) * c) * inv_z - pow2(((double)d[i] - top_q) * c) * inv_zq;
-        w[i] = tid * PER_THREAD + i < n ? fmax(e, 0.0) : 0.0;
-        sum += w[i];
+    for (int i = 0; i < PER_THREAD; i++) {
+      const double ea = pow2(((double)v[i] - top) * at.c), eb = pow2(((double)d[i] - top_q) * at.c);
+      if (count == RUN || place_of(i) < count) {
+        sum.a += ea;
+        sum.b += eb;
+        if (ea * at.rho > eb) { sum.above_a += ea; sum.above_b += eb; }
       }
-      return sum;
-    };
-    auto block_total = [&](double sum) {
-      sum = warp_sum_d(sum);
-      __syncthreads();
-      if (lane == 0) s_sum[warp] = sum;
-      __syncthreads();
-      sum = s_sum[0];
+    }
+    sum.b = warp_sum_d(sum.b);
+    sum.above_a = warp_sum_d(sum.above_a);
+    sum.above_b = warp_sum_d(sum.above_b);
+  } else {
 #pragma unroll
-      for (int i = 1; i < WARPS; i++) sum += s_sum[i];
-      return sum;
-    };
-    double mine = 0.0;
-    for (int run = run0; run < run1; run++) mine += difference(run);
-    mine = block_total(mine);
-    cluster.sync();                                    // every CTA of the cluster runs: its shared memory may be written
-    if (tid < CTAS) *cluster.map_shared_rank(&s_total[rank], tid) = mine;
-    cluster.sync();
-    double total = 0.0, before = 0.0;
-    int owner = -1, last = -1;
-    for (int i = 0; i < CTAS; i++) total += s_total[i];
-    const double target = draw * total;
-    double sum = 0.0;
-    for (int i = 0; i < CTAS; i++) {
-      if (s_total[i] > 0.0) last = i;
-      if (owner < 0 && sum + s_total[i] > target) { owner = i; before = sum; }
-      sum += s_total[i];
+    for (int i = 0; i < PER_THREAD; i++) {
+      const double ea = pow2(((double)v[i] - top) * at.c);
+      if ((count == RUN || place_of(i) < count) && begin + place_of(i) != at.without) sum.a += ea;
     }
-    if (owner < 0 && last >= 0) {                      // rounding: the last share with any weight
-      owner = last;
-      before = 0.0;
-      for (int i = 0; i < last; i++) before += s_total[i];
-    }
-    if (owner >= 0) {
-      if (rank != owner) return;
-      int chosen = -1;
-      double at = before;
-      bool falls = false;
-      for (int run = run0; run < run1 && !falls; run++) {
-        const double in_run = block_total(difference(run));
-        if (!(in_run > 0.0)) continue;
-        chosen = run;
-        before = at;
-        at += in_run;
-        falls = at > target;
-      }
-      if (!falls) difference(chosen);                  // rounding: the last run with any weight
-      const int place = pick_place(w, before, target, s_sum, s_pick);
-      if (tid == 0) p.out[first + row] = chosen * RUN + place;
-      return;
-    }
-    // p and q are the same everywhere (then nothing is rejected but by rounding): drawn from p
   }
-  if (rank != 0) return;
-  // from p, less the drafted token where it was rejected and nothing else was drafted with any probability
-  const int without = take_away && a.draft_rows == 0 ? p.drafts[first + row] : -1;
-  const RunSum* runs = a.sums + (size_t)(first + row) * a.runs;
+  sum.a = warp_sum_d(sum.a);
+  if (lane == 0) s_sums[warp] = sum;
+  __syncthreads();
+  if (tid < 4) {                                       // a thread per sum
+    double total = 0.0;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) total += ((const double*)&s_sums[w])[tid];
+    ((double*)&p.sums[(size_t)r * p.per_row + run])[tid] = total;
+  }
+}
+
+__global__ void __launch_bounds__(DRAW_THREADS)
+verify_draw_kernel(const Args p) {
+  __shared__ double s_sum[DRAW_WARPS], s_before, s_target, s_rho;
+  __shared__ int s_run, s_from_p, s_first, s_last;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Chosen at = p.chosen[r];
+  if (at.row < 0) return;
+  const Sums* sums = p.sums + (size_t)r * p.per_row;
   if (warp == 0) {
-    // the runs' weights relative to the row's maximum, a lane each, in order
-    auto weight = [&](int i, int skip) {
-      if (i >= a.runs) return 0.0;
-      double s = runs[i].sum;
-      if (skip >= 0 && skip / RUN == i) s = fmax(0.0, s - pow2(((double)logits[skip] - (double)runs[i].max) * c));
-      return s * pow2(((double)runs[i].max - top) * c);
-    };
-    auto sum_of = [&](int skip) {
-      double s = 0.0;
-      for (int i = lane; i < a.runs; i += 32) s += weight(i, skip);
-      return warp_sum_d(s);
-    };
-    int skip = without;
-    double total = sum_of(skip);
-    if (!(total > 0.0)) {                              // the drafted token has all the weight there is: drawn from p
-      skip = -1;
-      total = z;
+    // the run in which the draw falls, a lane a run
+    double rho = 1.0, total = 0.0;
+    bool from_p = at.draft_row < 0;
+    if (!from_p) {
+      double za = 0.0, zb = 0.0;
+      for (int i = lane; i < p.per_row; i += 32) { za += sums[i].a; zb += sums[i].b; }
+      rho = warp_sum_d(zb) / warp_sum_d(za);
     }
-    const double target = draw * total;
-    double at = 0.0, before = 0.0;
-    int chosen = -1;
+    auto weight = [&](int i) { return i >= p.per_row ? 0.0 : from_p ? sums[i].a : fmax(0.0, fma(sums[i].above_a, rho, -sums[i].above_b)); };
+    for (int attempt = 0; attempt < 2; attempt++) {
+      total = 0.0;
+      for (int i = lane; i < p.per_row; i += 32) total += weight(i);
+      total = warp_sum_d(total);
+      if (from_p || total > 0.0) break;
+      from_p = true;                                   // p and q are the same everywhere (what falls then fell by rounding): drawn from p
+    }
+    const double target = (double)p.draw[at.row] * total;
+    double passed = 0.0, before = 0.0;
+    int run = -1;                                      // stays so where the token that is left out has all the weight there is
     bool falls = false;
-    for (int base = 0; base < a.runs && !falls; base += 32) {
-      const double s = weight(base + lane, skip);
-      double upto = s;
+    for (int base = 0; base < p.per_row && !falls; base += 32) {
+      const double w = weight(base + lane);
+      double upto = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double other = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += other;
       }
-      const unsigned any = __ballot_sync(0xffffffffu, s > 0.0), over = __ballot_sync(0xffffffffu, s > 0.0 && at + upto > target);
+      const unsigned any = __ballot_sync(0xffffffffu, w > 0.0), over = __ballot_sync(0xffffffffu, w > 0.0 && passed + upto > target);
       if (any) {                                       // the first run that passes the target, or (so far) the last with any weight
         falls = over != 0;
         const int l = falls ? __ffs(over) - 1 : 31 - __clz(any);
-        chosen = base + l;
-        before = __shfl_sync(0xffffffffu, at + upto - s, l);
+        run = base + l;
+        before = __shfl_sync(0xffffffffu, passed + upto - w, l);
       }
-      at += __shfl_sync(0xffffffffu, upto, 31);
+      passed += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (lane == 0) { s_choice = chosen; s_before = before; s_target = target; s_pick[0] = skip; }
+    if (lane == 0) { s_run = run; s_before = before; s_target = target; s_rho = rho; s_from_p = from_p; s_first = 0x7fffffff; s_last = -1; }
   }
   __syncthreads();
-  const int run = s_choice, skip = s_pick[0];
-  __syncthreads();
-  float v[PER_THREAD];
-  const int begin = run * RUN, n = min(RUN, a.vocab - begin);
-  load_run<true>(logits + begin, n, v);
+  const int run = s_run;
+  if (run < 0) {
+    if (tid == 0) p.out[at.row] = at.without;
+    return;
+  }
+  const bool from_p = s_from_p != 0;
+  const double top = (double)at.top, top_q = (double)at.top_q, rho = s_rho, target = s_target;
+  const int begin = run * RUN, count = min(RUN, p.vocab - begin);
+  const float* logits = p.logits + (size_t)at.row * p.ld + begin;
+  const float* draft = from_p ? nullptr : p.draft_logits + (size_t)at.draft_row * p.draft_ld + begin;
+  const bool aligned = ((uintptr_t)logits & 15) == 0, aligned_q = ((uintptr_t)draft & 15) == 0;
+  float v[DRAW_LOGITS], d[DRAW_LOGITS];
 #pragma unroll
-  for (int i = 0; i < PER_THREAD; i++) {
-    const int at = tid * PER_THREAD + i;
-    w[i] = at < n && begin + at != skip ? pow2(((double)v[i] - top) * c) : 0.0;
+  for (int i = 0; i < DRAW_LOGITS; i += 4) {           // side by side in every thread
+    const int place = tid * DRAW_LOGITS + i;
+    const float4 t = load_four(logits, place, count, aligned), q = from_p ? t : load_four(draft, place, count, aligned_q);
+    v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
+    d[i] = q.x; d[i + 1] = q.y; d[i + 2] = q.z; d[i + 3] = q.w;
   }
-  const int place = pick_place(w, s_before, s_target, s_sum, s_pick);
-  if (tid == 0) p.out[first + row] = place >= 0 ? begin + place : s_best[slot];
+  double w[DRAW_LOGITS], own = 0.0;
+#pragma unroll
+  for (int i = 0; i < DRAW_LOGITS; i++) {
+    const int place = tid * DRAW_LOGITS + i;
+    double e = pow2(((double)v[i] - top) * at.c);
+    if (!from_p) e = fmax(0.0, fma(e, rho, -pow2(((double)d[i] - top_q) * at.c)));
+    w[i] = place < count && begin + place != at.without ? e : 0.0;
+    own += w[i];
+  }
+  double sum = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double other = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += other;
+  }
+  if (lane == 31) s_sum[warp] = sum;
+  __syncthreads();
+  double running = s_before;
+  for (int i = 0; i < warp; i++) running += s_sum[i];
+  running += sum - own;
+  int first = 0x7fffffff, last = -1;
+#pragma unroll
+  for (int i = 0; i < DRAW_LOGITS; i++) {
+    running += w[i];
+    if (w[i] > 0.0) {
+      last = begin + tid * DRAW_LOGITS + i;
+      if (running > target && first == 0x7fffffff) first = last;
+    }
+  }
+  if (first != 0x7fffffff) atomicMin(&s_first, first);
+  if (last >= 0) atomicMax(&s_last, last);
+  __syncthreads();
+  if (tid == 0) p.out[at.row] = s_first != 0x7fffffff ? s_first : s_last;      // none by rounding: the last with any weight
 }
 
 }  // namespace
 
-// Bytes of scratch for `rows` rows (target's and draft's together) of `vocab` logits.
-SPROUT_API long long sprout_verify_scratch_bytes(int rows, int vocab) { return (long long)rows * ((vocab + RUN - 1) / RUN) * (long long)sizeof(RunSum); }
+namespace {
+int runs_of(int vocab) { return (vocab + RUN - 1) / RUN; }
+long long aligned16(long long bytes) { return (bytes + 15) & ~15LL; }
+}  // namespace
+
+// Bytes of scratch, 16-byte aligned, for `rows` rows (target's and draft's together) of `vocab` logits.
+SPROUT_API long long sprout_verify_scratch_bytes(int rows, int requests, int vocab) {
+  const long long per_row = runs_of(vocab);
+  return aligned16(rows * per_row * (long long)sizeof(RunSum)) + aligned16(requests * (long long)sizeof(Chosen)) + requests * per_row * (long long)sizeof(Sums);
+}
 
 // Request r's rows are row_start[r] .. row_start[r + 1] - 1 of `logits` [rows, vocab], at least one; its draft rows, one fewer, begin at
 // row_start[r] - r of `draft_logits` (null with draft_rows 0: the drafts have no distribution).  temperature, accept and draw may be null
@@ -427,17 +469,29 @@ SPROUT_API long long sprout_verify_scratch_bytes(int rows, int vocab) { return (
 SPROUT_API int sprout_verify(const float* logits, long long ld, const float* draft_logits, long long draft_ld, const int* drafts, const int* row_start,
                              const float* temperature, const float* accept, const float* draw, int* out, int* accepted, void* scratch,
                              int rows, int draft_rows, int requests, int vocab, int* status, cudaStream_t stream) {
-  SPROUT_REQUIRE(rows > 0 && requests > 0 && requests <= rows && vocab > 0 && ld >= 0, "verify: bad sizes rows=%d requests=%d vocab=%d ld=%lld", rows, requests, vocab, ld);
+  SPROUT_REQUIRE(rows > 0 && requests > 0 && requests <= rows && vocab > 0 && vocab <= 1 << 30 && ld >= 0, "verify: bad sizes rows=%d requests=%d vocab=%d ld=%lld", rows, requests, vocab, ld);
   SPROUT_REQUIRE(draft_rows == 0 || (draft_rows == rows - requests && draft_logits && draft_ld >= 0), "verify: a draft row per drafted token");
   SPROUT_REQUIRE(logits && drafts && row_start && out && accepted && scratch && status, "verify: null pointer");
   SPROUT_REQUIRE((temperature == nullptr) == (accept == nullptr) && (accept == nullptr) == (draw == nullptr), "verify: temperatures and both kinds of uniform numbers go together");
-  const int runs = (vocab + RUN - 1) / RUN;
-  SPROUT_REQUIRE((long long)runs * (rows + (long long)draft_rows) <= 0x7fffffffLL && (long long)requests * CTAS <= 0x7fffffffLL, "verify: too many rows");
-  Pick p;
-  p.rows = Rows{logits, draft_logits, ld, draft_ld, row_start, temperature, (RunSum*)scratch, rows, draft_rows, requests, vocab, runs};
-  p.drafts = drafts; p.accept = accept; p.draw = draw; p.out = out; p.accepted = accepted; p.status = status;
-  sprout_launch(verify_rows_kernel, dim3(runs * (rows + draft_rows)), dim3(THREADS), 0, stream, p.rows);
+  const long long per_row = runs_of(vocab), all = per_row * (rows + (long long)draft_rows);
+  SPROUT_REQUIRE(rows + (long long)draft_rows <= 0x7fffffffLL && per_row * requests <= 0x7fffffffLL, "verify: too many rows");
+  Args p{logits, draft_logits, ld, draft_ld, row_start, temperature, drafts, accept, draw, out, accepted, status, nullptr, nullptr, nullptr,
+         rows, draft_rows, requests, vocab, (int)per_row, 0};
+  uint8_t* at = (uint8_t*)scratch;
+  p.runs = (RunSum*)at;
+  at += aligned16(all * (long long)sizeof(RunSum));
+  p.chosen = (Chosen*)at;
+  at += aligned16(requests * (long long)sizeof(Chosen));
+  p.sums = (Sums*)at;
+  const long long blocks = (long long)ROW_BLOCKS * sprout_sm_count(), items = (all + blocks - 1) / blocks;
+  SPROUT_REQUIRE(items <= 0x7fffffffLL, "verify: too many rows");
+  p.items = (int)items;
+  sprout_launch(verify_rows_kernel, dim3((unsigned)((all + items - 1) / items)), dim3(THREADS), 0, stream, p);
   if (sprout_check_launch("verify_rows")) return 1;
-  sprout_launch(verify_pick_kernel, dim3(requests * CTAS), dim3(THREADS), 0, stream, p);
-  return sprout_check_launch("verify_pick");
+  sprout_launch(verify_decide_kernel, dim3(requests), dim3(THREADS), 0, stream, p);
+  if (sprout_check_launch("verify_decide") || temperature == nullptr) return sprout_check_launch("verify_decide");
+  sprout_launch(verify_sums_kernel, dim3((unsigned)(per_row * requests)), dim3(THREADS), 0, stream, p);
+  if (sprout_check_launch("verify_sums")) return 1;
+  sprout_launch(verify_draw_kernel, dim3(requests), dim3(DRAW_THREADS), 0, stream, p);
+  return sprout_check_launch("verify_draw");
 }

@@ -130,7 +130,7 @@ def load_library(verbose: bool = True):
             lib.sprout_sample_scratch_bytes.restype = ctypes.c_longlong
             lib.sprout_sample_scratch_bytes.argtypes = [c_int]
             lib.sprout_verify_scratch_bytes.restype = ctypes.c_longlong
-            lib.sprout_verify_scratch_bytes.argtypes = [c_int, c_int]
+            lib.sprout_verify_scratch_bytes.argtypes = [c_int, c_int, c_int]
             lib.sprout_delta_scratch_floats.restype = ctypes.c_longlong
             lib.sprout_maps_attention_tc_scratch_floats.restype = ctypes.c_longlong
             lib.sprout_maps_attention_tc_scratch_floats.argtypes = [c_int] * 6
@@ -973,15 +973,13 @@ def sample(logits, out, status, temperature=None, uniform=None):
          _ptr(out, "out", torch.int32), _ptr(scratch, "scratch"), R, V, _ptr(status, "status", torch.int32), _stream())
 
 
-def _one_device(name, **tensors):
-    """All tensors (None: not given) on one CUDA device, the current one."""
-    current = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for what, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise KernelError(f"{name}: {what} must be a CUDA tensor; there is no CPU path")
-        if t.device.index != current:
+def _one_device(name, tensors):
+    """All of the (what, tensor) pairs (None: not given) on one CUDA device, the current one."""
+    current = torch.cuda.current_device() if torch.cuda.is_available() else 0
+    for what, t in tensors:
+        if t is not None and t.get_device() != current:
+            if not t.is_cuda:
+                raise KernelError(f"{name}: {what} must be a CUDA tensor; there is no CPU path")
             raise KernelError(f"{name}: {what} is on {t.device}, the current device is cuda:{current}")
 
 
@@ -994,8 +992,8 @@ def _overlap(a, b) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def verify_drafts(logits, drafts, row_start, out, accepted, status, draft_logits=None, temperatures=None, accept=None, draw=None):
-    """Which drafted tokens stand against the target's probabilities, and the token after the last that does.
+def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperatures=None, accept=None, draw=None, out=None, accepted=None):
+    """Which drafted tokens stand against the target's probabilities, and the token after the last that does: ``(out, accepted)``.
 
     Request r has rows ``row_start[r]`` to ``row_start[r + 1] - 1`` (int32 [requests + 1]) of ``logits`` (float32 [rows, vocab]), one more
     than it has drafts: row i is what the target says at the place of its i-th draft, the last what it says behind all of them.
@@ -1008,44 +1006,47 @@ def verify_drafts(logits, drafts, row_start, out, accepted, status, draft_logits
     ties), then the argmax follows.
 
     ``out`` (int32 [rows]): the drafts that stand, the token after them, and -1 in the rest of the request's rows; ``accepted`` (int32
-    [requests]): how many stand.  A row that is reached and holds a non-finite logit, or a draft outside the vocabulary, sets a status bit
-    and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
+    [requests]): how many stand; both are made here unless given.  A row that is reached and holds a non-finite logit, or a draft outside
+    the vocabulary, sets a status bit and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
     name = "verify_drafts"
-    _one_device(name, logits=logits, drafts=drafts, row_start=row_start, out=out, accepted=accepted, status=status, draft_logits=draft_logits,
-                temperatures=temperatures, accept=accept, draw=draw)
+    _one_device(name, (("logits", logits), ("drafts", drafts), ("row_start", row_start), ("status", status), ("draft_logits", draft_logits),
+                       ("temperatures", temperatures), ("accept", accept), ("draw", draw), ("out", out), ("accepted", accepted)))
     _rows_contiguous(logits, "logits")
     rows, vocab = logits.shape
     requests = row_start.numel() - 1
     if rows < 1 or vocab < 1 or not 1 <= requests <= rows:
         raise KernelError(f"{name}: at least one request and a row for each (got {rows} rows of {vocab} logits for {requests} requests)")
     for what, t, n in (("drafts", drafts, rows), ("row_start", row_start, requests + 1), ("out", out, rows), ("accepted", accepted, requests)):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous()):
             raise KernelError(f"{name}: {what} must be contiguous int32 [{n}]")
     if (temperatures is None) != (accept is None) or (accept is None) != (draw is None):
         raise KernelError(f"{name}: temperatures, accept and draw go together")
     for what, t, n in (("temperatures", temperatures, requests), ("accept", accept, rows), ("draw", draw, rows)):
-        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous()):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
             raise KernelError(f"{name}: {what} must be contiguous float32 [{n}]")
+    draft_rows = 0
     if draft_logits is not None:
         _rows_contiguous(draft_logits, "draft_logits")
-        if tuple(draft_logits.shape) != (rows - requests, vocab):
-            raise KernelError(f"{name}: draft_logits must be [{rows - requests}, {vocab}], a row per draft (got {tuple(draft_logits.shape)})")
-        if rows == requests:
-            draft_logits = None                # nobody drafted anything
-    for what, t in (("out", out), ("accepted", accepted)):
-        for other, s in (("logits", logits), ("drafts", drafts), ("row_start", row_start), ("draft_logits", draft_logits), ("temperatures", temperatures),
-                         ("accept", accept), ("draw", draw), ("status", status)):
-            if s is not None and _overlap(t, s):
-                raise KernelError(f"{name}: {what} and {other} share memory")
-    if _overlap(out, accepted):
-        raise KernelError(f"{name}: out and accepted share memory")
-    draft_rows = rows - requests if draft_logits is not None else 0
-    scratch = torch.empty(load_library().sprout_verify_scratch_bytes(rows + draft_rows, vocab), dtype=torch.uint8, device=logits.device)
-    _run("sprout_verify", _ptr(logits, "logits", torch.float32), logits.stride(0), _ptr(draft_logits, "draft_logits", torch.float32, True),
-         draft_logits.stride(0) if draft_logits is not None else 0, _ptr(drafts, "drafts"), _ptr(row_start, "row_start"),
-         _ptr(temperatures, "temperatures", torch.float32, True), _ptr(accept, "accept", torch.float32, True), _ptr(draw, "draw", torch.float32, True),
-         _ptr(out, "out"), _ptr(accepted, "accepted"), _ptr(scratch, "scratch"), rows, draft_rows, requests, vocab,
-         _ptr(status, "status", torch.int32), _stream())
+        draft_rows = rows - requests                       # none where nobody drafted anything
+        if draft_logits.shape != (draft_rows, vocab):
+            raise KernelError(f"{name}: draft_logits must be [{draft_rows}, {vocab}], a row per draft (got {tuple(draft_logits.shape)})")
+    if out is not None or accepted is not None:
+        inputs = [(w, t) for w, t in (("logits", logits), ("drafts", drafts), ("row_start", row_start), ("draft_logits", draft_logits), ("status", status),
+                                      ("temperatures", temperatures), ("accept", accept), ("draw", draw)) if t is not None]
+        for what, t, others in (("out", out, inputs + [("accepted", accepted)]), ("accepted", accepted, inputs)):
+            for other, s in others:
+                if t is not None and s is not None and _overlap(t, s):
+                    raise KernelError(f"{name}: {what} and {other} share memory")
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    if accepted is None:
+        accepted = torch.empty(requests, dtype=torch.int32, device=logits.device)
+    scratch = torch.empty((_lib or load_library()).sprout_verify_scratch_bytes(rows + draft_rows, requests, vocab), dtype=torch.uint8, device=logits.device)
+    _run("sprout_verify", _ptr(logits, "logits", torch.float32), logits.stride(0), _ptr(draft_logits, "draft_logits", torch.float32, True) if draft_rows else None,
+         draft_logits.stride(0) if draft_rows else 0, drafts.data_ptr(), row_start.data_ptr(), temperatures.data_ptr() if temperatures is not None else None,
+         accept.data_ptr() if accept is not None else None, draw.data_ptr() if draw is not None else None, out.data_ptr(), accepted.data_ptr(),
+         scratch.data_ptr(), rows, draft_rows, requests, vocab, _ptr(status, "status", torch.int32), _stream())
+    return out, accepted
 
 
 def advance_decode(token_ids, positions, context_lens, sampled, history, step_counter):

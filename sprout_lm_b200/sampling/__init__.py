@@ -48,7 +48,4 @@ def verify(logits: torch.Tensor, drafts: torch.Tensor, row_start: torch.Tensor, 
     ``tokens`` has a place per row of ``logits``: a request's drafts that stand, the token drawn after them, then -1; ``accepted`` says
     how many stand.  What is emitted is distributed as if drawn from the target alone; a greedy request (temperature 0, or none given)
     gets the target's argmax at every place.  The arguments are those of ``kernels.verify_drafts`` (csrc/verify.cu), which this launches."""
-    tokens = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
-    accepted = torch.empty(max(row_start.numel() - 1, 0), dtype=torch.int32, device=logits.device)
-    kernels.verify_drafts(logits, drafts, row_start, tokens, accepted, status, draft_logits, temperatures, accept, draw)
-    return tokens, accepted
+    return kernels.verify_drafts(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw)

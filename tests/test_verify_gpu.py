@@ -191,6 +191,15 @@ def test_drafted_token_with_all_the_weight(status):
     assert (tokens, accepted) == ([77, -1], [0])
 
 
+@pytest.mark.parametrize("size", [1e3, 1e9, 3e38])
+def test_large_logits(size, status):
+    """Logits far from zero: the differences decide."""
+    c = case([3, 2, 0], 9000, seed=14)
+    for name in ("logits", "draft_logits"):
+        c[name] = (c[name] + np.float32(size)).astype(np.float32)
+    check(c, status)
+
+
 @pytest.mark.parametrize("temperature", [1e-38, 1e-3, 1e30, float("inf")])
 def test_extreme_temperatures(temperature, status):
     c = case([3, 2, 0], 5000, seed=4)
@@ -262,11 +271,11 @@ def test_rows_of_nobody_stay(status):
     out = torch.full((5,), 99, dtype=torch.int32, device=DEV)
     accepted = torch.full((1,), 99, dtype=torch.int32, device=DEV)
     more["temperatures"] = more["temperatures"][:1].contiguous()
-    kernels.verify_drafts(args[0], args[1], args[2][:2].contiguous(), out, accepted, status, **more)
+    kernels.verify_drafts(args[0], args[1], args[2][:2].contiguous(), status, out=out, accepted=accepted, **more)
     assert out[3:].tolist() == [99, 99] and accepted.tolist() != [99] and int(status.item()) == 0
     for start in ([0, 6], [-1, 3], [3, 3], [4, 2]):
         out.fill_(99)
-        kernels.verify_drafts(args[0], args[1], torch.tensor(start, dtype=torch.int32, device=DEV), out, accepted, status, **more)
+        kernels.verify_drafts(args[0], args[1], torch.tensor(start, dtype=torch.int32, device=DEV), status, out=out, accepted=accepted, **more)
         assert out.tolist() == [99] * 5 and accepted.tolist() == [-1] and int(status.item()) == 64
         status.zero_()
 
@@ -338,6 +347,7 @@ def test_refusals(status):
             kernels.verify_drafts(**given)
 
     refused("CUDA tensor", logits=args[0].cpu())
+    refused("must be torch.float32", draft_logits=more["draft_logits"].double())
     refused("must be torch.float32", logits=args[0].double())
     refused("unit inner stride", logits=args[0].t())
     refused("at least one request", row_start=args[2][:1])
