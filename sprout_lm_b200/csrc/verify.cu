@@ -17,9 +17,8 @@
 // logits (some 15 64-bit operations, two cycles each), 1.09 T a second, while memory delivers 1.6 T logits a second: only the row that is
 // drawn from takes them.  Whether a draft stands is decided by float32 exponentials, whose sums are good to 1e-8.
 //
-// Four launches.  verify_rows_kernel: every row in runs of RUN logits, their maxima and sums of exponentials (greedy: the maximum's
-// first index), a block walking a stretch of the rows' runs with the next run on its way.  verify_decide_kernel: a block per request
-// merges its rows' runs, a warp a row, and finds the first row that does not stand.  verify_sums_kernel: the 64-bit sums of that row's
+// Four launches.  verify_rows_kernel: every row in pieces of PIECE logits, a warp each, their maxima and sums of exponentials (greedy:
+// the maximum's first index).  verify_decide_kernel: a block per request merges its rows' pieces, a warp a row, and finds the first row that does not stand.  verify_sums_kernel: the 64-bit sums of that row's
 // runs, a block each.  verify_draw_kernel: a block per request finds the run in which the draw falls and looks through it.
 //
 // The difference in one pass: max(p - q, 0) needs both rows' sums before a single element of it is known.  With a_j, b_j the
@@ -32,10 +31,17 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int PER_THREAD = 16, RUN = THREADS * PER_THREAD;       // logits of a run
-constexpr int ROW_BLOCKS = 4;              // of the first kernel, an SM
+#ifndef VERIFY_ROWS
+#define VERIFY_ROWS 2
+#define VERIFY_ITEMS 8
+#define VERIFY_PIECE 1024
+#endif
+constexpr int ROW_BLOCKS = VERIFY_ROWS;    // of the first kernel, an SM
+constexpr int MAX_ITEMS = VERIFY_ITEMS;    // pieces that one of its warps takes
+constexpr int PIECE = VERIFY_PIECE;        // logits of a piece
 constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_LOGITS = RUN / DRAW_THREADS;
 
-struct RunSum { double sum; float max; int index; int bad; int pad; };       // sum: of 2^((v - max) log2(e) / T)
+struct PieceSum { double sum; float max; int index; int bad; int pad; };     // sum: of 2^((v - max) log2(e) / T)
 
 // 2^y for y <= 0 to 1e-12: y = k + f with |f| <= 1/2, 2^f by a polynomial through the Chebyshev nodes, k into the exponent.
 // Below 2^-1000 it is zero.
@@ -111,122 +117,134 @@ struct Args {
   const int* row_start; const float* temperature;      // [requests + 1], [requests] (null: 0)
   const int* drafts; const float* accept; const float* draw;      // [rows]
   int* out; int* accepted; int* status;                // [rows], [requests]
-  RunSum* runs;                                        // [rows + draft_rows, per_row]
-  Chosen* chosen; Sums* sums;                          // [requests], [requests, per_row]
-  int rows, draft_rows, requests, vocab, per_row;      // per_row: runs of a row
-  int items;                                           // runs that a block of the first kernel takes
+  PieceSum* pieces;                                    // [rows + draft_rows, per_row]
+  Chosen* chosen; Sums* sums;                          // [requests], [requests, runs]
+  int rows, draft_rows, requests, vocab, per_row, runs;            // pieces and runs of a row
+  int items;                                           // pieces that a warp of the first kernel takes
 };
 
+// The temperature of the request that row `row` (a draft row from p.rows on) belongs to: the last whose rows (draft rows: one fewer
+// per request before) begin at or before it.  A warp asks 32 places at once.
+__device__ __forceinline__ float temperature_of(const Args& p, int row) {
+  if (p.temperature == nullptr) return 0.f;
+  const int lane = threadIdx.x & 31, draft = row >= p.rows, own = draft ? row - p.rows : row;
+  int lo = 0;
+  for (int n = p.requests; n > 1;) {
+    const int step = (n + 31) / 32, i = lo + lane * step;
+    const bool before = lane * step < n && p.row_start[i] - (draft ? i : 0) <= own;
+    const int last = max(0, 31 - __clz(__ballot_sync(0xffffffffu, before)));
+    n = min(step, n - last * step);
+    lo += last * step;
+  }
+  return p.temperature[lo];
+}
+
+// A warp takes `items` pieces one after the other, the next on its way while one is added up: no warp waits for another (a block a
+// piece of 4,096 with barriers in its sums kept 3.7 TB/s in flight).  What bounds it is memory; an element takes some five
+// instructions: its share of a load, of a maximum and a minimum of three, a difference, a product, the exponential and the sum.
 __global__ void __launch_bounds__(THREADS, ROW_BLOCKS)
 verify_rows_kernel(const Args p) {
-  __shared__ float s_val[WARPS];
-  __shared__ int s_idx[WARPS];
-  __shared__ double s_sum[WARPS];
+  constexpr int LOGITS = PIECE / 32;                   // a lane's, in fours side by side over the lanes
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long all = (long long)(p.rows + p.draft_rows) * p.per_row, first = (long long)blockIdx.x * p.items, end = min(first + p.items, all);
-  int row = (int)(first / p.per_row), run = (int)(first % p.per_row), known = -1;
-  auto fetch = [&](int row, int run, float (&v)[PER_THREAD]) {
-    const float* base = row >= p.rows ? p.draft_logits + (size_t)(row - p.rows) * p.draft_ld : p.logits + (size_t)row * p.ld;
-    load_run(base + run * RUN, min(RUN, p.vocab - run * RUN), v);
-  };
-  float next[PER_THREAD];
-  if (first < end) fetch(row, run, next);
-  float temp = 0.f;
-  for (long long item = first; item < end; item++) {
-    float v[PER_THREAD];
-#pragma unroll
-    for (int i = 0; i < PER_THREAD; i++) v[i] = next[i];
-    const int at_row = row, at_run = run, begin = run * RUN, count = min(RUN, p.vocab - begin);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long all = (long long)(p.rows + p.draft_rows) * p.per_row, first = ((long long)blockIdx.x * WARPS + warp) * p.items;
+  if (first >= all) return;
+  const int items = (int)min((long long)p.items, all - first);
+  int row = (int)(first / p.per_row), piece = (int)(first % p.per_row);
+  auto place = [&](int i) { return (i >> 2) * 128 + lane * 4 + (i & 3); };
+  // the piece is wanted: not of a greedy request's draft, whose probabilities nobody asks for
+  auto fetch = [&](float temp, float (&v)[LOGITS]) {
     const bool draft = row >= p.rows;
-    if (++run == p.per_row) { run = 0; row++; }
-    if (item + 1 < end) fetch(row, run, next);         // on its way while this run is added up
-    if (at_row != known) {
-      // the row's request: the last whose rows (draft rows: one fewer per request before) begin at or before it; a warp asks 32
-      // places at once
-      const int own = draft ? at_row - p.rows : at_row;
-      int lo = 0;
-      for (int n = p.requests; n > 1;) {
-        const int step = (n + 31) / 32, i = lo + lane * step;
-        const bool before = lane * step < n && p.row_start[i] - (draft ? i : 0) <= own;
-        const int last = max(0, 31 - __clz(__ballot_sync(0xffffffffu, before)));
-        n = min(step, n - last * step);
-        lo += last * step;
+    if (draft && !(temp > 0.f)) return;
+    const float* base = (draft ? p.draft_logits + (size_t)(row - p.rows) * p.draft_ld : p.logits + (size_t)row * p.ld) + piece * PIECE;
+    const int count = min(PIECE, p.vocab - piece * PIECE);
+    const bool aligned = ((uintptr_t)base & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < LOGITS; i += 4) {
+      const float4 t = load_four(base, place(i), count, aligned);
+      v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
+    }
+  };
+  float temp = 1.f, even[LOGITS], odd[LOGITS];
+  fetch(temp, even);                                   // before it is known whether it is wanted: the question takes as long as the answer
+  temp = temperature_of(p, row);
+  auto step = [&](const float (&v)[LOGITS], float (&next)[LOGITS], bool more) {
+    const int at_row = row, begin = piece * PIECE, count = min(PIECE, p.vocab - begin);
+    const size_t slot = (size_t)row * p.per_row + piece;
+    const float own_temp = temp;
+    if (++piece == p.per_row) {
+      piece = 0;
+      row++;
+      if (more) temp = temperature_of(p, row);
+    }
+    if (more) fetch(temp, next);
+    const bool greedy = !(own_temp > 0.f);
+    if (greedy && at_row >= p.rows) return;
+    float best = -INFINITY, low = INFINITY;            // NaN is met below
+    if (count == PIECE) {
+#pragma unroll
+      for (int i = 0; i < LOGITS; i += 2) {
+        asm("max.f32 %0, %0, %1, %2;" : "+f"(best) : "f"(v[i]), "f"(v[i + 1]));
+        asm("min.f32 %0, %0, %1, %2;" : "+f"(low) : "f"(v[i]), "f"(v[i + 1]));
       }
-      temp = p.temperature ? p.temperature[lo] : 0.f;
-      known = at_row;
-    }
-    const bool greedy = !(temp > 0.f);
-    if (draft && greedy) continue;                     // a greedy request's draft probabilities are not asked for
-    float best = -INFINITY;
-    bool bad = false;
+    } else {
 #pragma unroll
-    for (int i = 0; i < PER_THREAD; i++) {
-      best = fmaxf(best, v[i]);
-      bad |= !(fabsf(v[i]) < INFINITY);
-    }
-    if (count < RUN) {                                 // beyond the vocabulary: not what was read
-      bad = false;
-#pragma unroll
-      for (int i = 0; i < PER_THREAD; i++) bad |= place_of(i) < count && !(fabsf(v[i]) < INFINITY);
+      for (int i = 0; i < LOGITS; i++) {
+        best = fmaxf(best, v[i]);                      // beyond the vocabulary: -inf
+        if (place(i) < count) low = fminf(low, v[i]);
+      }
     }
     best = warp_max(best);
-    if (lane == 0) s_val[warp] = best;
-    bad = __syncthreads_or(bad);
-    best = s_val[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; w++) best = fmaxf(best, s_val[w]);
+    bool bad = __any_sync(0xffffffffu, !(low > -INFINITY)) || !(best < INFINITY);
     int index = 0x7fffffff;
     double sum = 0.0;
     if (greedy) {
 #pragma unroll
-      for (int i = PER_THREAD - 1; i >= 0; i--) if (v[i] == best) index = begin + place_of(i);      // places rise with i
+      for (int i = LOGITS - 1; i >= 0; i--) {          // places rise with i
+        bad |= v[i] != v[i];
+        if (v[i] == best) index = begin + place(i);
+      }
       index = __reduce_min_sync(0xffffffffu, index);
-      if (lane == 0) s_idx[warp] = index;
-    } else if (!bad) {
-      // a product in two floats: the rounding of log2(e) / T would shift all weights alike, by 1e-7
-      const double c = 1.4426950408889634 / (double)temp;
-      const float c_hi = (float)c, c_lo = isinf(c_hi) ? 0.f : (float)(c - (double)c_hi);
+    } else {
+      // log2(e) / T rounded to a float shifts the sums by 1e-7 at most; infinite, it would make NaN of the maximum
+      const float c = fminf((float)(1.4426950408889634 / (double)own_temp), 3e38f);
       float sums[4] = {0.f, 0.f, 0.f, 0.f};
+      if (count == PIECE) {
 #pragma unroll
-      for (int i = 0; i < PER_THREAD; i++) {
-        const float d = v[i] - best, y = fmaxf(fmaf(d, c_hi, d * c_lo), -200.f);      // -200: also where infinities meet
-        const float e = d == 0.f ? 1.f : exp2_fast(y);                       // 0 times an infinite 1 / T
-        sums[i & 3] += count == RUN || place_of(i) < count ? e : 0.f;
+        for (int i = 0; i < LOGITS; i++) sums[i & 3] += exp2_fast((v[i] - best) * c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < LOGITS; i++) if (place(i) < count) sums[i & 3] += exp2_fast((v[i] - best) * c);
       }
-      sum = warp_sum_d(((double)sums[0] + (double)sums[1]) + ((double)sums[2] + (double)sums[3]));
-      if (lane == 0) s_sum[warp] = sum;
+      sum = warp_sum_d((double)(sums[0] + sums[1]) + (double)(sums[2] + sums[3]));
+      bad |= sum != sum;                               // a NaN among the logits
     }
-    __syncthreads();
-    if (tid == 0) {
-      if (greedy) {
-        for (int w = 0; w < WARPS; w++) index = min(index, s_idx[w]);
-      } else if (!bad) {
-        sum = s_sum[0];
-        for (int w = 1; w < WARPS; w++) sum += s_sum[w];
-      }
-      p.runs[(size_t)at_row * p.per_row + at_run] = RunSum{sum, best, index, bad, 0};
-    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) p.pieces[slot] = PieceSum{sum, best, index, bad, 0};
+  };
+  for (int item = 0; item < items; item += 2) {
+    step(even, odd, item + 1 < items);
+    if (item + 1 < items) step(odd, even, item + 2 < items);
   }
 }
 
-// What a row's runs add up to: its maximum, first index and (with `sums`) sum relative to the maximum, in every lane of the warp.
+// What a row's pieces add up to: its maximum, first index and (with `sums`) sum relative to the maximum, in every lane of the warp.
 struct RowSum { double sum; float max; int index; int bad; };
-__device__ __forceinline__ RowSum merge_runs(const RunSum* runs, int count, bool sums, double c) {
+__device__ __forceinline__ RowSum merge_pieces(const PieceSum* pieces, int count, bool sums, double c) {
   const int lane = threadIdx.x & 31;
   float best = -INFINITY;
   int best_i = 0x7fffffff, bad = 0;
   for (int i = lane; i < count; i += 32) {
-    better(best, best_i, runs[i].max, runs[i].index);
-    bad |= runs[i].bad;
+    better(best, best_i, pieces[i].max, pieces[i].index);
+    bad |= pieces[i].bad;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) better(best, best_i, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_i, o));
   bad = __any_sync(0xffffffffu, bad);
   double sum = 0.0;
   if (sums && !bad)
-    for (int i = lane; i < count; i += 32) sum += runs[i].sum * pow2(((double)runs[i].max - (double)best) * c);
+    for (int i = lane; i < count; i += 32) sum += pieces[i].sum * pow2(((double)pieces[i].max - (double)best) * c);
   return RowSum{warp_sum_d(sum), best, best_i, bad};
 }
 
@@ -255,7 +273,7 @@ verify_decide_kernel(const Args p) {
       const float u = greedy ? 0.f : p.accept[first + i];
       // asked for before the runs are merged: a read that waits for another
       const float lx = token ? p.logits[(size_t)(first + i) * p.ld + x] : 0.f, dx = token && model && !greedy ? p.draft_logits[(size_t)d * p.draft_ld + x] : 0.f;
-      const RowSum s = merge_runs(p.runs + (size_t)(first + i) * p.per_row, p.per_row, !greedy, c);
+      const RowSum s = merge_pieces(p.pieces + (size_t)(first + i) * p.per_row, p.per_row, !greedy, c);
       int verdict = s.bad ? SPROUT_STATUS_NONFINITE : 1;           // the last row never "stands": the draw is made there
       double zq = 0.0;
       float mq = 0.f;
@@ -268,7 +286,7 @@ verify_decide_kernel(const Args p) {
           const double px = pow2(((double)lx - (double)s.max) * c) / s.sum;
           double qx = 1.0;
           if (model) {
-            const RowSum t = merge_runs(p.runs + (size_t)(p.rows + d) * p.per_row, p.per_row, true, c);
+            const RowSum t = merge_pieces(p.pieces + (size_t)(p.rows + d) * p.per_row, p.per_row, true, c);
             if (t.bad) verdict = SPROUT_STATUS_NONFINITE;
             zq = t.sum; mq = t.max;
             qx = pow2(((double)dx - (double)mq) * c) / zq;
@@ -304,7 +322,7 @@ verify_sums_kernel(const Args p) {
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = blockIdx.x / p.per_row, run = blockIdx.x % p.per_row;
+  const int r = blockIdx.x / p.runs, run = blockIdx.x % p.runs;
   const Chosen at = p.chosen[r];
   if (at.row < 0) return;
   const int begin = run * RUN, count = min(RUN, p.vocab - begin);
@@ -341,7 +359,7 @@ verify_sums_kernel(const Args p) {
     double total = 0.0;
 #pragma unroll
     for (int w = 0; w < WARPS; w++) total += ((const double*)&s_sums[w])[tid];
-    ((double*)&p.sums[(size_t)r * p.per_row + run])[tid] = total;
+    ((double*)&p.sums[(size_t)r * p.runs + run])[tid] = total;
   }
 }
 
@@ -354,20 +372,20 @@ verify_draw_kernel(const Args p) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Chosen at = p.chosen[r];
   if (at.row < 0) return;
-  const Sums* sums = p.sums + (size_t)r * p.per_row;
+  const Sums* sums = p.sums + (size_t)r * p.runs;
   if (warp == 0) {
     // the run in which the draw falls, a lane a run
     double rho = 1.0, total = 0.0;
     bool from_p = at.draft_row < 0;
     if (!from_p) {
       double za = 0.0, zb = 0.0;
-      for (int i = lane; i < p.per_row; i += 32) { za += sums[i].a; zb += sums[i].b; }
+      for (int i = lane; i < p.runs; i += 32) { za += sums[i].a; zb += sums[i].b; }
       rho = warp_sum_d(zb) / warp_sum_d(za);
     }
-    auto weight = [&](int i) { return i >= p.per_row ? 0.0 : from_p ? sums[i].a : fmax(0.0, fma(sums[i].above_a, rho, -sums[i].above_b)); };
+    auto weight = [&](int i) { return i >= p.runs ? 0.0 : from_p ? sums[i].a : fmax(0.0, fma(sums[i].above_a, rho, -sums[i].above_b)); };
     for (int attempt = 0; attempt < 2; attempt++) {
       total = 0.0;
-      for (int i = lane; i < p.per_row; i += 32) total += weight(i);
+      for (int i = lane; i < p.runs; i += 32) total += weight(i);
       total = warp_sum_d(total);
       if (from_p || total > 0.0) break;
       from_p = true;                                   // p and q are the same everywhere (what falls then fell by rounding): drawn from p
@@ -376,7 +394,7 @@ verify_draw_kernel(const Args p) {
     double passed = 0.0, before = 0.0;
     int run = -1;                                      // stays so where the token that is left out has all the weight there is
     bool falls = false;
-    for (int base = 0; base < p.per_row && !falls; base += 32) {
+    for (int base = 0; base < p.runs && !falls; base += 32) {
       const double w = weight(base + lane);
       double upto = w;
 #pragma unroll
@@ -453,14 +471,15 @@ verify_draw_kernel(const Args p) {
 }  // namespace
 
 namespace {
+int pieces_of(int vocab) { return (vocab + PIECE - 1) / PIECE; }
 int runs_of(int vocab) { return (vocab + RUN - 1) / RUN; }
 long long aligned16(long long bytes) { return (bytes + 15) & ~15LL; }
 }  // namespace
 
 // Bytes of scratch, 16-byte aligned, for `rows` rows (target's and draft's together) of `vocab` logits.
 SPROUT_API long long sprout_verify_scratch_bytes(int rows, int requests, int vocab) {
-  const long long per_row = runs_of(vocab);
-  return aligned16(rows * per_row * (long long)sizeof(RunSum)) + aligned16(requests * (long long)sizeof(Chosen)) + requests * per_row * (long long)sizeof(Sums);
+  return aligned16(rows * (long long)pieces_of(vocab) * (long long)sizeof(PieceSum)) + aligned16(requests * (long long)sizeof(Chosen)) +
+         requests * (long long)runs_of(vocab) * (long long)sizeof(Sums);
 }
 
 // Request r's rows are row_start[r] .. row_start[r + 1] - 1 of `logits` [rows, vocab], at least one; its draft rows, one fewer, begin at
@@ -473,24 +492,26 @@ SPROUT_API int sprout_verify(const float* logits, long long ld, const float* dra
   SPROUT_REQUIRE(draft_rows == 0 || (draft_rows == rows - requests && draft_logits && draft_ld >= 0), "verify: a draft row per drafted token");
   SPROUT_REQUIRE(logits && drafts && row_start && out && accepted && scratch && status, "verify: null pointer");
   SPROUT_REQUIRE((temperature == nullptr) == (accept == nullptr) && (accept == nullptr) == (draw == nullptr), "verify: temperatures and both kinds of uniform numbers go together");
-  const long long per_row = runs_of(vocab), all = per_row * (rows + (long long)draft_rows);
-  SPROUT_REQUIRE(rows + (long long)draft_rows <= 0x7fffffffLL && per_row * requests <= 0x7fffffffLL, "verify: too many rows");
+  const long long per_row = pieces_of(vocab), runs = runs_of(vocab), all = per_row * (rows + (long long)draft_rows);
+  SPROUT_REQUIRE(rows + (long long)draft_rows <= 0x7fffffffLL && runs * requests <= 0x7fffffffLL, "verify: too many rows");
   Args p{logits, draft_logits, ld, draft_ld, row_start, temperature, drafts, accept, draw, out, accepted, status, nullptr, nullptr, nullptr,
-         rows, draft_rows, requests, vocab, (int)per_row, 0};
+         rows, draft_rows, requests, vocab, (int)per_row, (int)runs, 0};
   uint8_t* at = (uint8_t*)scratch;
-  p.runs = (RunSum*)at;
-  at += aligned16(all * (long long)sizeof(RunSum));
+  p.pieces = (PieceSum*)at;
+  at += aligned16(all * (long long)sizeof(PieceSum));
   p.chosen = (Chosen*)at;
   at += aligned16(requests * (long long)sizeof(Chosen));
   p.sums = (Sums*)at;
-  const long long blocks = (long long)ROW_BLOCKS * sprout_sm_count(), items = (all + blocks - 1) / blocks;
-  SPROUT_REQUIRE(items <= 0x7fffffffLL, "verify: too many rows");
+  // few pieces: a warp each; many: MAX_ITEMS of them, so that warps whose rows nobody asks for leave their place to others
+  const long long warps = (long long)ROW_BLOCKS * WARPS * sprout_sm_count(), even = (all + warps - 1) / warps, items = even < MAX_ITEMS ? even : MAX_ITEMS;
+  const long long blocks = (all + items * WARPS - 1) / (items * WARPS);
+  SPROUT_REQUIRE(blocks <= 0x7fffffffLL, "verify: too many rows");
   p.items = (int)items;
-  sprout_launch(verify_rows_kernel, dim3((unsigned)((all + items - 1) / items)), dim3(THREADS), 0, stream, p);
+  sprout_launch(verify_rows_kernel, dim3((unsigned)blocks), dim3(THREADS), 0, stream, p);
   if (sprout_check_launch("verify_rows")) return 1;
   sprout_launch(verify_decide_kernel, dim3(requests), dim3(THREADS), 0, stream, p);
   if (sprout_check_launch("verify_decide") || temperature == nullptr) return sprout_check_launch("verify_decide");
-  sprout_launch(verify_sums_kernel, dim3((unsigned)(per_row * requests)), dim3(THREADS), 0, stream, p);
+  sprout_launch(verify_sums_kernel, dim3((unsigned)(runs * requests)), dim3(THREADS), 0, stream, p);
   if (sprout_check_launch("verify_sums")) return 1;
   sprout_launch(verify_draw_kernel, dim3(requests), dim3(DRAW_THREADS), 0, stream, p);
   return sprout_check_launch("verify_draw");
