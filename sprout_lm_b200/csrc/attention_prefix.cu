@@ -1,0 +1,491 @@
+// Attention of a step's tokens over the paged cache where requests hold the same leading pages, those pages' keys and values read once for
+// all requests that hold them.
+//
+// A softmax over keys that are divided into ranges is put together from the ranges: with m_S the maximum of a range's scores, l_S the
+// sum of e^(s - m_S) and o_S the sum of e^(s - m_S) v,   o = sum_S e^(m_S - m) o_S / sum_S e^(m_S - m) l_S,   m the largest m_S.
+// So the keys that several requests share are a range of their own, whose rows are the tokens of all of them: a matrix product in place of
+// as many passes over the same keys.  The requests' own keys are ranges of few rows, streams of keys and values.  Long ranges are
+// divided again, so that the launch fills the device.
+//
+// One launch computes the items' partial results (attention_prefix_simple_kernel: CUDA cores, 32-bit products, any head size and either
+// type; attention_prefix_mma_kernel: mma.sync, bfloat16, head sizes up to 128), one adds them up.
+#include "attention_bf16.cuh"
+#include "attention_prefix.cuh"
+
+using namespace sprout_prefix;
+using namespace sprout_attn;
+
+namespace {
+
+// ------------------------------------------------------------------ CUDA cores
+// 16 rows, 64 keys at a time in shared memory as float32.  A thread has 2 rows x 4 keys of the scores, and 2 rows x 4 columns in
+// every 64 of the output.
+constexpr int SIMPLE_ROWS = 16, SIMPLE_KEYS = 64, SIMPLE_THREADS = 128;
+
+__host__ __device__ constexpr int simple_width(int head_dim) { return (head_dim + 3) / 4 * 4; }
+size_t simple_smem(int head_dim) {
+  const size_t w = simple_width(head_dim);
+  return ((w + 4) * (SIMPLE_KEYS + SIMPLE_ROWS) + w * SIMPLE_KEYS + SIMPLE_ROWS * (SIMPLE_KEYS + 4) + SIMPLE_ROWS * 3) * sizeof(float) + SIMPLE_KEYS * sizeof(long long);
+}
+
+// COLUMNS: of 64, that hold head_dim
+template <typename T, int COLUMNS>
+__global__ void __launch_bounds__(SIMPLE_THREADS)
+attention_prefix_simple_kernel(const Params p) {
+  extern __shared__ __align__(16) float simple_shared[];
+  const int w = simple_width(p.head_dim), ks = w + 4;
+  long long* rows = (long long*)simple_shared;         // [64] element offsets, -1: no such key
+  float* sK = (float*)(rows + SIMPLE_KEYS);            // [64][ks]
+  float* sQ = sK + SIMPLE_KEYS * ks;                   // [16][ks]
+  float* sV = sQ + SIMPLE_ROWS * ks;                   // [64][w]
+  float* sP = sV + SIMPLE_KEYS * w;                    // [16][68]
+  float* s_m = sP + SIMPLE_ROWS * (SIMPLE_KEYS + 4);   // [16] maxima, sums, what a pass multiplies the outputs by
+  float* s_l = s_m + SIMPLE_ROWS;
+  float* s_a = s_l + SIMPLE_ROWS;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Item item = p.items[blockIdx.x];
+  const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int* table = p.block_table + (size_t)item.table * p.table_stride;
+  for (int idx = tid; idx < SIMPLE_ROWS * w; idx += SIMPLE_THREADS) {
+    const int i = idx / w, c = idx % w;
+    float v = 0.f;
+    if (i < item.rows && c < p.head_dim)
+      v = to_float(((const T*)p.q)[(size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * p.head_dim + c]);
+    sQ[i * ks + c] = v;
+  }
+  if (tid < SIMPLE_ROWS) { s_m[tid] = -INFINITY; s_l[tid] = 0.f; }
+  const int r0 = tid / 16 * 2, c0 = tid % 16 * 4;
+  float acc[2][COLUMNS][4];
+#pragma unroll
+  for (int a = 0; a < 2; a++)
+#pragma unroll
+    for (int b = 0; b < COLUMNS; b++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) acc[a][b][c] = 0.f;
+  for (int base = item.key_begin; base < item.key_end; base += SIMPLE_KEYS) {
+    __syncthreads();                                   // the pass before is done with the keys and values
+    if (tid < SIMPLE_KEYS) rows[tid] = base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1;
+    __syncthreads();
+    for (int idx = tid; idx < SIMPLE_KEYS * w; idx += SIMPLE_THREADS) {
+      const int j = idx / w, c = idx % w;
+      const long long at = rows[j];
+      const bool has = at >= 0 && c < p.head_dim;
+      sK[j * ks + c] = has ? to_float(((const T*)p.k_cache)[at + c]) : 0.f;
+      sV[j * w + c] = has ? to_float(((const T*)p.v_cache)[at + c]) : 0.f;
+    }
+    __syncthreads();
+    float s[2][4] = {};
+    for (int d = 0; d < w; d += 4) {
+      float4 q[2], k[4];
+#pragma unroll
+      for (int a = 0; a < 2; a++) q[a] = *(const float4*)(sQ + (r0 + a) * ks + d);
+#pragma unroll
+      for (int b = 0; b < 4; b++) k[b] = *(const float4*)(sK + (tid % 16 + b * 16) * ks + d);
+#pragma unroll
+      for (int a = 0; a < 2; a++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) s[a][b] = fmaf(q[a].x, k[b].x, fmaf(q[a].y, k[b].y, fmaf(q[a].z, k[b].z, fmaf(q[a].w, k[b].w, s[a][b]))));
+    }
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int b = 0; b < 4; b++) sP[(r0 + a) * (SIMPLE_KEYS + 4) + tid % 16 + b * 16] = s[a][b] * p.scale_log2;
+    __syncthreads();
+    // softmax: a warp four rows, a lane two keys
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = warp * 4 + i;
+      float* row = sP + r * (SIMPLE_KEYS + 4);
+      const float x0 = rows[lane] >= 0 ? row[lane] : -INFINITY;
+      const float x1 = rows[lane + 32] >= 0 ? row[lane + 32] : -INFINITY;
+      const float before = s_m[r], m = fmaxf(before, warp_max(fmaxf(x0, x1)));
+      const float e0 = x0 == -INFINITY ? 0.f : exp2f(x0 - m), e1 = x1 == -INFINITY ? 0.f : exp2f(x1 - m);
+      const float sum = warp_sum(e0 + e1);
+      row[lane] = e0;
+      row[lane + 32] = e1;
+      __syncwarp();
+      if (lane == 0) {
+        const float a = before == -INFINITY ? 0.f : exp2f(before - m);
+        s_m[r] = m;
+        s_l[r] = s_l[r] * a + sum;
+        s_a[r] = a;
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+    const float a0 = s_a[r0], a1 = s_a[r0 + 1];
+#pragma unroll
+    for (int b = 0; b < COLUMNS; b++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) { acc[0][b][c] *= a0; acc[1][b][c] *= a1; }
+    for (int j = 0; j < SIMPLE_KEYS; j++) {
+      const float p0 = sP[r0 * (SIMPLE_KEYS + 4) + j], p1 = sP[(r0 + 1) * (SIMPLE_KEYS + 4) + j];
+#pragma unroll
+      for (int b = 0; b < COLUMNS; b++) {
+        if (b * 64 + c0 >= w) break;
+        const float4 v = *(const float4*)(sV + j * w + b * 64 + c0);
+        acc[0][b][0] = fmaf(p0, v.x, acc[0][b][0]); acc[0][b][1] = fmaf(p0, v.y, acc[0][b][1]);
+        acc[0][b][2] = fmaf(p0, v.z, acc[0][b][2]); acc[0][b][3] = fmaf(p0, v.w, acc[0][b][3]);
+        acc[1][b][0] = fmaf(p1, v.x, acc[1][b][0]); acc[1][b][1] = fmaf(p1, v.y, acc[1][b][1]);
+        acc[1][b][2] = fmaf(p1, v.z, acc[1][b][2]); acc[1][b][3] = fmaf(p1, v.w, acc[1][b][3]);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int a = 0; a < 2; a++) {
+    const int i = r0 + a;
+    if (i >= item.rows) break;
+    const size_t at = (size_t)(p.part_start[place_of_row(item, i, group)] + item.part) * p.heads + head_of_row(item, i, group, g);
+#pragma unroll
+    for (int b = 0; b < COLUMNS; b++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) if (b * 64 + c0 + c < p.head_dim) p.part_out[at * p.head_dim + b * 64 + c0 + c] = acc[a][b][c];
+    if (tid % 16 == 0) p.part_sum[at] = make_float2(s_m[i], s_l[i]);
+  }
+}
+
+// ------------------------------------------------------------------ mma.sync
+// 2^x, the hardware approximation; results below the normal range are zero
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Keys and values in passes of 128 through shared memory (cp.async), three or more CTAs an SM so that one's copies run under the others'
+// products.  NARROW (an item of up to 16 rows): the rows are one tile of the MMA, each of the 4 warps takes 32 keys of a pass, and the
+// warps' results are merged at the end.  Else an item has up to 64 rows, 16 a warp, and every warp takes all keys.
+constexpr int MMA_KEYS = 128, MMA_THREADS = 128;
+
+template <int HD, bool NARROW>
+struct MmaShape {
+  static constexpr int ROWS = NARROW ? 16 : 64, STRIDE = HD + 8, CHUNK = NARROW ? 32 : 64;    // CHUNK: keys between two looks at the maximum
+  static constexpr size_t SMEM = (size_t)(ROWS + 2 * MMA_KEYS) * STRIDE * 2 + MMA_KEYS * sizeof(long long);
+  static constexpr int CTAS = HD > 96 ? 3 : 4;
+};
+
+template <int HD, bool NARROW>
+__global__ void __launch_bounds__(MMA_THREADS, MmaShape<HD, NARROW>::CTAS)
+attention_prefix_mma_kernel(const Params p) {
+  using L = MmaShape<HD, NARROW>;
+  constexpr int STRIDE = L::STRIDE, PIECES = HD / 8, CHUNK = L::CHUNK;
+  extern __shared__ __align__(16) uint8_t mma_shared[];
+  long long* rows = (long long*)mma_shared;            // [128] element offsets, -1: no such key
+  __nv_bfloat16* sQ = (__nv_bfloat16*)(rows + MMA_KEYS);           // [ROWS][STRIDE]
+  __nv_bfloat16* sK = sQ + L::ROWS * STRIDE;           // [128][STRIDE]
+  __nv_bfloat16* sV = sK + MMA_KEYS * STRIDE;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Item item = p.items[blockIdx.x];
+  const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int* table = p.block_table + (size_t)item.table * p.table_stride;
+  const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
+  for (int idx = tid; idx < L::ROWS * PIECES; idx += MMA_THREADS) {
+    const int i = idx / PIECES, c = idx % PIECES;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (i < item.rows) v = *(const uint4*)(q + (size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * HD + c * 8);
+    *(uint4*)(sQ + i * STRIDE + c * 8) = v;
+  }
+  const int tile = NARROW ? 0 : warp, gr = lane >> 2, qc = lane & 3;
+  const int row0 = tile * 16 + gr, row1 = row0 + 8;    // of the item, this lane's in the fragments
+  const bool works = tile * 16 < item.rows;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[HD / 8][4];
+#pragma unroll
+  for (int n = 0; n < HD / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  for (int base = item.key_begin; base < item.key_end; base += MMA_KEYS) {
+    __syncthreads();                                   // the pass before is done with the keys and values
+    const long long mine = base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1;
+    rows[tid] = mine;
+    const bool whole = __syncthreads_and(mine >= 0);
+    for (int idx = tid; idx < MMA_KEYS * PIECES; idx += MMA_THREADS) {
+      const int j = idx / PIECES, c = idx % PIECES;
+      const long long at = rows[j];
+      if (at >= 0) {
+        cp_async16(sK + j * STRIDE + c * 8, (const __nv_bfloat16*)p.k_cache + at + c * 8);
+        cp_async16(sV + j * STRIDE + c * 8, (const __nv_bfloat16*)p.v_cache + at + c * 8);
+      } else {                                         // what no key fills is finite: its weight is zero, and zero times a NaN is not
+        *(uint4*)(sK + j * STRIDE + c * 8) = make_uint4(0, 0, 0, 0);
+        *(uint4*)(sV + j * STRIDE + c * 8) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
+    if (!works) continue;
+    const int chunk0 = NARROW ? warp * CHUNK : 0, chunk1 = NARROW ? chunk0 + CHUNK : MMA_KEYS;
+    for (int chunk = chunk0; chunk < chunk1 && base + chunk < item.key_end; chunk += CHUNK) {
+      float s[CHUNK / 8][4];
+#pragma unroll
+      for (int n = 0; n < CHUNK / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; kk++) {
+        uint32_t a[4];
+        ldmatrix_x4(a, sQ + (tile * 16 + (lane & 15)) * STRIDE + kk * 16 + (lane >> 4) * 8);
+#pragma unroll
+        for (int n = 0; n < CHUNK / 16; n++) {
+          uint32_t b[4];                               // keys 16 n .. + 15: fragments of two MMAs
+          ldmatrix_x4(b, sK + (chunk + n * 16 + (lane & 7) + ((lane >> 4) << 3)) * STRIDE + kk * 16 + ((lane >> 3) & 1) * 8);
+          mma_bf16(s[2 * n], a, b[0], b[1]);
+          mma_bf16(s[2 * n + 1], a, b[2], b[3]);
+        }
+      }
+      float top0 = m0, top1 = m1;
+#pragma unroll
+      for (int n = 0; n < CHUNK / 8; n++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[n][i] *= p.scale_log2;
+      if (!whole)
+#pragma unroll
+        for (int n = 0; n < CHUNK / 8; n++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) if (rows[chunk + n * 8 + qc * 2 + i] < 0) s[n][i] = s[n][2 + i] = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < CHUNK / 8; n++) {
+        top0 = fmaxf(top0, fmaxf(s[n][0], s[n][1]));
+        top1 = fmaxf(top1, fmaxf(s[n][2], s[n][3]));
+      }
+      top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 1));
+      top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
+      top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
+      top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
+      const float alpha0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top0), alpha1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top1);
+      m0 = top0;
+      m1 = top1;
+      const float base0 = m0 == -INFINITY ? 0.f : m0, base1 = m1 == -INFINITY ? 0.f : m1;
+      float sum0 = 0.f, sum1 = 0.f;
+      uint32_t pf[CHUNK / 16][4];                      // the weights as bfloat16, the A operand of P V
+#pragma unroll
+      for (int n = 0; n < CHUNK / 8; n++) {
+        const float e0 = exp2_fast(s[n][0] - base0), e1 = exp2_fast(s[n][1] - base0), e2 = exp2_fast(s[n][2] - base1), e3 = exp2_fast(s[n][3] - base1);
+        sum0 += e0 + e1;
+        sum1 += e2 + e3;
+        pf[n >> 1][(n & 1) * 2] = pack_bf16(e0, e1);
+        pf[n >> 1][(n & 1) * 2 + 1] = pack_bf16(e2, e3);
+      }
+      l0 = l0 * alpha0 + sum0;
+      l1 = l1 * alpha1 + sum1;
+#pragma unroll
+      for (int n = 0; n < HD / 8; n++) { o[n][0] *= alpha0; o[n][1] *= alpha0; o[n][2] *= alpha1; o[n][3] *= alpha1; }
+#pragma unroll
+      for (int k = 0; k < CHUNK / 16; k++)
+#pragma unroll
+        for (int n = 0; n < HD / 16; n++) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, sV + (chunk + k * 16 + (lane & 15)) * STRIDE + n * 16 + (lane >> 4) * 8);
+          mma_bf16(o[2 * n], pf[k], b[0], b[1]);
+          mma_bf16(o[2 * n + 1], pf[k], b[2], b[3]);
+        }
+    }
+  }
+  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+  auto slot = [&](int i) { return (size_t)(p.part_start[place_of_row(item, i, group)] + item.part) * p.heads + head_of_row(item, i, group, g); };
+  if (!NARROW) {
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int i = half ? row1 : row0;
+      if (i >= item.rows) continue;
+      const size_t at = slot(i);
+#pragma unroll
+      for (int n = 0; n < HD / 8; n++) *(float2*)(p.part_out + at * HD + n * 8 + qc * 2) = make_float2(o[n][half * 2], o[n][half * 2 + 1]);
+      if (qc == 0) p.part_sum[at] = half ? make_float2(m1, l1) : make_float2(m0, l0);
+    }
+    return;
+  }
+  // the warps' results, in the keys' and values' room: [4 warps][16 rows][HD], maxima and sums behind them
+  float* w_out = (float*)sK;
+  float2* w_sum = (float2*)(w_out + 4 * 16 * HD);
+  static_assert((size_t)4 * 16 * HD * 4 + 64 * 8 <= (size_t)2 * MMA_KEYS * STRIDE * 2, "the warps' results fit the keys' and values' room");
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < HD / 8; n++) {
+    *(float2*)(w_out + (warp * 16 + gr) * HD + n * 8 + qc * 2) = make_float2(o[n][0], o[n][1]);
+    *(float2*)(w_out + (warp * 16 + gr + 8) * HD + n * 8 + qc * 2) = make_float2(o[n][2], o[n][3]);
+  }
+  if (qc == 0) { w_sum[warp * 16 + gr] = make_float2(m0, l0); w_sum[warp * 16 + gr + 8] = make_float2(m1, l1); }
+  __syncthreads();
+  for (int idx = tid; idx < item.rows * (HD / 4); idx += MMA_THREADS) {
+    const int i = idx / (HD / 4), c = idx % (HD / 4) * 4;
+    float2 ml[4];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) { ml[w] = w_sum[w * 16 + i]; m = fmaxf(m, ml[w].x); }
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = ml[w].x == -INFINITY ? 0.f : exp2f(ml[w].x - m);
+      const float4 t = *(const float4*)(w_out + (w * 16 + i) * HD + c);
+      sum.x = fmaf(t.x, f, sum.x); sum.y = fmaf(t.y, f, sum.y); sum.z = fmaf(t.z, f, sum.z); sum.w = fmaf(t.w, f, sum.w);
+      l = fmaf(ml[w].y, f, l);
+    }
+    const size_t at = slot(i);
+    *(float4*)(p.part_out + at * HD + c) = sum;
+    if (c == 0) p.part_sum[at] = make_float2(m, l);
+  }
+}
+
+// ------------------------------------------------------------------ the parts of a row put together
+// A warp per (token, head), a lane two columns in every 64; with the keys of the member's own tokens that the items leave out, a lane a key.
+constexpr int MERGE_THREADS = 128;
+
+template <typename T, int PAIRS>
+__global__ void __launch_bounds__(MERGE_THREADS)
+attention_prefix_merge_kernel(const Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, group = p.heads / p.kv_heads;
+  const long long row = (long long)blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5);
+  if (row >= (long long)p.tokens * p.heads) return;
+  const int head = (int)(row % p.heads), place = (int)(row / p.heads), token = p.order[place], g = head / group;
+  const int first = p.part_start[place], end = p.part_start[place + 1];
+  const int seen = p.seen[place], extra = p.extra[place];
+  if (p.positions[token] != seen + extra - 1 && head == 0 && lane == 0) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);      // another step's plan
+  float m = -INFINITY, l = 0.f, sum[PAIRS][2];
+#pragma unroll
+  for (int k = 0; k < PAIRS; k++) sum[k][0] = sum[k][1] = 0.f;
+  for (int part = first + lane; part < end; part += 32) m = fmaxf(m, p.part_sum[(size_t)part * p.heads + head].x);
+  float score = -INFINITY;                             // of this lane's extra key
+  long long at = -1;
+  if (extra > 0) {
+    if (lane < extra) at = key_row(p, p.block_table + (size_t)p.table_of[place] * p.table_stride, seen + lane, g);
+    const T* q = (const T*)p.q + (size_t)token * p.q_stride + (size_t)head * p.head_dim;
+    for (int j = 0; j < extra; j++) {
+      const long long k_at = __shfl_sync(0xffffffffu, at, j);
+      if (k_at < 0) continue;
+      float dot = 0.f;
+#pragma unroll
+      for (int k = 0; k < PAIRS; k++) {
+        const int c = k * 64 + lane * 2;
+        if (c < p.head_dim) dot = fmaf(to_float(q[c]), to_float(((const T*)p.k_cache)[k_at + c]), fmaf(to_float(q[c + 1]), to_float(((const T*)p.k_cache)[k_at + c + 1]), dot));
+      }
+      dot = warp_sum(dot);
+      if (lane == j) score = dot * p.scale_log2;
+    }
+  }
+  m = warp_max(fmaxf(m, score));
+  for (int part = first; part < end; part++) {
+    const float2 ml = p.part_sum[(size_t)part * p.heads + head];
+    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+    const float* from = p.part_out + ((size_t)part * p.heads + head) * p.head_dim;
+#pragma unroll
+    for (int k = 0; k < PAIRS; k++) {
+      const int c = k * 64 + lane * 2;
+      if (c < p.head_dim) {
+        const float2 t = *(const float2*)(from + c);
+        sum[k][0] = fmaf(t.x, f, sum[k][0]);
+        sum[k][1] = fmaf(t.y, f, sum[k][1]);
+      }
+    }
+    l = fmaf(ml.y, f, l);
+  }
+  for (int j = 0; j < extra; j++) {
+    const long long v_at = __shfl_sync(0xffffffffu, at, j);
+    const float e = exp2f(__shfl_sync(0xffffffffu, score, j) - m);
+    if (v_at < 0) continue;
+#pragma unroll
+    for (int k = 0; k < PAIRS; k++) {
+      const int c = k * 64 + lane * 2;
+      if (c < p.head_dim) {
+        sum[k][0] = fmaf(e, to_float(((const T*)p.v_cache)[v_at + c]), sum[k][0]);
+        sum[k][1] = fmaf(e, to_float(((const T*)p.v_cache)[v_at + c + 1]), sum[k][1]);
+      }
+    }
+    l += e;
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;         // no key at all (every page outside the pool): zero
+  T* to = (T*)p.out + (size_t)token * p.out_stride + (size_t)head * p.head_dim;
+#pragma unroll
+  for (int k = 0; k < PAIRS; k++) {
+    const int c = k * 64 + lane * 2;
+    if (c < p.head_dim) { to[c] = from_float<T>(sum[k][0] * inv); to[c + 1] = from_float<T>(sum[k][1] * inv); }
+  }
+}
+
+// ------------------------------------------------------------------ launches
+template <typename F>
+int reserve(F kernel, size_t bytes, const char* what) {
+  if (bytes <= 48 * 1024) return 0;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return err == cudaSuccess ? 0 : sprout_fail("%s: cannot reserve %zu bytes of shared memory: %s", what, bytes, cudaGetErrorString(err));
+}
+
+template <typename T, int COLUMNS>
+int launch_simple(const Params& p, int items, cudaStream_t stream) {
+  if (reserve(attention_prefix_simple_kernel<T, COLUMNS>, simple_smem(p.head_dim), "attention_shared_prefix")) return 1;
+  sprout_launch(attention_prefix_simple_kernel<T, COLUMNS>, dim3(items, p.kv_heads), dim3(SIMPLE_THREADS), simple_smem(p.head_dim), stream, p);
+  return sprout_check_launch("attention_prefix_simple");
+}
+template <typename T>
+int launch_simple_any(const Params& p, int items, cudaStream_t stream) {
+  if (p.head_dim <= 64) return launch_simple<T, 1>(p, items, stream);
+  if (p.head_dim <= 128) return launch_simple<T, 2>(p, items, stream);
+  return launch_simple<T, 4>(p, items, stream);
+}
+
+template <int HD, bool NARROW>
+int launch_mma(const Params& p, int items, cudaStream_t stream) {
+  constexpr size_t bytes = MmaShape<HD, NARROW>::SMEM;
+  if (reserve(attention_prefix_mma_kernel<HD, NARROW>, bytes, "attention_shared_prefix")) return 1;
+  sprout_launch(attention_prefix_mma_kernel<HD, NARROW>, dim3(items, p.kv_heads), dim3(MMA_THREADS), bytes, stream, p);
+  return sprout_check_launch("attention_prefix_mma");
+}
+template <bool NARROW>
+int launch_mma_any(const Params& p, int items, cudaStream_t stream) {
+  switch (p.head_dim) {
+    case 16: return launch_mma<16, NARROW>(p, items, stream);
+    case 32: return launch_mma<32, NARROW>(p, items, stream);
+    case 48: return launch_mma<48, NARROW>(p, items, stream);
+    case 64: return launch_mma<64, NARROW>(p, items, stream);
+    case 80: return launch_mma<80, NARROW>(p, items, stream);
+    case 96: return launch_mma<96, NARROW>(p, items, stream);
+    case 112: return launch_mma<112, NARROW>(p, items, stream);
+    case 128: return launch_mma<128, NARROW>(p, items, stream);
+  }
+  return sprout_fail("attention_shared_prefix: head_dim %d is not the tensor cores'", p.head_dim);
+}
+
+template <typename T>
+int launch_merge(const Params& p, cudaStream_t stream) {
+  const long long blocks = ((long long)p.tokens * p.heads + MERGE_THREADS / 32 - 1) / (MERGE_THREADS / 32);
+  SPROUT_REQUIRE(blocks <= 0x7fffffffLL, "attention_shared_prefix: too many tokens");
+  if (p.head_dim <= 64) sprout_launch(attention_prefix_merge_kernel<T, 1>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
+  else if (p.head_dim <= 128) sprout_launch(attention_prefix_merge_kernel<T, 2>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
+  else sprout_launch(attention_prefix_merge_kernel<T, 4>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
+  return sprout_check_launch("attention_prefix_merge");
+}
+
+}  // namespace
+
+// Whether bfloat16 items of this head size run on the tensor cores.
+SPROUT_API int sprout_attention_prefix_mma_supported(int head_dim) { return head_dim % 16 == 0 && head_dim > 0 && head_dim <= 128; }
+
+// items: `simple_items` for the CUDA cores, or `narrow_items` of up to 16 rows and `wide_items` of up to 64 behind them.  `parts`: the
+// partial results in all; part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
+SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
+                                       const int* positions, const int* items, int simple_items, int narrow_items, int wide_items, const int* order,
+                                       const int* part_start, const int* seen, const int* extra, const int* table_of, float* part_out, float* part_sum, void* out, long long out_stride, int dtype, int tokens,
+                                       int heads, int kv_heads, int head_dim, int page_tokens, int num_pages, int* status, cudaStream_t stream) {
+  SPROUT_REQUIRE(q && k_cache && v_cache && block_table && positions && items && order && part_start && seen && extra && table_of && part_out && part_sum && out && status,
+                 "attention_shared_prefix: null pointer");
+  SPROUT_REQUIRE(tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
+                 "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
+  SPROUT_REQUIRE(simple_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (simple_items > 0) != (narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
+  SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
+  Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, (const Item*)items, order, part_start, seen, extra, table_of, part_out, (float2*)part_sum, out, out_stride,
+           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status};
+  if (simple_items > 0) {
+    if (dtype == SPROUT_F32 ? launch_simple_any<float>(p, simple_items, stream) : launch_simple_any<__nv_bfloat16>(p, simple_items, stream)) return 1;
+  } else {
+    SPROUT_REQUIRE(dtype == SPROUT_BF16 && sprout_attention_prefix_mma_supported(head_dim), "attention_shared_prefix: these sizes run on the CUDA cores");
+    SPROUT_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0,
+                   "attention_shared_prefix: rows must start on 16-byte boundaries");
+    if (narrow_items > 0 && launch_mma_any<true>(p, narrow_items, stream)) return 1;
+    p.items += narrow_items;
+    if (wide_items > 0 && launch_mma_any<false>(p, wide_items, stream)) return 1;
+  }
+  return dtype == SPROUT_F32 ? launch_merge<float>(p, stream) : launch_merge<__nv_bfloat16>(p, stream);
+}

@@ -1,0 +1,55 @@
+// What the kernels of attention over shared prefixes (attention_prefix.cu, attention_prefix_tcgen05.cu) share: a launch's parameters, the
+// items of its plan, and where an item's partial results go.
+#pragma once
+#include "common.cuh"
+
+namespace sprout_prefix {
+
+// A plan takes a step's tokens in members: up to MEMBER_TOKENS tokens of a request, one behind the other.  It divides the keys that all of
+// a member's tokens see into segments: a run of pages that several members hold, or a member's own keys behind those.  Tokens stand in
+// the plan's order, in which the members of every segment lie side by side.  A segment's rows are its tokens times the query heads of a
+// key/value head; an item is some of its rows over some of its keys, for every key/value head.  So every row of an item sees every
+// key of it: there is no mask, and what a later token of the step left in the cache reaches no earlier one.  The keys that only some of
+// a member's tokens see (those of the member's own later tokens, fewer than MEMBER_TOKENS) are added where the parts are put together.
+constexpr int MEMBER_TOKENS = 16;
+
+struct Item {
+  int table;                           // the request whose block table gives the pages (any that holds them)
+  int key_begin, key_end;
+  int token_begin;                     // the segment's first token, in the plan's order
+  int row_begin, rows;                 // of the segment's rows: (token - token_begin) * group + head within the group
+  int part;                            // the place of this range among the token's ranges
+  int pad;
+};
+
+struct Params {
+  const void* q; long long q_stride;   // [tokens, heads * head_dim]
+  const void* k_cache; const void* v_cache;            // [pages, kv_heads, page_tokens, head_dim]
+  const int* block_table; int table_stride;
+  const int* positions;                // [tokens]: the tokens' own, which have to be the plan's
+  const Item* items;
+  const int* order;                    // [tokens]: the step's token at a place of the plan's order
+  const int* part_start;               // [tokens + 1]: the first of the place's partial results
+  const int* seen;                     // [tokens]: keys that the items of a place's member hold
+  const int* extra;                    // [tokens]: and the further ones that the place sees, fewer than MEMBER_TOKENS
+  const int* table_of;                 // [tokens]: the place's request
+  float* part_out;                     // [partial results, heads, head_dim], unnormalised
+  float2* part_sum;                    // [partial results, heads]: the maximum (scaled, times log2(e)) and the sum
+  void* out; long long out_stride;
+  int tokens, heads, kv_heads, head_dim, page_tokens, num_pages;
+  float scale_log2;                    // log2(e) / sqrt(head_dim)
+  int* status;
+};
+
+// An item's row i, 0 <= i < rows: its place in the plan's order, and its query head.
+__device__ __forceinline__ int place_of_row(const Item& item, int i, int group) { return item.token_begin + (item.row_begin + i) / group; }
+__device__ __forceinline__ int head_of_row(const Item& item, int i, int group, int g) { return g * group + (item.row_begin + i) % group; }
+
+// The element offset of a key's row in the cache; -1 (and a status bit) where its page lies outside the pool.
+__device__ __forceinline__ long long key_row(const Params& p, const int* table, int key, int g) {
+  const int page = table[key / p.page_tokens];
+  if (page < 0 || page >= p.num_pages) { atomicOr(p.status, SPROUT_STATUS_BAD_PAGE); return -1; }
+  return (((long long)page * p.kv_heads + g) * p.page_tokens + key % p.page_tokens) * p.head_dim;
+}
+
+}  // namespace sprout_prefix

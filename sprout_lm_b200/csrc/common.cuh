@@ -22,7 +22,7 @@ enum SproutStatus : int {
   SPROUT_STATUS_BAD_TOKEN = 2,      // a token id outside the vocabulary
   SPROUT_STATUS_NONFINITE = 4,      // non-finite logits met while sampling
   SPROUT_STATUS_WAIT_TIMEOUT = 8,   // a bounded mbarrier wait ran out
-  SPROUT_STATUS_BAD_POSITION = 16,  // a position outside the rotary table
+  SPROUT_STATUS_BAD_POSITION = 16,  // a position outside the rotary table, or other than a plan's
   SPROUT_STATUS_BAD_LAYOUT = 32,    // a kernel's shared memory did not start where its tiles need it
   SPROUT_STATUS_BAD_ROWS = 64,      // a request's rows outside the step's
 };

@@ -16,11 +16,12 @@ from ctypes import c_float, c_int, c_void_p
 import torch
 
 from .csrc.build import BuildError, library_path
+from .prefix_plan import HostPlan, PlanError
 
 F32, BF16 = 0, 1
 LAUNCHES = 0          # kernels launched through this module (one per call); benchmarks read the difference
 STATUS_BITS = {1: "a block-table entry outside the page pool", 2: "a token id outside the vocabulary",
-               4: "non-finite logits", 8: "a bounded device-side wait ran out", 16: "a position outside the rotary table",
+               4: "non-finite logits", 8: "a bounded device-side wait ran out", 16: "a position outside the rotary table, or other than a plan's",
                32: "a kernel's shared memory was not aligned for its tiles", 64: "a request's rows outside the step's"}
 
 
@@ -39,6 +40,8 @@ _SIGNATURES = {
     "sprout_attention_simple": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
+    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "sprout_attention_prefix_mma_supported": [_I],
     "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
     "sprout_feed_tokens": [_P, _P, _P, _I, _I, _I, _P],
@@ -958,6 +961,83 @@ def paged_attention(q, cache, ctx, out, heads, kv_heads, head_dim, status):
                               ctx.max_q_len, status)
     attention_simple(q, cache.k, cache.v, cache.block_table, ctx.seq_of_token, ctx.positions, out,
                      heads, kv_heads, head_dim, status)
+
+
+# ---------------------------------------------------------------------------------- attention over shared prefixes
+
+class SharedPrefixPlan:
+    """A step's plan on the device (``shared_prefix_plan``): the arrays that ``attention_shared_prefix`` walks, for all layers of the step."""
+
+    def __init__(self, host: HostPlan, page_tokens: int, heads: int, kv_heads: int, head_dim: int, dtype, buffer: torch.Tensor):
+        self.host, self.page_tokens, self.heads, self.kv_heads, self.head_dim, self.dtype, self.buffer = host, page_tokens, heads, kv_heads, head_dim, dtype, buffer
+        base = buffer.data_ptr()
+        self.pointers = [base + 4 * at for at, _ in host.offsets]
+        # maxima and sums of the partial results, then the results
+        self.scratch_floats = host.parts * heads * (head_dim + 2)
+
+
+def _prefix_slots(head_dim: int, tensor_cores: bool) -> int:
+    """Items that the device holds at once, by their registers and shared memory."""
+    sms = sm_count() if torch.cuda.is_available() else 148
+    return sms * ((3 if head_dim > 96 else 4) if tensor_cores else 2)
+
+
+def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, head_dim: int, dtype, device=None) -> SharedPrefixPlan:
+    """How ``attention_shared_prefix`` divides the keys of a step.  All on the host: ``tables`` [requests, pages] the requests' pages
+    (entries behind a request's last page are not read), ``q_start`` [requests + 1] where each request's tokens start among the step's,
+    ``contexts`` [requests] the keys that each request's last token sees.  Runs of leading pages that several requests hold are found in
+    the tables, branching ones too; pages that this step still writes are nobody else's.  ``dtype``: of the cache.  The plan depends on
+    nothing else, and one made for a step serves all its layers with these sizes."""
+    _dtype_code(dtype)
+    if not 0 < head_dim <= 256 or head_dim % 2:
+        raise KernelError(f"shared_prefix_plan: head_dim must be even and at most 256 (got {head_dim})")
+    tensor_cores = dtype == torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 128
+    try:
+        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, _prefix_slots(head_dim, tensor_cores))
+    except PlanError as error:
+        raise KernelError(f"shared_prefix_plan: {error}") from None
+    packed = torch.from_numpy(host.pack())
+    return SharedPrefixPlan(host, page_tokens, heads, kv_heads, head_dim, dtype, packed.to(device if device is not None else "cuda"))
+
+
+def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: SharedPrefixPlan, out, status, scratch=None):
+    """Causal attention of a step's tokens over their requests' pages, a run of pages that several requests hold read once for all of
+    them.  ``q`` and ``out`` [tokens, heads * head_dim] (rows may lie apart), the caches [pages, kv_heads, page_tokens, head_dim], all
+    of the plan's type; ``block_table`` int32 [requests, pages] holds what the plan was made of; ``positions`` int32 [tokens]: a token
+    sees the keys up to its own, and a position other than the plan's sets a status bit (another step's plan).  float32 runs on CUDA
+    cores with 32-bit products, bfloat16 on tensor cores for head sizes up to 128 in steps of 16.  ``scratch``: float32 memory of
+    ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own."""
+    name = "attention_shared_prefix"
+    host = plan.host
+    _one_device(name, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("positions", positions), ("plan", plan.buffer),
+                       ("out", out), ("status", status), ("scratch", scratch)))
+    _rows_contiguous(q, "q")
+    _rows_contiguous(out, "out")
+    _rows_contiguous(block_table, "block_table")
+    width = plan.heads * plan.head_dim
+    if q.shape != (host.tokens, width) or out.shape != (host.tokens, width):
+        raise KernelError(f"{name}: q and out must be [{host.tokens}, {width}], the plan's tokens and heads")
+    if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or k_cache.shape[1:] != (plan.kv_heads, plan.page_tokens, plan.head_dim) or k_cache.shape[0] < 1 \
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise KernelError(f"{name}: caches must be contiguous [pages, {plan.kv_heads}, {plan.page_tokens}, {plan.head_dim}], the plan's sizes")
+    if not (q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == plan.dtype):
+        raise KernelError(f"{name}: q, out and the caches must be {plan.dtype}, the plan's type")
+    if block_table.shape[0] < host.requests or block_table.shape[1] < host.pages:
+        raise KernelError(f"{name}: block_table must hold the plan's {host.requests} requests and {host.pages} pages")
+    if positions.dtype != torch.int32 or positions.shape != (host.tokens,) or not positions.is_contiguous():
+        raise KernelError(f"{name}: positions must be contiguous int32 [{host.tokens}]")
+    if _overlap(q, out):
+        raise KernelError(f"{name}: q and out share memory")
+    if scratch is None:
+        scratch = torch.empty(plan.scratch_floats, dtype=torch.float32, device=q.device)
+    elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < plan.scratch_floats or scratch.data_ptr() % 16:
+        raise KernelError(f"{name}: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
+    items, order, part_start, seen, extra, table_of = plan.pointers
+    at = scratch.data_ptr()
+    _run("sprout_attention_prefix", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(block_table, "block_table", torch.int32),
+         block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.narrow_items, host.wide_items, order, part_start, seen, extra, table_of,
+         at, at + 4 * host.parts * plan.heads * plan.head_dim, out.data_ptr(), out.stride(0), _dtype_code(q.dtype), host.tokens, plan.heads, plan.kv_heads,
+         plan.head_dim, plan.page_tokens, k_cache.shape[0], _ptr(status, "status", torch.int32), _stream())
 
 
 def sample(logits, out, status, temperature=None, uniform=None):
@@ -2323,4 +2403,4 @@ def describe_status(word: int) -> str:
 
 __all__ = ["KernelError", "BuildError", "load_library", "library_file", "embed", "rmsnorm", "swiglu",
            "rope_append", "gemm_simple", "gemm_bf16", "attention_simple", "attention_tile", "attention_decode", "attention_decode_fused", "attention_decode_resident", "decode_attention_plan", "decode_fusable", "attention_prefill",
-           "paged_attention", "sample", "verify_drafts", "advance_decode", "feed_tokens", "describe_status"]
+           "paged_attention", "shared_prefix_plan", "attention_shared_prefix", "sample", "verify_drafts", "advance_decode", "feed_tokens", "describe_status"]

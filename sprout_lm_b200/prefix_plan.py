@@ -1,0 +1,177 @@
+"""How attention divides the keys of a step whose requests hold the same leading pages (host only; csrc/attention_prefix.cuh says what
+the kernels make of it).
+
+The step's tokens are taken in *members*: up to ``MEMBER_TOKENS`` tokens of one request.  Members' block tables are a trie over pages:
+a run of pages that several members hold is a *segment* read once for all of them; what lies behind its last shared run is a member's own
+segment.  Runs may branch: all requests share a system prompt, some of them a document behind it.  Only keys that all of a member's tokens
+see are divided this way; what its later tokens see of one another is added where the parts are put together.
+
+A segment's rows (its tokens times the query heads of a key/value head) are cut into tiles and its keys into ranges, so that the tiles'
+ranges, the *items*, fill the device once.  Everything is arrays: a plan is made once a step and serves all layers.
+"""
+from __future__ import annotations
+
+import numpy as np
+
+MEMBER_TOKENS = 16          # attention_prefix.cuh: MEMBER_TOKENS
+KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole steps
+NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS = 16, 64, 16      # rows of an item of each kind
+MAX_RANGES = 64             # of a segment
+# A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
+# the members read it themselves.
+MIN_SAVED_KEYS = 64
+
+
+class PlanError(ValueError):
+    pass
+
+
+class Segment:
+    """Keys ``key_begin`` to ``key_end`` of the pages in block table row ``table``, seen by the places ``token_begin`` to ``token_end`` of the
+    plan's order; ``part``: the first of its partial results at each of these places (``ranges`` of them)."""
+    __slots__ = ("table", "key_begin", "key_end", "token_begin", "token_end", "part", "ranges")
+
+    def __init__(self, table, key_begin, key_end, token_begin=0, token_end=0):
+        self.table, self.key_begin, self.key_end, self.token_begin, self.token_end = table, key_begin, key_end, token_begin, token_end
+        self.part, self.ranges = 0, 1
+
+
+def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray, page_tokens: int):
+    """(segments, order, seen, extra, table_of): the trie's segments, parents before their children; per place of the plan's order the
+    step's token there, the keys that its member's tokens all see, the further ones that it sees itself, and its request.  The
+    parent of a segment is in ``parents`` of the result (-1: none)."""
+    counts = np.diff(q_start)
+    # members: request, first token, tokens, keys that all of them see
+    blocks = -(-counts // MEMBER_TOKENS)
+    request = np.repeat(np.arange(len(counts)), blocks)
+    offset = (np.arange(len(request)) - np.repeat(np.cumsum(blocks) - blocks, blocks)) * MEMBER_TOKENS
+    tokens = np.minimum(MEMBER_TOKENS, counts[request] - offset)
+    first = q_start[request] + offset
+    sees = contexts[request] - counts[request] + offset + 1
+    whole = sees // page_tokens                          # full pages among them: what may be shared
+    segments, parents, leaves = [], [], []               # leaves: members in the plan's order
+    placed = 0
+
+    def own(member, start, parent):
+        nonlocal placed
+        if int(sees[member]) > start * page_tokens:      # else all it sees lies in shared runs
+            segments.append(Segment(int(request[member]), int(start) * page_tokens, int(sees[member]), placed, placed + int(tokens[member])))
+            parents.append(parent)
+        leaves.append(member)
+        placed += int(tokens[member])
+
+    def walk(members, start, depth, parent):
+        # all of `members` (two or more) hold the same pages up to `depth`; those from `start` on are in no segment yet
+        rows = tables[request[members], depth:int(whole[members].min())]
+        same = (rows == rows[0]).all(axis=0)
+        end = depth + (int(same.argmin()) if not same.all() else rows.shape[1])
+        mine = None
+        if (len(members) - 1) * (end - start) * page_tokens >= MIN_SAVED_KEYS:
+            mine = Segment(int(request[members[0]]), start * page_tokens, end * page_tokens, placed)
+            segments.append(mine)
+            parents.append(parent)
+            parent, start = len(segments) - 1, end
+        branch(members, start, end, parent)
+        if mine is not None:
+            mine.token_end = placed
+
+    def branch(members, start, depth, parent):
+        groups = {}
+        for member in members:
+            groups.setdefault(int(tables[request[member], depth]) if whole[member] > depth else -1 - int(member), []).append(member)
+        for group in groups.values():
+            if len(group) > 1:
+                walk(np.asarray(group), start, depth, parent)
+            else:
+                own(group[0], start, parent)
+
+    branch(np.arange(len(request)), 0, 0, -1)
+    leaves = np.asarray(leaves)
+    lengths = tokens[leaves]
+    within = np.arange(placed) - np.repeat(np.cumsum(lengths) - lengths, lengths)
+    return segments, parents, np.repeat(first[leaves], lengths) + within, np.repeat(sees[leaves], lengths), within, np.repeat(request[leaves], lengths)
+
+
+def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> np.ndarray:
+    """Into how many ranges each segment's keys go (``steps`` key steps, ``tiles`` tiles of rows), on a device that runs ``slots`` items at
+    once: none longer than an even share of all the steps."""
+    share = max(1, -(-int((tiles * steps).sum()) * kv_heads // slots))
+    return np.minimum(-(-steps // share), MAX_RANGES)
+
+
+class HostPlan:
+    """The plan's arrays on the host: ``items`` [n, 8] (simple ones, or narrow ones before wide ones), ``order``, ``part_start``, ``seen``,
+    ``extra``, ``table_of``."""
+
+    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int):
+        tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
+        if tables.ndim != 2 or q_start.ndim != 1 or contexts.ndim != 1 or len(contexts) == 0 or len(q_start) != len(contexts) + 1 or len(tables) < len(contexts):
+            raise PlanError("a block table row and a context per request, and where each request's tokens start")
+        if any(a.dtype.kind not in "iu" for a in (tables, q_start, contexts)):
+            raise PlanError("tables, starts and contexts are whole numbers")
+        q_start, contexts = q_start.astype(np.int64), contexts.astype(np.int64)
+        counts = np.diff(q_start)
+        if q_start[0] != 0 or (counts < 1).any() or (contexts < counts).any():
+            raise PlanError("every request brings a token or more, and its context holds them")
+        if page_tokens < 1 or int(contexts.max()) > tables.shape[1] * page_tokens or int(contexts.max()) > 0x7fffffff:
+            raise PlanError("a context reaches beyond its block table")
+        if kv_heads < 1 or heads < 1 or heads % kv_heads:
+            raise PlanError(f"heads ({heads}) must be a multiple of the key/value heads ({kv_heads})")
+        self.tokens, self.requests = int(q_start[-1]), len(contexts)
+        self.pages = int(-(-contexts.max() // page_tokens))
+        group = heads // kv_heads
+        segments, parents, order, seen, extra, table_of = find_segments(tables, q_start, contexts, page_tokens)
+        begin = np.array([s.key_begin for s in segments])
+        end = np.array([s.key_end for s in segments])
+        token_begin = np.array([s.token_begin for s in segments])
+        rows = (np.array([s.token_end for s in segments]) - token_begin) * group
+        if tensor_cores:
+            tile_rows = np.where(rows <= NARROW_ROWS, NARROW_ROWS, WIDE_ROWS)
+        else:
+            tile_rows = np.full(len(segments), SIMPLE_ROWS)
+        tiles, steps = -(-rows // tile_rows), -(-(end - begin) // KEY_STEP)
+        ranges = divide(tiles, steps, kv_heads, slots)
+        per_range = -(-steps // ranges)                  # steps of a range
+        ranges = -(-steps // per_range)
+        parts = np.zeros(self.tokens, dtype=np.int64)    # of each place
+        for i, s in enumerate(segments):
+            s.ranges = int(ranges[i])
+            s.part = 0 if parents[i] < 0 else segments[parents[i]].part + segments[parents[i]].ranges
+            parts[s.token_begin:s.token_end] = s.part + s.ranges
+        part = np.array([s.part for s in segments])
+        # the items: segment by segment, tile by tile, range by range
+        count = tiles * ranges
+        of = np.repeat(np.arange(len(segments)), count)
+        index = np.arange(len(of)) - np.repeat(np.cumsum(count) - count, count)
+        tile, rng = index // ranges[of], index % ranges[of]
+        items = np.zeros((len(of), 8), dtype=np.int32)
+        items[:, 0] = np.array([s.table for s in segments])[of]
+        items[:, 1] = begin[of] + rng * per_range[of] * KEY_STEP
+        items[:, 2] = np.minimum(end[of], items[:, 1] + per_range[of] * KEY_STEP)
+        items[:, 3] = token_begin[of]
+        items[:, 4] = tile * tile_rows[of]
+        items[:, 5] = np.minimum(rows[of] - items[:, 4], tile_rows[of])
+        items[:, 6] = part[of] + rng
+        wide = tile_rows[of] == WIDE_ROWS if tensor_cores else np.zeros(len(of), dtype=bool)
+        items = items[np.lexsort((items[:, 1] - items[:, 2], wide))]        # longest first within a kind
+        self.wide_items = int(wide.sum())
+        self.narrow_items = len(items) - self.wide_items if tensor_cores else 0
+        self.simple_items = 0 if tensor_cores else len(items)
+        self.items, self.segments, self.parents = items, segments, parents
+        self.order, self.seen, self.extra, self.table_of = (a.astype(np.int32) for a in (order, seen, extra, table_of))
+        self.part_start = np.concatenate([[0], np.cumsum(parts)]).astype(np.int32)
+        self.parts = int(self.part_start[-1])
+        # keys that the items read, and those that the requests' contexts hold
+        self.read_keys, self.context_keys = int((end - begin).sum()), int(contexts.sum())
+
+    def pack(self) -> np.ndarray:
+        """All arrays in one of int32, each starting on a multiple of four."""
+        arrays = (self.items.reshape(-1), self.order, self.part_start, self.seen, self.extra, self.table_of)
+        self.offsets, at = [], 0
+        for a in arrays:
+            self.offsets.append((at, len(a)))
+            at += -(-len(a) // 4) * 4
+        packed = np.zeros(at, dtype=np.int32)
+        for (where, n), a in zip(self.offsets, arrays):
+            packed[where:where + n] = a
+        return packed

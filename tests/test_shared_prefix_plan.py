@@ -1,0 +1,129 @@
+"""The plan of attention over shared prefixes, on the host: every (token, key) pair exactly once, through a page that the token's request
+holds there, whatever the tables share."""
+import random
+
+import numpy as np
+import pytest
+
+from sprout_lm_b200.prefix_plan import MEMBER_TOKENS, MIN_SAVED_KEYS, HostPlan, PlanError
+
+
+def batch(rng, requests, page, stems, counts, own):
+    """Tables, starts and contexts of requests whose leading pages come from common stems."""
+    fresh = iter(range(1000, 10 ** 9))
+    stems = [[next(fresh) for _ in range(n)] for n in stems]
+    stems.append(stems[0][:max(1, len(stems[0]) // 2)] + [next(fresh) for _ in range(9)])       # branches off the first
+    tables, contexts, tokens = [], [], []
+    for _ in range(requests):
+        stem = rng.choice(stems)
+        held = stem[:rng.randint(0, len(stem))] if rng.random() < 0.4 else stem
+        n = rng.choice(counts)
+        contexts.append(len(held) * page + rng.randint(0, own) + n)
+        tables.append(held + [next(fresh) for _ in range(-(-contexts[-1] // page) - len(held))])
+        tokens.append(n)
+    table = np.full((requests, max(map(len, tables))), -1, dtype=np.int32)
+    for row, pages in zip(table, tables):
+        row[:len(pages)] = pages
+    return table, np.concatenate([[0], np.cumsum(tokens)]), np.asarray(contexts)
+
+
+def covered(plan, tables, group):
+    """Per (place, head of the group): the (key, page) pairs of the plan's items."""
+    pairs = {}
+    for table, key_begin, key_end, token_begin, row_begin, rows, part, _ in plan.items.tolist():
+        for i in range(rows):
+            place, head = token_begin + (row_begin + i) // group, (row_begin + i) % group
+            assert 0 <= part < plan.part_start[place + 1] - plan.part_start[place]
+            pairs.setdefault((place, head), []).append((part, key_begin, key_end, table))
+    return pairs
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_every_key_once(seed):
+    rng = random.Random(seed)
+    page, group, kv_heads = rng.choice([1, 4, 8, 32]), rng.choice([1, 3, 7]), rng.choice([1, 2])
+    tables, q_start, contexts = batch(rng, rng.randint(1, 12), page, [rng.randint(1, 30) for _ in range(3)], rng.choice([[1], [1, 2, 5], [1, 16, 17, 40]]), 60)
+    for tensor_cores in (True, False):
+        plan = HostPlan(tables, q_start, contexts, page, group * kv_heads, kv_heads, tensor_cores, rng.choice([1, 8, 60, 600]))
+        assert sorted(plan.order.tolist()) == list(range(plan.tokens))
+        assert plan.simple_items + plan.narrow_items + plan.wide_items == len(plan.items) and (plan.simple_items > 0) != tensor_cores
+        pairs = covered(plan, tables, group)
+        for place, token in enumerate(plan.order.tolist()):
+            request = int(plan.table_of[place])
+            assert q_start[request] <= token < q_start[request + 1]
+            position = contexts[request] - (q_start[request + 1] - token)
+            assert plan.seen[place] + plan.extra[place] == position + 1 and 0 <= plan.extra[place] < MEMBER_TOKENS
+            for head in range(group):
+                held = sorted(pairs[place, head])
+                assert [part for part, *_ in held] == list(range(plan.part_start[place + 1] - plan.part_start[place]))     # a result each
+                keys = sorted((k, int(tables[table, k // page])) for _, begin, end, table in held for k in range(begin, end))
+                assert keys == [(k, int(tables[request, k // page])) for k in range(plan.seen[place])]
+
+
+def test_a_shared_prefix_is_read_once():
+    requests, page, prefix = 50, 16, 1600
+    tables = np.arange(requests * 110, dtype=np.int32).reshape(requests, 110)
+    tables[:, :100] = tables[0, :100]
+    plan = HostPlan(tables, np.arange(requests + 1), np.full(requests, prefix + 40), page, 14, 2, True, 592)
+    assert plan.read_keys == prefix + 40 * requests and plan.context_keys == requests * (prefix + 40)
+    assert len(plan.segments) == requests + 1 and plan.segments[0].token_end == requests
+
+
+def test_branching_prefixes():
+    """Two documents behind one system prompt, four requests each."""
+    page = 8
+    tables = np.arange(8 * 60, dtype=np.int32).reshape(8, 60)
+    tables[:, :20] = tables[0, :20]
+    tables[:4, 20:50], tables[4:, 20:50] = tables[0, 20:50], tables[7, 20:50]
+    plan = HostPlan(tables, np.arange(9), np.full(8, 60 * page), page, 4, 1, True, 592)
+    assert plan.read_keys == (20 + 2 * 30 + 8 * 10) * page
+    assert sorted(s.token_end - s.token_begin for s in plan.segments) == [1] * 8 + [4, 4, 8]
+
+
+def test_short_runs_stay_the_requests_own():
+    page = 8
+    tables = np.arange(2 * 20, dtype=np.int32).reshape(2, 20)
+    for shared in (MIN_SAVED_KEYS // page - 1, MIN_SAVED_KEYS // page):
+        tables[1, :shared] = tables[0, :shared]
+        plan = HostPlan(tables, [0, 1, 2], [100, 120], page, 4, 1, True, 592)
+        assert len(plan.segments) == (2 if shared * page < MIN_SAVED_KEYS else 3)
+
+
+def test_no_range_is_much_longer_than_an_even_share():
+    requests, page = 200, 16
+    tables = np.arange(requests * 1030, dtype=np.int32).reshape(requests, 1030)
+    tables[:, :1000] = tables[0, :1000]
+    plan = HostPlan(tables, np.arange(requests + 1), np.full(requests, 16000 + 200), page, 28, 4, True, 444)
+    lengths = plan.items[:, 2] - plan.items[:, 1]
+    total = int((-(-lengths // 128)).sum()) * 4
+    assert -(-int(lengths.max()) // 128) <= -(-total // 444)
+
+
+def test_one_token_of_context():
+    plan = HostPlan([[3]], [0, 1], [1], 16, 4, 2, True, 592)
+    assert plan.items[:, :7].tolist() == [[0, 0, 1, 0, 0, 2, 0]] and plan.parts == 1
+
+
+@pytest.mark.parametrize("change", [dict(q_start=[0, 1]), dict(q_start=[1, 2, 3]), dict(q_start=[0, 0, 2]), dict(contexts=[0, 5]), dict(contexts=[5, 33]),
+                                    dict(tables=[1, 2]), dict(tables=[[1, 2]]), dict(contexts=[5.0, 6.0]), dict(page_tokens=0), dict(heads=3), dict(contexts=[], q_start=[0])])
+def test_refusals(change):
+    given = dict(tables=[[1, 2], [1, 3]], q_start=[0, 1, 3], contexts=[5, 9], page_tokens=16, heads=4, kv_heads=2, tensor_cores=True, slots=10)
+    HostPlan(**given)
+    with pytest.raises(PlanError):
+        HostPlan(**{**given, **change})
+
+
+def test_kernel_binding_refuses_what_it_cannot_run():
+    import torch
+    from sprout_lm_b200 import kernels
+    for head_dim in (0, 7, 258):
+        with pytest.raises(kernels.KernelError, match="head_dim"):
+            kernels.shared_prefix_plan([[1]], [0, 1], [1], 16, 4, 2, head_dim, torch.bfloat16, "cpu")
+    with pytest.raises(kernels.KernelError, match="unsupported element type"):
+        kernels.shared_prefix_plan([[1]], [0, 1], [1], 16, 4, 2, 64, torch.float16, "cpu")
+    with pytest.raises(kernels.KernelError, match="context"):
+        kernels.shared_prefix_plan([[1]], [0, 1], [17], 16, 4, 2, 64, torch.bfloat16, "cpu")
+    plan = kernels.shared_prefix_plan([[1]], [0, 1], [1], 16, 4, 2, 64, torch.bfloat16, "cpu")
+    q = torch.zeros(1, 256, dtype=torch.bfloat16)
+    with pytest.raises(kernels.KernelError, match="CUDA tensor"):
+        kernels.attention_shared_prefix(q, q, q, q, q, plan, q, q)
