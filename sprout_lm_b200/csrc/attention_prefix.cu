@@ -7,8 +7,9 @@
 // as many passes over the same keys.  The requests' own keys are ranges of few rows, streams of keys and values.  Long ranges are
 // divided again, so that the launch fills the device.
 //
-// One launch computes the items' partial results (attention_prefix_simple_kernel: CUDA cores, 32-bit products, any head size and either
-// type; attention_prefix_mma_kernel: mma.sync, bfloat16, head sizes up to 128), one adds them up.
+// The items' partial results come from attention_prefix_simple_kernel (CUDA cores, 32-bit products, any head size and either type), or, for
+// bfloat16 and head sizes up to 128, from attention_prefix_mma_kernel (mma.sync) and, for many rows over whole pages, from
+// attention_prefix_tcgen05.cu; one launch adds them up.
 #include "attention_bf16.cuh"
 #include "attention_prefix.cuh"
 
@@ -460,20 +461,22 @@ int launch_merge(const Params& p, cudaStream_t stream) {
 
 }  // namespace
 
+int sprout_attention_prefix_tc(const sprout_prefix::Params& p, int items, cudaStream_t stream);      // attention_prefix_tcgen05.cu
+
 // Whether bfloat16 items of this head size run on the tensor cores.
 SPROUT_API int sprout_attention_prefix_mma_supported(int head_dim) { return head_dim % 16 == 0 && head_dim > 0 && head_dim <= 128; }
 
-// items: `simple_items` for the CUDA cores, or `narrow_items` of up to 16 rows and `wide_items` of up to 64 behind them.  `parts`: the
+// items: `simple_items` for the CUDA cores, or `matrix_items` of up to 256 rows, `narrow_items` of up to 16 and `wide_items` of up to 64.  `parts`: the
 // partial results in all; part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
 SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
-                                       const int* positions, const int* items, int simple_items, int narrow_items, int wide_items, const int* order,
+                                       const int* positions, const int* items, int simple_items, int matrix_items, int narrow_items, int wide_items, const int* order,
                                        const int* part_start, const int* seen, const int* extra, const int* table_of, float* part_out, float* part_sum, void* out, long long out_stride, int dtype, int tokens,
                                        int heads, int kv_heads, int head_dim, int page_tokens, int num_pages, int* status, cudaStream_t stream) {
   SPROUT_REQUIRE(q && k_cache && v_cache && block_table && positions && items && order && part_start && seen && extra && table_of && part_out && part_sum && out && status,
                  "attention_shared_prefix: null pointer");
   SPROUT_REQUIRE(tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
                  "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
-  SPROUT_REQUIRE(simple_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (simple_items > 0) != (narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
+  SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
   Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, (const Item*)items, order, part_start, seen, extra, table_of, part_out, (float2*)part_sum, out, out_stride,
            tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status};
@@ -483,6 +486,8 @@ SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const 
     SPROUT_REQUIRE(dtype == SPROUT_BF16 && sprout_attention_prefix_mma_supported(head_dim), "attention_shared_prefix: these sizes run on the CUDA cores");
     SPROUT_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0,
                    "attention_shared_prefix: rows must start on 16-byte boundaries");
+    if (matrix_items > 0 && sprout_attention_prefix_tc(p, matrix_items, stream)) return 1;
+    p.items += matrix_items;
     if (narrow_items > 0 && launch_mma_any<true>(p, narrow_items, stream)) return 1;
     p.items += narrow_items;
     if (wide_items > 0 && launch_mma_any<false>(p, wide_items, stream)) return 1;

@@ -40,7 +40,8 @@ _SIGNATURES = {
     "sprout_attention_simple": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
-    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "sprout_attention_prefix_tc_supported": [_I, _I],
+    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_attention_prefix_mma_supported": [_I],
     "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
@@ -992,8 +993,10 @@ def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, 
     if not 0 < head_dim <= 256 or head_dim % 2:
         raise KernelError(f"shared_prefix_plan: head_dim must be even and at most 256 (got {head_dim})")
     tensor_cores = dtype == torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 128
+    # pages that the tcgen05 kernel copies a box at a time
+    matrix_slots = _prefix_slots(0, False) // 2 if tensor_cores and head_dim in (64, 128) and (page_tokens in (8, 16, 32, 64) or page_tokens % 128 == 0) else 0
     try:
-        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, _prefix_slots(head_dim, tensor_cores))
+        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, _prefix_slots(head_dim, tensor_cores), matrix_slots)
     except PlanError as error:
         raise KernelError(f"shared_prefix_plan: {error}") from None
     packed = torch.from_numpy(host.pack())
@@ -1035,7 +1038,7 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     items, order, part_start, seen, extra, table_of = plan.pointers
     at = scratch.data_ptr()
     _run("sprout_attention_prefix", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(block_table, "block_table", torch.int32),
-         block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.narrow_items, host.wide_items, order, part_start, seen, extra, table_of,
+         block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.matrix_items, host.narrow_items, host.wide_items, order, part_start, seen, extra, table_of,
          at, at + 4 * host.parts * plan.heads * plan.head_dim, out.data_ptr(), out.stride(0), _dtype_code(q.dtype), host.tokens, plan.heads, plan.kv_heads,
          plan.head_dim, plan.page_tokens, k_cache.shape[0], _ptr(status, "status", torch.int32), _stream())
 

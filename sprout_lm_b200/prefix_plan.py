@@ -15,7 +15,8 @@ import numpy as np
 
 MEMBER_TOKENS = 16          # attention_prefix.cuh: MEMBER_TOKENS
 KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole steps
-NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS = 16, 64, 16      # rows of an item of each kind
+NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS, MATRIX_ROWS = 16, 64, 16, 256      # rows of an item of each kind
+MATRIX_FROM = 128           # rows of a segment
 MAX_RANGES = 64             # of a segment
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
 # the members read it themselves.
@@ -92,18 +93,38 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
     return segments, parents, np.repeat(first[leaves], lengths) + within, np.repeat(sees[leaves], lengths), within, np.repeat(request[leaves], lengths)
 
 
-def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> np.ndarray:
+def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int, start: float, step: float) -> np.ndarray:
     """Into how many ranges each segment's keys go (``steps`` key steps, ``tiles`` tiles of rows), on a device that runs ``slots`` items at
-    once: none longer than an even share of all the steps."""
-    share = max(1, -(-int((tiles * steps).sum()) * kv_heads // slots))
-    return np.minimum(-(-steps // share), MAX_RANGES)
+    once, an item of n steps taking ``start + n * step``: ranges of the length that makes the fewest full rounds of items the shortest."""
+    if not len(tiles):
+        return steps
+    items = lambda n: int((tiles * np.minimum(-(-steps // n), MAX_RANGES)).sum()) * kv_heads
+    best = None
+    for rounds in range(1, 9):
+        low, high = 1, int(steps.max())                  # the shortest ranges whose items fit that many rounds
+        if items(high) > rounds * slots:
+            continue
+        while low < high:
+            middle = (low + high) // 2
+            if items(middle) <= rounds * slots:
+                high = middle
+            else:
+                low = middle + 1
+        cost = -(-items(low) // slots) * (start + low * step)
+        if best is None or cost < best[0]:
+            best = cost, low
+        if low == 1:
+            break
+    # more segments than eight rounds hold: an even share of the steps
+    length = best[1] if best is not None else max(1, -(-int((tiles * steps).sum()) * kv_heads // (8 * slots)))
+    return np.minimum(-(-steps // length), MAX_RANGES)
 
 
 class HostPlan:
-    """The plan's arrays on the host: ``items`` [n, 8] (simple ones, or narrow ones before wide ones), ``order``, ``part_start``, ``seen``,
+    """The plan's arrays on the host: ``items`` [n, 8] (simple ones, or matrix, narrow and wide ones), ``order``, ``part_start``, ``seen``,
     ``extra``, ``table_of``."""
 
-    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int):
+    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0):
         tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
         if tables.ndim != 2 or q_start.ndim != 1 or contexts.ndim != 1 or len(contexts) == 0 or len(q_start) != len(contexts) + 1 or len(tables) < len(contexts):
             raise PlanError("a block table row and a context per request, and where each request's tokens start")
@@ -125,12 +146,19 @@ class HostPlan:
         end = np.array([s.key_end for s in segments])
         token_begin = np.array([s.token_begin for s in segments])
         rows = (np.array([s.token_end for s in segments]) - token_begin) * group
+        # the kinds: 0 a matrix product's worth of rows over whole pages, 1 few rows, 2 more; all of 1 on the CUDA cores
         if tensor_cores:
-            tile_rows = np.where(rows <= NARROW_ROWS, NARROW_ROWS, WIDE_ROWS)
+            kind = np.where(rows <= NARROW_ROWS, 1, 2)
+            if matrix_slots:
+                kind[(rows >= MATRIX_FROM) & (end % page_tokens == 0) & (begin % page_tokens == 0)] = 0
+            tile_rows = np.array([MATRIX_ROWS, NARROW_ROWS, WIDE_ROWS])[kind]
         else:
-            tile_rows = np.full(len(segments), SIMPLE_ROWS)
+            kind, tile_rows = np.ones(len(segments), dtype=np.int64), np.full(len(segments), SIMPLE_ROWS)
         tiles, steps = -(-rows // tile_rows), -(-(end - begin) // KEY_STEP)
-        ranges = divide(tiles, steps, kv_heads, slots)
+        ranges = np.empty(len(segments), dtype=np.int64)
+        matrix = kind == 0
+        ranges[matrix] = divide(tiles[matrix], steps[matrix], kv_heads, max(1, matrix_slots), 7.0, 2.4)
+        ranges[~matrix] = divide(tiles[~matrix], steps[~matrix], kv_heads, slots, 4.0, 1.5)
         per_range = -(-steps // ranges)                  # steps of a range
         ranges = -(-steps // per_range)
         parts = np.zeros(self.tokens, dtype=np.int64)    # of each place
@@ -152,11 +180,11 @@ class HostPlan:
         items[:, 4] = tile * tile_rows[of]
         items[:, 5] = np.minimum(rows[of] - items[:, 4], tile_rows[of])
         items[:, 6] = part[of] + rng
-        wide = tile_rows[of] == WIDE_ROWS if tensor_cores else np.zeros(len(of), dtype=bool)
-        items = items[np.lexsort((items[:, 1] - items[:, 2], wide))]        # longest first within a kind
-        self.wide_items = int(wide.sum())
-        self.narrow_items = len(items) - self.wide_items if tensor_cores else 0
-        self.simple_items = 0 if tensor_cores else len(items)
+        of_kind = kind[of]
+        items = items[np.lexsort((items[:, 1] - items[:, 2], of_kind))]     # longest first within a kind
+        counts = np.bincount(of_kind, minlength=3).tolist()
+        self.matrix_items, self.wide_items = counts[0], counts[2]
+        self.simple_items, self.narrow_items = (0, counts[1]) if tensor_cores else (counts[1], 0)
         self.items, self.segments, self.parents = items, segments, parents
         self.order, self.seen, self.extra, self.table_of = (a.astype(np.int32) for a in (order, seen, extra, table_of))
         self.part_start = np.concatenate([[0], np.cumsum(parts)]).astype(np.int32)

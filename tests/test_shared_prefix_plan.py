@@ -44,9 +44,9 @@ def test_every_key_once(seed):
     page, group, kv_heads = rng.choice([1, 4, 8, 32]), rng.choice([1, 3, 7]), rng.choice([1, 2])
     tables, q_start, contexts = batch(rng, rng.randint(1, 12), page, [rng.randint(1, 30) for _ in range(3)], rng.choice([[1], [1, 2, 5], [1, 16, 17, 40]]), 60)
     for tensor_cores in (True, False):
-        plan = HostPlan(tables, q_start, contexts, page, group * kv_heads, kv_heads, tensor_cores, rng.choice([1, 8, 60, 600]))
+        plan = HostPlan(tables, q_start, contexts, page, group * kv_heads, kv_heads, tensor_cores, rng.choice([1, 8, 60, 600]), rng.choice([0, 1, 148]))
         assert sorted(plan.order.tolist()) == list(range(plan.tokens))
-        assert plan.simple_items + plan.narrow_items + plan.wide_items == len(plan.items) and (plan.simple_items > 0) != tensor_cores
+        assert plan.simple_items + plan.matrix_items + plan.narrow_items + plan.wide_items == len(plan.items) and (plan.simple_items > 0) != tensor_cores
         pairs = covered(plan, tables, group)
         for place, token in enumerate(plan.order.tolist()):
             request = int(plan.table_of[place])
@@ -89,14 +89,17 @@ def test_short_runs_stay_the_requests_own():
         assert len(plan.segments) == (2 if shared * page < MIN_SAVED_KEYS else 3)
 
 
-def test_no_range_is_much_longer_than_an_even_share():
+@pytest.mark.parametrize("matrix_slots", [0, 148])
+def test_no_range_is_much_longer_than_an_even_share(matrix_slots):
+    """A long prefix for many requests is divided so far that its items fill a few rounds of the device evenly."""
     requests, page = 200, 16
     tables = np.arange(requests * 1030, dtype=np.int32).reshape(requests, 1030)
     tables[:, :1000] = tables[0, :1000]
-    plan = HostPlan(tables, np.arange(requests + 1), np.full(requests, 16000 + 200), page, 28, 4, True, 444)
-    lengths = plan.items[:, 2] - plan.items[:, 1]
-    total = int((-(-lengths // 128)).sum()) * 4
-    assert -(-int(lengths.max()) // 128) <= -(-total // 444)
+    plan = HostPlan(tables, np.arange(requests + 1), np.full(requests, 16000 + 200), page, 28, 4, True, 444, matrix_slots)
+    prefix = plan.items[plan.items[:, 5] > 16]
+    assert (plan.matrix_items > 0) == (matrix_slots > 0) and len(prefix) == (plan.matrix_items or plan.wide_items)
+    lengths = -(-(prefix[:, 2] - prefix[:, 1]) // 128)
+    assert int(lengths.max()) * (matrix_slots or 444) <= 1.3 * int(lengths.sum()) * 4
 
 
 def test_one_token_of_context():
