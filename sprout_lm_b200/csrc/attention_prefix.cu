@@ -182,12 +182,17 @@ attention_prefix_mma_kernel(const Params p) {
   const Item item = p.items[blockIdx.x];
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
-  const __nv_bfloat16* q = (const __nv_bfloat16*)p.q;
-  for (int idx = tid; idx < L::ROWS * PIECES; idx += MMA_THREADS) {
-    const int i = idx / PIECES, c = idx % PIECES;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (i < item.rows) v = *(const uint4*)(q + (size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * HD + c * 8);
-    *(uint4*)(sQ + i * STRIDE + c * 8) = v;
+  // the query rows, their offsets first (in the room of the keys' offsets): each is behind a read of its own
+  if (tid < L::ROWS)
+    rows[tid] = tid < item.rows ? (long long)p.order[place_of_row(item, tid, group)] * p.q_stride + (long long)head_of_row(item, tid, group, g) * HD : -1;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < (L::ROWS * PIECES + MMA_THREADS - 1) / MMA_THREADS; k++) {
+    const int idx = tid + k * MMA_THREADS, i = idx / PIECES, c = idx % PIECES;
+    if (i < L::ROWS) {
+      const long long at = rows[i];
+      *(uint4*)(sQ + i * STRIDE + c * 8) = at >= 0 ? *(const uint4*)((const __nv_bfloat16*)p.q + at + c * 8) : make_uint4(0, 0, 0, 0);
+    }
   }
   const int tile = NARROW ? 0 : warp, gr = lane >> 2, qc = lane & 3;
   const int row0 = tile * 16 + gr, row1 = row0 + 8;    // of the item, this lane's in the fragments

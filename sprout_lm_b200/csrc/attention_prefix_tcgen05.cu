@@ -24,10 +24,14 @@ using namespace sprout_prefix;
 namespace {
 
 constexpr int ROWS = 128, KEYS = 64;        // rows of a Q tile (tensor-memory lanes), keys of a tile
-constexpr int THREADS = 384;                // warpgroup 0: key copies, MMA, value copies (one warp idle); 1, 2: softmax of Q tile 0, 1
+constexpr int THREADS = 384;                // warpgroup 0: key copies, MMA, value copies, MMA; 1, 2: softmax of Q tile 0, 1
 constexpr int ATOM = 128 * 128;             // bytes of a [128 rows, 64 bf16] swizzled tile
 constexpr int KV_ATOM = KEYS * 128;         // and of [KEYS rows, 64 bf16]
 constexpr int TMEM_COLS = 512;
+#ifndef PREFIX_GROWTH
+#define PREFIX_GROWTH 8.0f
+#endif
+constexpr float GROWTH = PREFIX_GROWTH;
 constexpr int MARKS = 16;                   // tiles whose missing boxes are remembered: more than the ring's stages and the two tiles ahead
 
 template <int DIM>
@@ -72,11 +76,6 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   }
   // rows of a stage that no copy fills must hold finite numbers: their probabilities are zero, and zero times a NaN is not
   for (int i = tid; i < NS * L::KV_BYTES / 16; i += THREADS) ((uint4*)sV)[i] = make_uint4(0, 0, 0, 0);
-  if (tid == 0) {
-    for (int i = 0; i < BARS; i++) mbar_init(&bars[i], &bars[i] >= p_full && &bars[i] < o_done ? 4 : 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
   pdl_launch_dependents();
   pdl_wait();
@@ -87,14 +86,29 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   const bool two = item.rows > ROWS;                   // the second Q tile has rows
   const int n_tiles = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
 
-  // Q rows -> shared memory, K-major with the 128-byte swizzle (16-byte chunk c of row r at position c ^ (r & 7))
-  constexpr int CHUNKS = DIM / 8;
-  for (int idx = tid; idx < 2 * ROWS * CHUNKS; idx += THREADS) {
-    const int i = idx / CHUNKS, c = idx % CHUNKS, q = i >> 7, row = i & (ROWS - 1);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (i < item.rows)
-      v = *(const uint4*)((const __nv_bfloat16*)p.q + (size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * DIM + c * 8);
-    *(uint4*)(sQ + q * L::Q_BYTES + (c >> 3) * ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+  // Q rows -> shared memory, K-major with the 128-byte swizzle (16-byte chunk c of row r at position c ^ (r & 7)); the rows' addresses first, in
+  // the room of the first keys (a thread that finds its rows' one after the other waits for two reads each time: 5.6 us in all)
+  const __nv_bfloat16** from = (const __nv_bfloat16**)sK;
+  if (tid < 2 * ROWS)
+    from[tid] = tid < item.rows ? (const __nv_bfloat16*)p.q + (size_t)p.order[place_of_row(item, tid, group)] * p.q_stride + (size_t)head_of_row(item, tid, group, g) * DIM : nullptr;
+  if (tid == THREADS - 1) {
+    for (int i = 0; i < BARS; i++) {
+      const bool writes_p = &bars[i] >= p_full && &bars[i] < o_done, empty = (&bars[i] >= k_empty && &bars[i] < v_full) || (&bars[i] >= v_empty && &bars[i] < s_full);
+      mbar_init(&bars[i], writes_p ? 4 : empty && two ? 2 : 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  constexpr int CHUNKS = DIM / 8, EACH = (2 * ROWS * CHUNKS + THREADS - 1) / THREADS;
+#pragma unroll
+  for (int k = 0; k < EACH; k++) {
+    const int idx = tid + k * THREADS, i = idx / CHUNKS, c = idx % CHUNKS, q = i >> 7, row = i & (ROWS - 1);
+    if (i < 2 * ROWS) {
+      const __nv_bfloat16* at = from[i];
+      const uint4 v = at != nullptr ? *(const uint4*)(at + c * 8) : make_uint4(0, 0, 0, 0);
+      *(uint4*)(sQ + q * L::Q_BYTES + (c >> 3) * ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+    }
   }
   fence_proxy_async();
   tc_fence_before();
@@ -146,41 +160,42 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
             tma_load_2d_addr(stages + s * L::KV_BYTES + a * KV_ATOM + lane * box_rows * 128, map, smem_u32(&full[s]), a * 64, row_at);
         issued = j + 1;
       }
-    } else if (warp == 1) {
-      // ---------------- MMA issuer: S(0) and S(1) of both Q tiles, then for every key tile and Q tile  [P(j)] P V(j), S(j + 2).
-      // The last product that reads a stage releases it.  The whole warp walks the loop on values that are the same in all lanes (they
-      // stay in uniform registers, where the products take them from); one elected lane issues.
+    } else if (warp == 1 || two) {
+      // ---------------- MMA issuers, warp 1 for the first Q tile and warp 3 for the second: S(0) and S(1), then for every key tile
+      // [P(j)] P V(j), S(j + 2).  (One warp for both took 2,300 cycles a tile, 1,400 of them to issue 24 products and the rest in waits
+      // that found what they waited for.)  The products that read a stage release it.  The whole warp walks the loop on values that are
+      // the same in all lanes (they stay in uniform registers, where the products take them from); one elected lane issues.
+      const int q = __shfl_sync(0xffffffffu, warp >> 1, 0);
       const uint32_t idesc_s = umma_idesc(ROWS, KEYS), idesc_o = umma_idesc_b_mn(ROWS, DIM);
       const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
       const int tiles = __shfl_sync(0xffffffffu, n_tiles, 0);
-      const bool both = __shfl_sync(0xffffffffu, (int)two, 0) != 0;
-      const uint32_t k0 = (smem_u32(sK) & 0x3FFFF) >> 4, v0 = (smem_u32(sV) & 0x3FFFF) >> 4, q0 = (smem_u32(sQ) & 0x3FFFF) >> 4;
+      const uint32_t k0 = (smem_u32(sK) & 0x3FFFF) >> 4, v0 = (smem_u32(sV) & 0x3FFFF) >> 4, q0 = ((smem_u32(sQ) & 0x3FFFF) + q * L::Q_BYTES) >> 4;
       const uint32_t bar0 = smem_u32(bars);
       auto bar_of = [&](const uint64_t* bar) { return bar0 + (uint32_t)((const char*)bar - (const char*)bars); };
       auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_addr(bar, parity, abort_flag)) != 0; };
       // descriptors: the start address / 16 in the low word, layout constants (umma_smem_desc, umma_smem_desc_mn) in the high one
       constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
-      auto issue_s = [&](int q, int stage, int buf) {
+      auto issue_s = [&](int stage, int buf) {
         if (elect_one()) {
 #pragma unroll
           for (int a = 0; a < DIM / 64; a++)
 #pragma unroll
             for (int kk = 0; kk < 4; kk++)
-              umma_bf16_words(tmem + (q * 2 + buf) * KEYS, q0 + (q * L::Q_BYTES + a * ATOM) / 16 + 2 * kk, DESC_HI,
+              umma_bf16_words(tmem + (q * 2 + buf) * KEYS, q0 + a * (ATOM / 16) + 2 * kk, DESC_HI,
                               k0 + stage * (L::KV_BYTES / 16) + a * (KV_ATOM / 16) + 2 * kk, DESC_HI, idesc_s, (a | kk) != 0);
           umma_commit_addr(bar_of(s_full) + (q * 2 + buf) * 8);
-          if (q == 1 || !both) umma_commit_addr(bar_of(k_empty) + stage * 8);
+          umma_commit_addr(bar_of(k_empty) + stage * 8);
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int q, int stage, int buf, bool first) {
+      auto issue_pv = [&](int stage, int buf, bool first) {
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < KEYS / 16; ks++)
             umma_bf16_from_tmem_words(tmem + L::O_COLUMN + q * DIM, tmem + (q * 2 + buf) * KEYS + ks * 8,
                                       (v0 + stage * (L::KV_BYTES / 16) + ks * 128) | ((uint32_t)(KV_ATOM >> 4) << 16), DESC_HI, idesc_o, !first || ks != 0);
           umma_commit_addr(bar_of(o_done) + (q * 2 + buf) * 8);
-          if (q == 1 || !both) umma_commit_addr(bar_of(v_empty) + stage * 8);
+          umma_commit_addr(bar_of(v_empty) + stage * 8);
         }
         __syncwarp();
       };
@@ -191,8 +206,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         ok = wait(bar_of(k_full) + k_stage * 8, 0);
         if (!ok) break;
         tc_fence_after();
-        issue_s(0, k_stage, j);
-        if (both) issue_s(1, k_stage, j);
+        issue_s(k_stage, j);
         k_stage++;
       }
       for (int j = 0; j < tiles && ok; j++) {
@@ -201,13 +215,11 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         ok = wait(bar_of(v_full) + v_stage * 8, v_parity);
         if (ok && j + 2 < tiles) ok = wait(bar_of(k_full) + k_stage * 8, k_parity);
         if (!ok) break;
-        for (int q = 0; q < (both ? 2 : 1); q++) {
-          ok = wait(bar_of(p_full) + (q * 2 + buf) * 8, parity);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(q, v_stage, buf, j == 0);
-          if (j + 2 < tiles) issue_s(q, k_stage, buf);
-        }
+        ok = wait(bar_of(p_full) + (q * 2 + buf) * 8, parity);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(v_stage, buf, j == 0);
+        if (j + 2 < tiles) issue_s(k_stage, buf);
         if (++k_stage == NS) { k_stage = 0; k_parity ^= 1; }
         if (++v_stage == NS) { v_stage = 0; v_parity ^= 1; }
       }
@@ -258,8 +270,8 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
           mx[3] = max3(mx[3], __uint_as_float(sc[c][k + 6]), __uint_as_float(sc[c][k + 7]));
         }
       const float n = max3(m, fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      // the maximum moved: bring O and the sum to it
-      const bool moved = n != m;
+      // the maximum moved: bring O and the sum to it (by less than 2^GROWTH: they stay, and weights are up to that large)
+      const bool moved = m == -INFINITY ? n != m : (n - m) * scale_log2 > GROWTH;
       if (__any_sync(0xffffffffu, moved)) {
         const float alpha = !moved ? 1.0f : m == -INFINITY ? 0.f : exp2_fast((m - n) * scale_log2);
         if (moved) m = n;
@@ -283,18 +295,26 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       }
       const float base = m == -INFINITY ? 0.f : m * scale_log2;
       const uint64_t nbase2 = pair(-base, -base);
-      // probabilities, their sum, and P as bfloat16 into tensor memory
+      // probabilities, P as bfloat16 into tensor memory, and their sum: each a pass over the registers, so that no instruction waits for the one
+      // before it
 #pragma unroll
-      for (int c = 0; c < KEYS / 32; c++) {
-        uint32_t packed[16];
+      for (int c = 0; c < KEYS / 32; c++)
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           float x0, x1;
           unpair(fma2(pair(sc[c][k], sc[c][k + 1]), scale2, nbase2), x0, x1);
-          const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
-          __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+          sc[c][k] = __float_as_uint(x0);
+          sc[c][k + 1] = __float_as_uint(x1);
+        }
+#pragma unroll
+      for (int c = 0; c < KEYS / 32; c++) {
+#pragma unroll
+        for (int k = 0; k < 32; k++) sc[c][k] = __float_as_uint(exp2_fast(__uint_as_float(sc[c][k])));
+        uint32_t packed[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(sc[c][k]), __uint_as_float(sc[c][k + 1]));
           packed[k >> 1] = *(uint32_t*)&h;
-          l2 = add2(l2, pair(p0, p1));
         }
         tmem_store16(s_addr + c * 16, packed);
       }
@@ -302,6 +322,12 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[q * 2 + (j & 1)]);
+      uint64_t sums[4] = {l2, 0ull, 0ull, 0ull};       // while the product that P goes into runs
+#pragma unroll
+      for (int c = 0; c < KEYS / 32; c++)
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) sums[(k >> 1) & 3] = add2(sums[(k >> 1) & 3], pair(sc[c][k], sc[c][k + 1]));
+      l2 = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
     }
     if (ok && my_tiles > 0) {
       ok = !*abort_flag && mbar_wait(&o_done[q * 2 + ((my_tiles - 1) & 1)], ((my_tiles - 1) >> 1) & 1, abort_flag);
