@@ -186,13 +186,18 @@ attention_prefix_mma_kernel(const Params p) {
   if (tid < L::ROWS)
     rows[tid] = tid < item.rows ? (long long)p.order[place_of_row(item, tid, group)] * p.q_stride + (long long)head_of_row(item, tid, group, g) * HD : -1;
   __syncthreads();
+  constexpr int EACH = (L::ROWS * PIECES + MMA_THREADS - 1) / MMA_THREADS;
+  uint4 held[EACH];                                    // all on their way before the first is stored
 #pragma unroll
-  for (int k = 0; k < (L::ROWS * PIECES + MMA_THREADS - 1) / MMA_THREADS; k++) {
-    const int idx = tid + k * MMA_THREADS, i = idx / PIECES, c = idx % PIECES;
-    if (i < L::ROWS) {
-      const long long at = rows[i];
-      *(uint4*)(sQ + i * STRIDE + c * 8) = at >= 0 ? *(const uint4*)((const __nv_bfloat16*)p.q + at + c * 8) : make_uint4(0, 0, 0, 0);
-    }
+  for (int k = 0; k < EACH; k++) {
+    const int idx = tid + k * MMA_THREADS;
+    const long long at = rows[min(idx / PIECES, L::ROWS - 1)];
+    held[k] = at >= 0 ? *(const uint4*)((const __nv_bfloat16*)p.q + at + idx % PIECES * 8) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int k = 0; k < EACH; k++) {
+    const int idx = tid + k * MMA_THREADS;
+    if (idx < L::ROWS * PIECES) *(uint4*)(sQ + idx / PIECES * STRIDE + idx % PIECES * 8) = held[k];
   }
   const int tile = NARROW ? 0 : warp, gr = lane >> 2, qc = lane & 3;
   const int row0 = tile * 16 + gr, row1 = row0 + 8;    // of the item, this lane's in the fragments

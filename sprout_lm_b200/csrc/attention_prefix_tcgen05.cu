@@ -9,8 +9,7 @@
 //   O += P V     tcgen05.mma with P from tensor memory, V as it lies in the cache (MN-major); O stays in tensor memory
 //
 // as the prompt kernel of attention_maps_tcgen05.cu does, but every row sees every key, the rows are gathered from many requests, and O
-// leaves unnormalised with its maximum and sum.  A row's O and sum follow its maximum.  The exponentials (16 an SM and cycle) and the
-// products take about as long, a thousand cycles a tile of 256 x 64 each, and run side by side.
+// leaves unnormalised with its maximum and sum.  A row's O and sum follow its maximum only once it has grown by 2^GROWTH.
 //
 // K and V come by TMA, one box per page, through a ring of stages.  Every mbarrier wait is bounded: on a timeout the CTA sets
 // the status word, waits (bounded) for its copies in flight, frees its tensor memory and returns.
@@ -28,10 +27,7 @@ constexpr int THREADS = 384;                // warpgroup 0: key copies, MMA, val
 constexpr int ATOM = 128 * 128;             // bytes of a [128 rows, 64 bf16] swizzled tile
 constexpr int KV_ATOM = KEYS * 128;         // and of [KEYS rows, 64 bf16]
 constexpr int TMEM_COLS = 512;
-#ifndef PREFIX_GROWTH
-#define PREFIX_GROWTH 8.0f
-#endif
-constexpr float GROWTH = PREFIX_GROWTH;
+constexpr float GROWTH = 8.f;                // log2 of how far a row's weights may grow before its O and sum follow the maximum
 constexpr int MARKS = 16;                   // tiles whose missing boxes are remembered: more than the ring's stages and the two tiles ahead
 
 template <int DIM>
@@ -44,6 +40,29 @@ struct Layout {
   static_assert(O_COLUMN + 2 * DIM <= TMEM_COLS, "tensor memory columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x0 and 2^x1 for x <= 8 by packed products in place of the special function unit, to 4e-6 (the weights that they become have 2^-8): x = n + f
+// with |f| <= 1/2, 2^f by its Taylor polynomial, n into the exponent; results below 2^-126 are 2^-126.
+__device__ __forceinline__ void exp2_by_products(float x0, float x1, float& p0, float& p1) {
+  const uint64_t x = pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t t = add2(x, pair(12582912.f, 12582912.f));        // 1.5 * 2^23: the sum's low bits are x rounded to a whole number
+  const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
+  uint64_t r = fma2(f, pair(1.3333558e-3f, 1.3333558e-3f), pair(9.6181291e-3f, 9.6181291e-3f));
+  r = fma2(r, f, pair(5.5504109e-2f, 5.5504109e-2f));
+  r = fma2(r, f, pair(0.24022651f, 0.24022651f));
+  r = fma2(r, f, pair(0.69314718f, 0.69314718f));
+  r = fma2(r, f, pair(1.f, 1.f));
+  float r0, r1, t0, t1;
+  unpair(r, r0, r1);
+  unpair(t, t0, t1);
+  p0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
+  p1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
+}
 
 template <int DIM>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -87,7 +106,8 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   const int n_tiles = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
 
   // Q rows -> shared memory, K-major with the 128-byte swizzle (16-byte chunk c of row r at position c ^ (r & 7)); the rows' addresses first, in
-  // the room of the first keys (a thread that finds its rows' one after the other waits for two reads each time: 5.6 us in all)
+  // the room of the first keys (a thread that finds them one after the other, or stores a row before it asks for the next, waits for every
+  // read: 4 to 6 us in all)
   const __nv_bfloat16** from = (const __nv_bfloat16**)sK;
   if (tid < 2 * ROWS)
     from[tid] = tid < item.rows ? (const __nv_bfloat16*)p.q + (size_t)p.order[place_of_row(item, tid, group)] * p.q_stride + (size_t)head_of_row(item, tid, group, g) * DIM : nullptr;
@@ -101,14 +121,17 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   }
   __syncthreads();
   constexpr int CHUNKS = DIM / 8, EACH = (2 * ROWS * CHUNKS + THREADS - 1) / THREADS;
+  uint4 held[EACH];                                    // all on their way before the first is stored
+#pragma unroll
+  for (int k = 0; k < EACH; k++) {
+    const int idx = tid + k * THREADS, i = min(idx / CHUNKS, 2 * ROWS - 1);
+    const __nv_bfloat16* at = from[i];
+    held[k] = at != nullptr ? *(const uint4*)(at + idx % CHUNKS * 8) : make_uint4(0, 0, 0, 0);
+  }
 #pragma unroll
   for (int k = 0; k < EACH; k++) {
     const int idx = tid + k * THREADS, i = idx / CHUNKS, c = idx % CHUNKS, q = i >> 7, row = i & (ROWS - 1);
-    if (i < 2 * ROWS) {
-      const __nv_bfloat16* at = from[i];
-      const uint4 v = at != nullptr ? *(const uint4*)(at + c * 8) : make_uint4(0, 0, 0, 0);
-      *(uint4*)(sQ + q * L::Q_BYTES + (c >> 3) * ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
-    }
+    if (i < 2 * ROWS) *(uint4*)(sQ + q * L::Q_BYTES + (c >> 3) * ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = held[k];
   }
   fence_proxy_async();
   tc_fence_before();
@@ -259,19 +282,15 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
           for (int k = 0; k < 32; k++)
             if (c * 32 + k >= there || (marks >> ((c * 32 + k) / box_rows) & 1)) sc[c][k] = 0xff800000u;          // -inf
       }
+      // the maximum, NaN if there is one (the exponentials by products would lose it)
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < KEYS / 32; c++)
 #pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          mx[0] = max3(mx[0], __uint_as_float(sc[c][k]), __uint_as_float(sc[c][k + 1]));
-          mx[1] = max3(mx[1], __uint_as_float(sc[c][k + 2]), __uint_as_float(sc[c][k + 3]));
-          mx[2] = max3(mx[2], __uint_as_float(sc[c][k + 4]), __uint_as_float(sc[c][k + 5]));
-          mx[3] = max3(mx[3], __uint_as_float(sc[c][k + 6]), __uint_as_float(sc[c][k + 7]));
-        }
-      const float n = max3(m, fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      // the maximum moved: bring O and the sum to it (by less than 2^GROWTH: they stay, and weights are up to that large)
-      const bool moved = m == -INFINITY ? n != m : (n - m) * scale_log2 > GROWTH;
+        for (int k = 0; k < 32; k += 2) mx[(k >> 1) & 3] = max3_nan(mx[(k >> 1) & 3], __uint_as_float(sc[c][k]), __uint_as_float(sc[c][k + 1]));
+      const float n = max3_nan(max3_nan(m, mx[0], mx[1]), mx[2], mx[3]);
+      // it moved: bring O and the sum to it (by less than 2^GROWTH: they stay, and weights are up to that large)
+      const bool moved = m == -INFINITY ? n != m : !((n - m) * scale_log2 <= GROWTH);
       if (__any_sync(0xffffffffu, moved)) {
         const float alpha = !moved ? 1.0f : m == -INFINITY ? 0.f : exp2_fast((m - n) * scale_log2);
         if (moved) m = n;
@@ -295,39 +314,29 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       }
       const float base = m == -INFINITY ? 0.f : m * scale_log2;
       const uint64_t nbase2 = pair(-base, -base);
-      // probabilities, P as bfloat16 into tensor memory, and their sum: each a pass over the registers, so that no instruction waits for the one
-      // before it
+      // probabilities, their sum, and P as bfloat16 into tensor memory
+      uint64_t sums[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < KEYS / 32; c++)
+      for (int c = 0; c < KEYS / 32; c++) {
+        uint32_t packed[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           float x0, x1;
           unpair(fma2(pair(sc[c][k], sc[c][k + 1]), scale2, nbase2), x0, x1);
-          sc[c][k] = __float_as_uint(x0);
-          sc[c][k + 1] = __float_as_uint(x1);
-        }
-#pragma unroll
-      for (int c = 0; c < KEYS / 32; c++) {
-#pragma unroll
-        for (int k = 0; k < 32; k++) sc[c][k] = __float_as_uint(exp2_fast(__uint_as_float(sc[c][k])));
-        uint32_t packed[16];
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(sc[c][k]), __uint_as_float(sc[c][k + 1]));
+          float p0, p1;
+          if ((k & 6) == 6) exp2_by_products(x0, x1, p0, p1);
+          else { p0 = exp2_fast(x0); p1 = exp2_fast(x1); }
+          __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
           packed[k >> 1] = *(uint32_t*)&h;
+          sums[(k >> 1) & 1] = add2(sums[(k >> 1) & 1], pair(p0, p1));
         }
         tmem_store16(s_addr + c * 16, packed);
       }
+      l2 = add2(l2, add2(sums[0], sums[1]));
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[q * 2 + (j & 1)]);
-      uint64_t sums[4] = {l2, 0ull, 0ull, 0ull};       // while the product that P goes into runs
-#pragma unroll
-      for (int c = 0; c < KEYS / 32; c++)
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) sums[(k >> 1) & 3] = add2(sums[(k >> 1) & 3], pair(sc[c][k], sc[c][k + 1]));
-      l2 = add2(add2(sums[0], sums[1]), add2(sums[2], sums[3]));
     }
     if (ok && my_tiles > 0) {
       ok = !*abort_flag && mbar_wait(&o_done[q * 2 + ((my_tiles - 1) & 1)], ((my_tiles - 1) >> 1) & 1, abort_flag);
