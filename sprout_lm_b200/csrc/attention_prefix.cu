@@ -43,8 +43,7 @@ attention_prefix_simple_kernel(const Params p) {
   float* s_m = sP + SIMPLE_ROWS * (SIMPLE_KEYS + 4);   // [16] maxima, sums, what a pass multiplies the outputs by
   float* s_l = s_m + SIMPLE_ROWS;
   float* s_a = s_l + SIMPLE_ROWS;
-  pdl_launch_dependents();
-  pdl_wait();
+  begin_items(p);
   const Item item = p.items[blockIdx.x];
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
@@ -145,6 +144,7 @@ attention_prefix_simple_kernel(const Params p) {
       for (int c = 0; c < 4; c++) if (b * 64 + c0 + c < p.head_dim) p.part_out[at * p.head_dim + b * 64 + c0 + c] = acc[a][b][c];
     if (tid % 16 == 0) p.part_sum[at] = make_float2(s_m[i], s_l[i]);
   }
+  end_items(p);
 }
 
 // ------------------------------------------------------------------ mma.sync
@@ -155,15 +155,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Keys and values in passes of 128 through shared memory (cp.async), three or more CTAs an SM so that one's copies run under the others'
-// products.  NARROW (an item of up to 16 rows): the rows are one tile of the MMA, each of the 4 warps takes 32 keys of a pass, and the
-// warps' results are merged at the end.  Else an item has up to 64 rows, 16 a warp, and every warp takes all keys.
-constexpr int MMA_KEYS = 128, MMA_THREADS = 128;
+// Keys and values in steps through shared memory (cp.async), three or four CTAs an SM.  The next step's keys are asked for when this
+// step's scores are done, its values when this step's outputs are, so that a buffer of each is always on its way or in use.  NARROW (an
+// item of up to 16 rows): the rows are one tile of the MMA, each of the 4 warps takes 32 of a step's 128 keys, and the warps' results are
+// merged at the end.  Else an item has up to 64 rows, 16 a warp, and every warp takes all 64 keys of a step.
+constexpr int MMA_THREADS = 128;
 
 template <int HD, bool NARROW>
 struct MmaShape {
-  static constexpr int ROWS = NARROW ? 16 : 64, STRIDE = HD + 8, CHUNK = NARROW ? 32 : 64;    // CHUNK: keys between two looks at the maximum
-  static constexpr size_t SMEM = (size_t)(ROWS + 2 * MMA_KEYS) * STRIDE * 2 + MMA_KEYS * sizeof(long long);
+  static constexpr int ROWS = NARROW ? 16 : 64, KEYS = NARROW ? 128 : 64, STRIDE = HD + 8, CHUNK = NARROW ? 32 : 64;      // CHUNK: a warp's keys of a step
+  static constexpr size_t SMEM = (size_t)(ROWS + 2 * KEYS) * STRIDE * 2 + 2 * KEYS * sizeof(long long);
   static constexpr int CTAS = HD > 96 ? 3 : 4;
 };
 
@@ -171,27 +172,43 @@ template <int HD, bool NARROW>
 __global__ void __launch_bounds__(MMA_THREADS, MmaShape<HD, NARROW>::CTAS)
 attention_prefix_mma_kernel(const Params p) {
   using L = MmaShape<HD, NARROW>;
-  constexpr int STRIDE = L::STRIDE, PIECES = HD / 8, CHUNK = L::CHUNK;
+  constexpr int STRIDE = L::STRIDE, PIECES = HD / 8, CHUNK = L::CHUNK, KEYS = L::KEYS;
   extern __shared__ __align__(16) uint8_t mma_shared[];
-  long long* rows = (long long*)mma_shared;            // [128] element offsets, -1: no such key
-  __nv_bfloat16* sQ = (__nv_bfloat16*)(rows + MMA_KEYS);           // [ROWS][STRIDE]
-  __nv_bfloat16* sK = sQ + L::ROWS * STRIDE;           // [128][STRIDE]
-  __nv_bfloat16* sV = sK + MMA_KEYS * STRIDE;
-  pdl_launch_dependents();
-  pdl_wait();
+  long long* rows = (long long*)mma_shared;            // [2][KEYS] element offsets of this step's keys and the next one's, -1: no such key
+  __nv_bfloat16* sQ = (__nv_bfloat16*)(rows + 2 * KEYS);           // [ROWS][STRIDE]
+  __nv_bfloat16* sK = sQ + L::ROWS * STRIDE;           // [KEYS][STRIDE]
+  __nv_bfloat16* sV = sK + KEYS * STRIDE;
+  begin_items(p);
   const Item item = p.items[blockIdx.x];
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
-  // the query rows, their offsets first (in the room of the keys' offsets): each is behind a read of its own
+  auto look_up = [&](int base) { return tid < KEYS && base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1ll; };
+  auto fetch = [&](__nv_bfloat16* to, const void* cache, const long long* at) {
+#pragma unroll
+    for (int k = 0; k < (KEYS * PIECES + MMA_THREADS - 1) / MMA_THREADS; k++) {
+      const int idx = tid + k * MMA_THREADS, j = idx / PIECES, c = idx % PIECES;
+      if (KEYS * PIECES % MMA_THREADS != 0 && j >= KEYS) break;
+      const long long from = at[j];
+      if (from >= 0) cp_async16(to + j * STRIDE + c * 8, (const __nv_bfloat16*)cache + from + c * 8);
+      else *(uint4*)(to + j * STRIDE + c * 8) = make_uint4(0, 0, 0, 0);      // finite: its weight is zero, and zero times a NaN is not
+    }
+  };
+  const long long mine = look_up(item.key_begin);
+  // the query rows, their offsets first (in the room of the next step's): each is behind a read of its own
+  if (tid < KEYS) rows[tid] = mine;
   if (tid < L::ROWS)
-    rows[tid] = tid < item.rows ? (long long)p.order[place_of_row(item, tid, group)] * p.q_stride + (long long)head_of_row(item, tid, group, g) * HD : -1;
-  __syncthreads();
+    rows[KEYS + tid] = tid < item.rows ? (long long)p.order[place_of_row(item, tid, group)] * p.q_stride + (long long)head_of_row(item, tid, group, g) * HD : -1;
+  bool whole = __syncthreads_and(tid >= KEYS || mine >= 0);
+  fetch(sK, p.k_cache, rows);
+  cp_async_commit();
+  fetch(sV, p.v_cache, rows);
+  cp_async_commit();
   constexpr int EACH = (L::ROWS * PIECES + MMA_THREADS - 1) / MMA_THREADS;
   uint4 held[EACH];                                    // all on their way before the first is stored
 #pragma unroll
   for (int k = 0; k < EACH; k++) {
     const int idx = tid + k * MMA_THREADS;
-    const long long at = rows[min(idx / PIECES, L::ROWS - 1)];
+    const long long at = rows[KEYS + min(idx / PIECES, L::ROWS - 1)];
     held[k] = at >= 0 ? *(const uint4*)((const __nv_bfloat16*)p.q + at + idx % PIECES * 8) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
@@ -199,37 +216,21 @@ attention_prefix_mma_kernel(const Params p) {
     const int idx = tid + k * MMA_THREADS;
     if (idx < L::ROWS * PIECES) *(uint4*)(sQ + idx / PIECES * STRIDE + idx % PIECES * 8) = held[k];
   }
-  const int tile = NARROW ? 0 : warp, gr = lane >> 2, qc = lane & 3;
+  const int tile = NARROW ? 0 : warp, gr = lane >> 2, qc = lane & 3, chunk = NARROW ? warp * CHUNK : 0;
   const int row0 = tile * 16 + gr, row1 = row0 + 8;    // of the item, this lane's in the fragments
-  const bool works = tile * 16 < item.rows;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[HD / 8][4];
 #pragma unroll
   for (int n = 0; n < HD / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  for (int base = item.key_begin; base < item.key_end; base += MMA_KEYS) {
-    __syncthreads();                                   // the pass before is done with the keys and values
-    const long long mine = base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1;
-    rows[tid] = mine;
-    const bool whole = __syncthreads_and(mine >= 0);
-    for (int idx = tid; idx < MMA_KEYS * PIECES; idx += MMA_THREADS) {
-      const int j = idx / PIECES, c = idx % PIECES;
-      const long long at = rows[j];
-      if (at >= 0) {
-        cp_async16(sK + j * STRIDE + c * 8, (const __nv_bfloat16*)p.k_cache + at + c * 8);
-        cp_async16(sV + j * STRIDE + c * 8, (const __nv_bfloat16*)p.v_cache + at + c * 8);
-      } else {                                         // what no key fills is finite: its weight is zero, and zero times a NaN is not
-        *(uint4*)(sK + j * STRIDE + c * 8) = make_uint4(0, 0, 0, 0);
-        *(uint4*)(sV + j * STRIDE + c * 8) = make_uint4(0, 0, 0, 0);
-      }
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
-    if (!works) continue;
-    const int chunk0 = NARROW ? warp * CHUNK : 0, chunk1 = NARROW ? chunk0 + CHUNK : MMA_KEYS;
-    for (int chunk = chunk0; chunk < chunk1 && base + chunk < item.key_end; chunk += CHUNK) {
-      float s[CHUNK / 8][4];
+  int held_rows = 0;                                   // which half of `rows` this step's are in
+  for (int base = item.key_begin; base < item.key_end; base += KEYS, held_rows ^= KEYS) {
+    const bool more = base + KEYS < item.key_end, works = tile * 16 < item.rows && base + chunk < item.key_end;
+    const long long next = more ? look_up(base + KEYS) : -1;
+    cp_async_wait<1>();
+    __syncthreads();                                   // the keys (and the query rows) are there
+    float s[CHUNK / 8][4];
 #pragma unroll
-      for (int n = 0; n < CHUNK / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int n = 0; n < CHUNK / 8; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    if (works) {
 #pragma unroll
       for (int kk = 0; kk < HD / 16; kk++) {
         uint32_t a[4];
@@ -242,6 +243,14 @@ attention_prefix_mma_kernel(const Params p) {
           mma_bf16(s[2 * n + 1], a, b[2], b[3]);
         }
       }
+    }
+    if (tid < KEYS) rows[(held_rows ^ KEYS) + tid] = next;
+    const bool next_whole = __syncthreads_and(tid >= KEYS || next >= 0);      // all are done with the keys
+    if (more) fetch(sK, p.k_cache, rows + (held_rows ^ KEYS));
+    cp_async_commit();
+    uint32_t pf[CHUNK / 16][4];                        // the weights as bfloat16, the A operand of P V
+    float alpha0 = 1.f, alpha1 = 1.f;
+    if (works) {
       float top0 = m0, top1 = m1;
 #pragma unroll
       for (int n = 0; n < CHUNK / 8; n++)
@@ -251,7 +260,7 @@ attention_prefix_mma_kernel(const Params p) {
 #pragma unroll
         for (int n = 0; n < CHUNK / 8; n++)
 #pragma unroll
-          for (int i = 0; i < 2; i++) if (rows[chunk + n * 8 + qc * 2 + i] < 0) s[n][i] = s[n][2 + i] = -INFINITY;
+          for (int i = 0; i < 2; i++) if (rows[held_rows + chunk + n * 8 + qc * 2 + i] < 0) s[n][i] = s[n][2 + i] = -INFINITY;
 #pragma unroll
       for (int n = 0; n < CHUNK / 8; n++) {
         top0 = fmaxf(top0, fmaxf(s[n][0], s[n][1]));
@@ -261,12 +270,12 @@ attention_prefix_mma_kernel(const Params p) {
       top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, 2));
       top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 1));
       top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, 2));
-      const float alpha0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top0), alpha1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top1);
+      alpha0 = m0 == -INFINITY ? 0.f : exp2_fast(m0 - top0);
+      alpha1 = m1 == -INFINITY ? 0.f : exp2_fast(m1 - top1);
       m0 = top0;
       m1 = top1;
       const float base0 = m0 == -INFINITY ? 0.f : m0, base1 = m1 == -INFINITY ? 0.f : m1;
       float sum0 = 0.f, sum1 = 0.f;
-      uint32_t pf[CHUNK / 16][4];                      // the weights as bfloat16, the A operand of P V
 #pragma unroll
       for (int n = 0; n < CHUNK / 8; n++) {
         const float e0 = exp2_fast(s[n][0] - base0), e1 = exp2_fast(s[n][1] - base0), e2 = exp2_fast(s[n][2] - base1), e3 = exp2_fast(s[n][3] - base1);
@@ -279,6 +288,10 @@ attention_prefix_mma_kernel(const Params p) {
       l1 = l1 * alpha1 + sum1;
 #pragma unroll
       for (int n = 0; n < HD / 8; n++) { o[n][0] *= alpha0; o[n][1] *= alpha0; o[n][2] *= alpha1; o[n][3] *= alpha1; }
+    }
+    cp_async_wait<1>();
+    __syncthreads();                                   // the values are there
+    if (works) {
 #pragma unroll
       for (int k = 0; k < CHUNK / 16; k++)
 #pragma unroll
@@ -289,7 +302,12 @@ attention_prefix_mma_kernel(const Params p) {
           mma_bf16(o[2 * n + 1], pf[k], b[2], b[3]);
         }
     }
+    __syncthreads();                                   // all are done with the values
+    if (more) fetch(sV, p.v_cache, rows + (held_rows ^ KEYS));
+    cp_async_commit();
+    whole = next_whole;
   }
+  cp_async_wait<0>();
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
   l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -305,12 +323,13 @@ attention_prefix_mma_kernel(const Params p) {
       for (int n = 0; n < HD / 8; n++) *(float2*)(p.part_out + at * HD + n * 8 + qc * 2) = make_float2(o[n][half * 2], o[n][half * 2 + 1]);
       if (qc == 0) p.part_sum[at] = half ? make_float2(m1, l1) : make_float2(m0, l0);
     }
+    end_items(p);
     return;
   }
   // the warps' results, in the keys' and values' room: [4 warps][16 rows][HD], maxima and sums behind them
   float* w_out = (float*)sK;
   float2* w_sum = (float2*)(w_out + 4 * 16 * HD);
-  static_assert((size_t)4 * 16 * HD * 4 + 64 * 8 <= (size_t)2 * MMA_KEYS * STRIDE * 2, "the warps' results fit the keys' and values' room");
+  static_assert((size_t)4 * 16 * HD * 4 + 64 * 8 <= (size_t)2 * KEYS * STRIDE * 2 || !NARROW, "the warps' results fit the keys' and values' room");
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < HD / 8; n++) {
@@ -337,6 +356,7 @@ attention_prefix_mma_kernel(const Params p) {
     *(float4*)(p.part_out + at * HD + c) = sum;
     if (c == 0) p.part_sum[at] = make_float2(m, l);
   }
+  end_items(p);
 }
 
 // ------------------------------------------------------------------ the parts of a row put together
@@ -358,7 +378,7 @@ attention_prefix_merge_kernel(const Params p) {
   float m = -INFINITY, l = 0.f, sum[PAIRS][2];
 #pragma unroll
   for (int k = 0; k < PAIRS; k++) sum[k][0] = sum[k][1] = 0.f;
-  for (int part = first + lane; part < end; part += 32) m = fmaxf(m, p.part_sum[(size_t)part * p.heads + head].x);
+  for (int part = first + lane; part < end; part += 32) m = fmaxf(m, __ldcg(&p.part_sum[(size_t)part * p.heads + head]).x);
   float score = -INFINITY;                             // of this lane's extra key
   long long at = -1;
   if (extra > 0) {
@@ -378,21 +398,36 @@ attention_prefix_merge_kernel(const Params p) {
     }
   }
   m = warp_max(fmaxf(m, score));
-  for (int part = first; part < end; part++) {
-    const float2 ml = p.part_sum[(size_t)part * p.heads + head];
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-    const float* from = p.part_out + ((size_t)part * p.heads + head) * p.head_dim;
+  // 32 parts at a time, a lane a part's factor; their outputs AHEAD at a time on their way
+  constexpr int AHEAD = 8 / PAIRS;
+  for (int base = first; base < end; base += 32) {
+    const int count = min(32, end - base);
+    float factor = 0.f;
+    if (lane < count) {
+      const float2 ml = __ldcg(&p.part_sum[(size_t)(base + lane) * p.heads + head]);
+      factor = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
+      l = fmaf(ml.y, factor, l);
+    }
+    const float* from = p.part_out + ((size_t)base * p.heads + head) * p.head_dim;
+    for (int part = 0; part < count; part += AHEAD) {
+      float2 t[AHEAD][PAIRS];
 #pragma unroll
-    for (int k = 0; k < PAIRS; k++) {
-      const int c = k * 64 + lane * 2;
-      if (c < p.head_dim) {
-        const float2 t = *(const float2*)(from + c);
-        sum[k][0] = fmaf(t.x, f, sum[k][0]);
-        sum[k][1] = fmaf(t.y, f, sum[k][1]);
+      for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+        for (int k = 0; k < PAIRS; k++) {
+          const int c = k * 64 + lane * 2;
+          t[i][k] = part + i < count && c < p.head_dim ? __ldcg((const float2*)(from + (size_t)(part + i) * p.heads * p.head_dim + c)) : make_float2(0.f, 0.f);
+        }
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++) {
+        const float f = __shfl_sync(0xffffffffu, factor, (part + i) & 31);
+        if (part + i < count)
+#pragma unroll
+          for (int k = 0; k < PAIRS; k++) { sum[k][0] = fmaf(t[i][k].x, f, sum[k][0]); sum[k][1] = fmaf(t[i][k].y, f, sum[k][1]); }
       }
     }
-    l = fmaf(ml.y, f, l);
   }
+  l = warp_sum(l);
   for (int j = 0; j < extra; j++) {
     const long long v_at = __shfl_sync(0xffffffffu, at, j);
     const float e = exp2f(__shfl_sync(0xffffffffu, score, j) - m);
@@ -489,18 +524,25 @@ SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const 
   SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
   Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, (const Item*)items, order, part_start, seen, extra, table_of, part_out, (float2*)part_sum, out, out_stride,
-           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status};
+           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, 1};
   if (simple_items > 0) {
     if (dtype == SPROUT_F32 ? launch_simple_any<float>(p, simple_items, stream) : launch_simple_any<__nv_bfloat16>(p, simple_items, stream)) return 1;
   } else {
     SPROUT_REQUIRE(dtype == SPROUT_BF16 && sprout_attention_prefix_mma_supported(head_dim), "attention_shared_prefix: these sizes run on the CUDA cores");
     SPROUT_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0,
                    "attention_shared_prefix: rows must start on 16-byte boundaries");
-    if (matrix_items > 0 && sprout_attention_prefix_tc(p, matrix_items, stream)) return 1;
+    if (matrix_items > 0) {
+      if (sprout_attention_prefix_tc(p, matrix_items, stream)) return 1;
+      p.first = 0;
+    }
     p.items += matrix_items;
+    if (wide_items > 0) {
+      p.items += narrow_items;
+      if (launch_mma_any<false>(p, wide_items, stream)) return 1;
+      p.items -= narrow_items;
+      p.first = 0;
+    }
     if (narrow_items > 0 && launch_mma_any<true>(p, narrow_items, stream)) return 1;
-    p.items += narrow_items;
-    if (wide_items > 0 && launch_mma_any<false>(p, wide_items, stream)) return 1;
   }
   return dtype == SPROUT_F32 ? launch_merge<float>(p, stream) : launch_merge<__nv_bfloat16>(p, stream);
 }

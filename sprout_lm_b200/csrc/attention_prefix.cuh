@@ -39,7 +39,17 @@ struct Params {
   int tokens, heads, kv_heads, head_dim, page_tokens, num_pages;
   float scale_log2;                    // log2(e) / sqrt(head_dim)
   int* status;
+  int first;                           // the call's first launch (see begin_items)
 };
+
+// The launches of a call's items do not depend on one another.  The first waits for the stream's earlier kernels before it lets the next
+// start; the others start when all of its CTAs have, so after those kernels, and wait for it only before they end: then the launch that
+// puts the parts together, which waits for the last of them, starts behind all.
+__device__ __forceinline__ void begin_items(const Params& p) {
+  if (p.first) pdl_wait();
+  pdl_launch_dependents();
+}
+__device__ __forceinline__ void end_items(const Params& p) { if (!p.first) pdl_wait(); }
 
 // An item's row i, 0 <= i < rows: its place in the plan's order, and its query head.
 __device__ __forceinline__ int place_of_row(const Item& item, int i, int group) { return item.token_begin + (item.row_begin + i) / group; }

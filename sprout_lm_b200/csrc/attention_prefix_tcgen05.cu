@@ -90,14 +90,15 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if ((smem_u32(smem) & 1023) != 0) {
+    begin_items(p);
     if (tid == 0) atomicOr(p.status, SPROUT_STATUS_BAD_LAYOUT);
+    end_items(p);
     return;
   }
   // rows of a stage that no copy fills must hold finite numbers: their probabilities are zero, and zero times a NaN is not
   for (int i = tid; i < NS * L::KV_BYTES / 16; i += THREADS) ((uint4*)sV)[i] = make_uint4(0, 0, 0, 0);
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
-  pdl_launch_dependents();
-  pdl_wait();
+  begin_items(p);
 
   const Item item = p.items[blockIdx.x];
   const int g = blockIdx.y, group = p.heads / p.kv_heads;
@@ -382,6 +383,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   }
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem_base, TMEM_COLS);
+  end_items(p);
 }
 
 template <int DIM>
