@@ -8,8 +8,8 @@
 // divided again, so that the launch fills the device.
 //
 // The items' partial results come from attention_prefix_simple_kernel (CUDA cores, 32-bit products, any head size and either type), or, for
-// bfloat16 and head sizes up to 128, from attention_prefix_mma_kernel (mma.sync) and, for many rows over whole pages, from
-// attention_prefix_tcgen05.cu; one launch adds them up.
+// bfloat16 and head sizes up to 128, from attention_prefix_mma_kernel (mma.sync), for few rows of most caches from
+// attention_prefix_stream.cu and for many rows over whole pages from attention_prefix_tcgen05.cu; one launch adds them up.
 #include "attention_bf16.cuh"
 #include "attention_prefix.cuh"
 
@@ -506,7 +506,9 @@ int launch_merge(const Params& p, cudaStream_t stream) {
 
 }  // namespace
 
-int sprout_attention_prefix_tc(const sprout_prefix::Params& p, int items, cudaStream_t stream);      // attention_prefix_tcgen05.cu
+int sprout_attention_prefix_tc(const sprout_prefix::Params& p, int items, cudaStream_t stream);          // attention_prefix_tcgen05.cu
+int sprout_attention_prefix_stream(const sprout_prefix::Params& p, int items, cudaStream_t stream);      // attention_prefix_stream.cu
+extern "C" int sprout_attention_prefix_tc_supported(int head_dim, int page_tokens);
 
 // Whether bfloat16 items of this head size run on the tensor cores.
 SPROUT_API int sprout_attention_prefix_mma_supported(int head_dim) { return head_dim % 16 == 0 && head_dim > 0 && head_dim <= 128; }
@@ -542,7 +544,10 @@ SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const 
       p.items -= narrow_items;
       p.first = 0;
     }
-    if (narrow_items > 0 && launch_mma_any<true>(p, narrow_items, stream)) return 1;
+    if (narrow_items > 0) {
+      const bool boxes = sprout_attention_prefix_tc_supported(head_dim, page_tokens) && (long long)num_pages * kv_heads * page_tokens <= 0x7fffffffLL;
+      if (boxes ? sprout_attention_prefix_stream(p, narrow_items, stream) : launch_mma_any<true>(p, narrow_items, stream)) return 1;
+    }
   }
   return dtype == SPROUT_F32 ? launch_merge<float>(p, stream) : launch_merge<__nv_bfloat16>(p, stream);
 }

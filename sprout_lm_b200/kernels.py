@@ -977,10 +977,13 @@ class SharedPrefixPlan:
         self.scratch_floats = host.parts * heads * (head_dim + 2)
 
 
-def _prefix_slots(head_dim: int, tensor_cores: bool) -> int:
-    """Items that the device holds at once, by their registers and shared memory."""
+def _prefix_slots(head_dim: int, tensor_cores: bool) -> tuple[int, int, int]:
+    """Items that the device holds at once, by their registers and shared memory: of up to 64 rows (or of the CUDA cores), of 256, and CTAs
+    that walk those of up to 16."""
     sms = sm_count() if torch.cuda.is_available() else 148
-    return sms * ((3 if head_dim > 96 else 4) if tensor_cores else 2)
+    if not tensor_cores:
+        return 2 * sms, 0, 0
+    return sms * (3 if head_dim > 96 else 4), sms, sms * (2 if head_dim > 64 else 3 if head_dim > 48 else 4)
 
 
 def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, head_dim: int, dtype, device=None) -> SharedPrefixPlan:
@@ -994,9 +997,11 @@ def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, 
         raise KernelError(f"shared_prefix_plan: head_dim must be even and at most 256 (got {head_dim})")
     tensor_cores = dtype == torch.bfloat16 and head_dim % 16 == 0 and head_dim <= 128
     # pages that the tcgen05 kernel copies a box at a time
-    matrix_slots = _prefix_slots(0, False) // 2 if tensor_cores and head_dim in (64, 128) and (page_tokens in (8, 16, 32, 64) or page_tokens % 128 == 0) else 0
+    slots, matrix_slots, narrow_slots = _prefix_slots(head_dim, tensor_cores)
+    if head_dim not in (64, 128) or not (page_tokens in (8, 16, 32, 64) or page_tokens % 128 == 0):
+        matrix_slots = 0
     try:
-        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, _prefix_slots(head_dim, tensor_cores), matrix_slots)
+        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, slots, matrix_slots, narrow_slots)
     except PlanError as error:
         raise KernelError(f"shared_prefix_plan: {error}") from None
     packed = torch.from_numpy(host.pack())

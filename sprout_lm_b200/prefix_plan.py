@@ -17,6 +17,7 @@ MEMBER_TOKENS = 16          # attention_prefix.cuh: MEMBER_TOKENS
 KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole steps
 NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS, MATRIX_ROWS = 16, 64, 16, 256      # rows of an item of each kind
 MATRIX_FROM = 128           # rows of a segment
+SPREAD = 1                  # items that a CTA's share of few-row items goes into
 MAX_RANGES = 64             # of a segment
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
 # the members read it themselves.
@@ -120,11 +121,19 @@ def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int, star
     return np.minimum(-(-steps // length), MAX_RANGES)
 
 
+def spread(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> np.ndarray:
+    """The same for items that ``slots`` CTAs walk one after the other at little cost for each: none longer than a CTA's even share."""
+    if not len(tiles):
+        return steps
+    share = max(1, -(-int((tiles * steps).sum()) * kv_heads // (slots * SPREAD)))
+    return np.minimum(-(-steps // share), MAX_RANGES)
+
+
 class HostPlan:
     """The plan's arrays on the host: ``items`` [n, 8] (simple ones, or matrix, narrow and wide ones), ``order``, ``part_start``, ``seen``,
     ``extra``, ``table_of``."""
 
-    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0):
+    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0, narrow_slots: int | None = None):
         tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
         if tables.ndim != 2 or q_start.ndim != 1 or contexts.ndim != 1 or len(contexts) == 0 or len(q_start) != len(contexts) + 1 or len(tables) < len(contexts):
             raise PlanError("a block table row and a context per request, and where each request's tokens start")
@@ -158,7 +167,12 @@ class HostPlan:
         ranges = np.empty(len(segments), dtype=np.int64)
         matrix = kind == 0
         ranges[matrix] = divide(tiles[matrix], steps[matrix], kv_heads, max(1, matrix_slots), 7.0, 2.4)
-        ranges[~matrix] = divide(tiles[~matrix], steps[~matrix], kv_heads, slots, 4.0, 1.5)
+        if tensor_cores:
+            wide, narrow = kind == 2, kind == 1
+            ranges[wide] = divide(tiles[wide], steps[wide], kv_heads, slots, 4.0, 1.5)
+            ranges[narrow] = spread(tiles[narrow], steps[narrow], kv_heads, narrow_slots or slots)
+        else:
+            ranges[:] = divide(tiles, steps, kv_heads, slots, 4.0, 1.5)
         per_range = -(-steps // ranges)                  # steps of a range
         ranges = -(-steps // per_range)
         parts = np.zeros(self.tokens, dtype=np.int64)    # of each place
