@@ -17,7 +17,7 @@ MEMBER_TOKENS = 16          # attention_prefix.cuh: MEMBER_TOKENS
 KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole steps
 NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS, MATRIX_ROWS = 16, 64, 16, 256      # rows of an item of each kind
 MATRIX_FROM = 128           # rows of a segment
-SPREAD = 1                  # items that a CTA's share of few-row items goes into
+ITEM_STEPS = 0.5            # what an item of few rows costs beside its steps
 MAX_RANGES = 64             # of a segment
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
 # the members read it themselves.
@@ -122,11 +122,33 @@ def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int, star
 
 
 def spread(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> np.ndarray:
-    """The same for items that ``slots`` CTAs walk one after the other at little cost for each: none longer than a CTA's even share."""
+    """The same for items that ``slots`` CTAs walk, each taking one of every ``slots`` of them, longest first, forwards and backwards in
+    turn: ranges of the length with which the CTA that has most to do has least (an item costs ``ITEM_STEPS`` steps beside its own)."""
     if not len(tiles):
         return steps
-    share = max(1, -(-int((tiles * steps).sum()) * kv_heads // (slots * SPREAD)))
-    return np.minimum(-(-steps // share), MAX_RANGES)
+
+    def busiest(length):
+        ranges = np.minimum(-(-steps // length), MAX_RANGES)
+        each = -(-steps // ranges)
+        items = np.repeat(np.concatenate([each, steps - each * (ranges - 1)]), np.concatenate([tiles * (ranges - 1), tiles]) * kv_heads)
+        rounds = -(-len(items) // slots)
+        loads = np.zeros(rounds * slots)
+        loads[:len(items)] = np.sort(items)[::-1] + ITEM_STEPS
+        loads = loads.reshape(rounds, slots)
+        loads[1::2] = loads[1::2, ::-1]
+        return loads.sum(0).max()
+
+    share = int((tiles * steps).sum()) * kv_heads / slots
+    count = lambda n: int((tiles * np.minimum(-(-steps // n), MAX_RANGES)).sum()) * kv_heads
+    lengths = {int(steps.max())} | {max(1, -(-int(share * 16) // k)) for k in (8, 12, 16, 24, 32, 48, 64)}
+    low, high = 1, int(steps.max())                      # and the shortest ranges that are one round
+    if count(high) <= slots:
+        while low < high:
+            middle = (low + high) // 2
+            low, high = (low, middle) if count(middle) <= slots else (middle + 1, high)
+        lengths.add(low)
+    best = min(sorted(lengths, reverse=True), key=busiest)
+    return np.minimum(-(-steps // best), MAX_RANGES)
 
 
 class HostPlan:
