@@ -452,16 +452,9 @@ attention_prefix_merge_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ launches
-template <typename F>
-int reserve(F kernel, size_t bytes, const char* what) {
-  if (bytes <= 48 * 1024) return 0;
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return err == cudaSuccess ? 0 : sprout_fail("%s: cannot reserve %zu bytes of shared memory: %s", what, bytes, cudaGetErrorString(err));
-}
-
 template <typename T, int COLUMNS>
 int launch_simple(const Params& p, int items, cudaStream_t stream) {
-  if (reserve(attention_prefix_simple_kernel<T, COLUMNS>, simple_smem(p.head_dim), "attention_shared_prefix")) return 1;
+  if (reserve_shared<attention_prefix_simple_kernel<T, COLUMNS>>(simple_smem(COLUMNS * 64), "attention_shared_prefix")) return 1;
   sprout_launch(attention_prefix_simple_kernel<T, COLUMNS>, dim3(items, p.kv_heads), dim3(SIMPLE_THREADS), simple_smem(p.head_dim), stream, p);
   return sprout_check_launch("attention_prefix_simple");
 }
@@ -475,7 +468,7 @@ int launch_simple_any(const Params& p, int items, cudaStream_t stream) {
 template <int HD, bool NARROW>
 int launch_mma(const Params& p, int items, cudaStream_t stream) {
   constexpr size_t bytes = MmaShape<HD, NARROW>::SMEM;
-  if (reserve(attention_prefix_mma_kernel<HD, NARROW>, bytes, "attention_shared_prefix")) return 1;
+  if (reserve_shared<attention_prefix_mma_kernel<HD, NARROW>>(bytes, "attention_shared_prefix")) return 1;
   sprout_launch(attention_prefix_mma_kernel<HD, NARROW>, dim3(items, p.kv_heads), dim3(MMA_THREADS), bytes, stream, p);
   return sprout_check_launch("attention_prefix_mma");
 }

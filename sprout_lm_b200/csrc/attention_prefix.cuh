@@ -62,4 +62,17 @@ __device__ __forceinline__ long long key_row(const Params& p, const int* table, 
   return (((long long)page * p.kv_heads + g) * p.page_tokens + key % p.page_tokens) * p.head_dim;
 }
 
+// Room for `bytes` of dynamic shared memory, always the same for a kernel; asked for once a device.
+template <auto KERNEL>
+int reserve_shared(size_t bytes, const char* what) {
+  static bool done[64] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return sprout_fail("%s: no current device", what);
+  if (done[device]) return 0;
+  const cudaError_t err = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (err != cudaSuccess) return sprout_fail("%s: cannot reserve %zu bytes of shared memory: %s", what, bytes, cudaGetErrorString(err));
+  done[device] = true;
+  return 0;
+}
+
 }  // namespace sprout_prefix

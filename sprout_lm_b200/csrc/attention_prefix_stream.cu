@@ -292,8 +292,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
 template <int HD>
 int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, int items, int box_rows, cudaStream_t stream) {
   using L = Layout<HD>;
-  const cudaError_t err = cudaFuncSetAttribute(attention_prefix_stream_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-  if (err != cudaSuccess) return sprout_fail("attention_shared_prefix (few rows): cannot reserve %d bytes of shared memory: %s", L::SMEM, cudaGetErrorString(err));
+  if (reserve_shared<attention_prefix_stream_kernel<HD>>(L::SMEM, "attention_shared_prefix (few rows)")) return 1;
   const long long pairs = (long long)items * p.kv_heads, slots = (long long)L::CTAS * sprout_sm_count();
   SPROUT_REQUIRE(pairs <= 0x7fffffffLL, "attention_shared_prefix: too many items");
   sprout_launch(attention_prefix_stream_kernel<HD>, dim3((unsigned)(pairs < slots ? pairs : slots)), dim3(THREADS), L::SMEM, stream, map_k, map_v, p, (int)pairs, box_rows);

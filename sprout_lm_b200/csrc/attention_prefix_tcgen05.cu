@@ -35,7 +35,7 @@ struct Layout {
   static constexpr int Q_BYTES = DIM / 64 * ATOM, KV_BYTES = DIM / 64 * KV_ATOM;
   static constexpr int STAGES = 5;
   static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_BAR = OFF_V + STAGES * KV_BYTES;
-  static constexpr int SMEM = OFF_BAR + 512;
+  static constexpr int OFF_ROWS = OFF_BAR + 512, SMEM = OFF_ROWS + 2 * ROWS * 8;       // the query rows' addresses
   static constexpr int O_COLUMN = 4 * KEYS;                        // tensor memory: S of the Q tiles, two buffers each, then their O
   static_assert(O_COLUMN + 2 * DIM <= TMEM_COLS, "tensor memory columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -106,10 +106,9 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   const bool two = item.rows > ROWS;                   // the second Q tile has rows
   const int n_tiles = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
 
-  // Q rows -> shared memory, K-major with the 128-byte swizzle (16-byte chunk c of row r at position c ^ (r & 7)); the rows' addresses first, in
-  // the room of the first keys (a thread that finds them one after the other, or stores a row before it asks for the next, waits for every
-  // read: 4 to 6 us in all)
-  const __nv_bfloat16** from = (const __nv_bfloat16**)sK;
+  // Q rows -> shared memory, K-major with the 128-byte swizzle (16-byte chunk c of row r at position c ^ (r & 7)); the rows' addresses first
+  // (a thread that finds them one after the other, or stores a row before it asks for the next, waits for every read: 4 to 6 us in all)
+  const __nv_bfloat16** from = (const __nv_bfloat16**)(smem + L::OFF_ROWS);
   if (tid < 2 * ROWS)
     from[tid] = tid < item.rows ? (const __nv_bfloat16*)p.q + (size_t)p.order[place_of_row(item, tid, group)] * p.q_stride + (size_t)head_of_row(item, tid, group, g) * DIM : nullptr;
   if (tid == THREADS - 1) {
@@ -121,27 +120,29 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  constexpr int CHUNKS = DIM / 8, EACH = (2 * ROWS * CHUNKS + THREADS - 1) / THREADS;
-  uint4 held[EACH];                                    // all on their way before the first is stored
-#pragma unroll
-  for (int k = 0; k < EACH; k++) {
-    const int idx = tid + k * THREADS, i = min(idx / CHUNKS, 2 * ROWS - 1);
-    const __nv_bfloat16* at = from[i];
-    held[k] = at != nullptr ? *(const uint4*)(at + idx % CHUNKS * 8) : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int k = 0; k < EACH; k++) {
-    const int idx = tid + k * THREADS, i = idx / CHUNKS, c = idx % CHUNKS, q = i >> 7, row = i & (ROWS - 1);
-    if (i < 2 * ROWS) *(uint4*)(sQ + q * L::Q_BYTES + (c >> 3) * ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = held[k];
-  }
-  fence_proxy_async();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-
   int issued = 0;                                     // tiles whose copies were issued (copy warps)
   auto gave_up = [&]() { *abort_flag = 1; atomicOr(p.status, SPROUT_STATUS_WAIT_TIMEOUT); };
+  if (warp != 0 && warp != 2) {                        // the copies start meanwhile
+    const int other = tid - (warp == 1 ? 32 : 64);
+    constexpr int CHUNKS = DIM / 8, OTHERS = THREADS - 64, EACH = (2 * ROWS * CHUNKS + OTHERS - 1) / OTHERS;
+    uint4 held[EACH];                                    // all on their way before the first is stored
+  #pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const int idx = other + k * OTHERS, i = min(idx / CHUNKS, 2 * ROWS - 1);
+      const __nv_bfloat16* at = from[i];
+      held[k] = at != nullptr ? *(const uint4*)(at + idx % CHUNKS * 8) : make_uint4(0, 0, 0, 0);
+    }
+  #pragma unroll
+    for (int k = 0; k < EACH; k++) {
+      const int idx = other + k * OTHERS, i = idx / CHUNKS, c = idx % CHUNKS, q = i >> 7, row = i & (ROWS - 1);
+      if (i < 2 * ROWS) *(uint4*)(sQ + q * L::Q_BYTES + (c >> 3) * ATOM + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = held[k];
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    named_barrier(1, OTHERS);
+    tc_fence_after();
+  }
+  const uint32_t tmem_base = *tmem_slot;
   if (warp < 4) {
     warpgroup_regs_give<104>();
     if (warp == 0 || warp == 2) {
@@ -357,6 +358,9 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         p.part_sum[slot] = make_float2(m == -INFINITY ? -INFINITY : m * scale_log2, l_lo + l_hi);
       }
       const unsigned long long to = mine ? (unsigned long long)(p.part_out + slot * DIM) : 0ull;
+      float* dst[8];                                   // of the rows whose 16-byte chunk lane % 8 this lane stores
+#pragma unroll
+      for (int k = 0; k < 8; k++) dst[k] = (float*)__shfl_sync(0xffffffffu, to, k * 4 + (lane >> 3));
       float* room = (float*)(sQ + q * L::Q_BYTES) + quarter * (32 * 32);       // 4 KB: 32 rows of 32 columns, 16-byte chunk c of row r at c ^ (r & 7)
       for (int c = 0; c < DIM; c += 32) {
         uint32_t o[32];
@@ -368,8 +372,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 #pragma unroll
         for (int k = 0; k < 8; k++) {
           const int r = k * 4 + (lane >> 3), chunk = lane & 7;
-          float* dst = (float*)__shfl_sync(0xffffffffu, to, r);
-          if (dst != nullptr) *(uint4*)(dst + c + chunk * 4) = *(const uint4*)(room + r * 32 + ((chunk ^ (r & 7)) << 2));
+          if (dst[k] != nullptr) *(uint4*)(dst[k] + c + chunk * 4) = *(const uint4*)(room + r * 32 + ((chunk ^ (r & 7)) << 2));
         }
       }
     }
@@ -389,8 +392,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
 template <int DIM>
 int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, int items, int box_rows, cudaStream_t stream) {
   using L = Layout<DIM>;
-  const cudaError_t err = cudaFuncSetAttribute(attention_prefix_tc_kernel<DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-  if (err != cudaSuccess) return sprout_fail("attention_shared_prefix (tcgen05): cannot reserve %d bytes of shared memory: %s", L::SMEM, cudaGetErrorString(err));
+  if (reserve_shared<attention_prefix_tc_kernel<DIM>>(L::SMEM, "attention_shared_prefix (tcgen05)")) return 1;
   sprout_launch(attention_prefix_tc_kernel<DIM>, dim3(items, p.kv_heads), dim3(THREADS), L::SMEM, stream, map_k, map_v, p, box_rows);
   return sprout_check_launch("attention_shared_prefix (tcgen05)");
 }

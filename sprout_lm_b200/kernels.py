@@ -1063,21 +1063,28 @@ def sample(logits, out, status, temperature=None, uniform=None):
 
 def _one_device(name, tensors):
     """All of the (what, tensor) pairs (None: not given) on one CUDA device, the current one."""
-    current = torch.cuda.current_device() if torch.cuda.is_available() else 0
+    device = None                          # the current one, once a tensor was found on it
     for what, t in tensors:
-        if t is not None and t.get_device() != current:
-            if not t.is_cuda:
-                raise KernelError(f"{name}: {what} must be a CUDA tensor; there is no CPU path")
-            raise KernelError(f"{name}: {what} is on {t.device}, the current device is cuda:{current}")
+        if t is None:
+            continue
+        index = t.get_device()             # -1: not a CUDA tensor
+        if index < 0:
+            raise KernelError(f"{name}: {what} must be a CUDA tensor; there is no CPU path")
+        if index != device:
+            if index != torch.cuda.current_device():
+                raise KernelError(f"{name}: {what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+            device = index
 
 
 def _overlap(a, b) -> bool:
     """Whether two tensors' memory (from the first to the last element) meets."""
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if not a.numel() or not b.numel():
+        return False
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if a0 == b0:
+        return True
+    low, gap = (a, b0 - a0) if a0 < b0 else (b, a0 - b0)       # the one that starts first reaches the other's start?
+    return gap < (sum((n - 1) * s for n, s in zip(low.shape, low.stride())) + 1) * low.element_size()
 
 
 def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperatures=None, accept=None, draw=None, out=None, accepted=None):

@@ -126,7 +126,50 @@ def test_kernel_binding_refuses_what_it_cannot_run():
         kernels.shared_prefix_plan([[1]], [0, 1], [1], 16, 4, 2, 64, torch.float16, "cpu")
     with pytest.raises(kernels.KernelError, match="context"):
         kernels.shared_prefix_plan([[1]], [0, 1], [17], 16, 4, 2, 64, torch.bfloat16, "cpu")
+    # tensors that are not on a GPU are refused, whichever they are, before anything else is looked at
     plan = kernels.shared_prefix_plan([[1]], [0, 1], [1], 16, 4, 2, 64, torch.bfloat16, "cpu")
-    q = torch.zeros(1, 256, dtype=torch.bfloat16)
-    with pytest.raises(kernels.KernelError, match="CUDA tensor"):
-        kernels.attention_shared_prefix(q, q, q, q, q, plan, q, q)
+    q, cache = torch.zeros(1, 256, dtype=torch.bfloat16), torch.zeros(2, 2, 16, 64, dtype=torch.bfloat16)
+    word = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(kernels.KernelError, match="q must be a CUDA tensor"):
+        kernels.attention_shared_prefix(q, cache, cache.clone(), torch.ones(1, 1, dtype=torch.int32), word, plan, torch.zeros_like(q), word)
+    with pytest.raises(kernels.KernelError, match="logits must be a CUDA tensor"):
+        kernels.verify_drafts(torch.zeros(2, 5), torch.zeros(2, dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32), word)
+
+
+class OnDevice:
+    """What the device check sees of a tensor."""
+
+    def __init__(self, index):
+        self.index, self.device = index, f"device {index}"
+
+    def get_device(self):
+        return self.index
+
+
+def test_device_check(monkeypatch):
+    """One tensor off the GPU, or on another GPU than the current one, is found at any place among the others."""
+    import torch
+    from sprout_lm_b200 import kernels
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    kernels._one_device("name", [("a", OnDevice(1)), ("b", None), ("c", OnDevice(1))])
+    for at in range(3):
+        for index, text in ((-1, "CUDA tensor"), (0, "the current device is cuda:1")):
+            tensors = [(f"t{i}", OnDevice(index if i == at else 1)) for i in range(3)]
+            with pytest.raises(kernels.KernelError, match=f"t{at} .*{text}"):
+                kernels._one_device("name", tensors)
+    with pytest.raises(kernels.KernelError, match="t0 is on"):
+        kernels._one_device("name", [("t0", OnDevice(0)), ("t1", OnDevice(0))])
+
+
+def test_overlap_check():
+    import torch
+    from sprout_lm_b200 import kernels
+    whole = torch.zeros(40)
+    for a0 in range(0, 40, 3):
+        for a1 in range(a0 + 1, 41, 4):
+            for b0 in range(0, 40, 5):
+                for b1 in range(b0 + 1, 41, 3):
+                    assert kernels._overlap(whole[a0:a1], whole[b0:b1]) == (a0 < b1 and b0 < a1)
+    rows = torch.zeros(4, 10)
+    assert kernels._overlap(rows[:, :3], rows[:, 5:]) and not kernels._overlap(rows[:2, 5:], rows[2:, :3])      # from the first to the last element
+    assert not kernels._overlap(whole[3:3], whole)
