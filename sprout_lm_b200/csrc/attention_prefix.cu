@@ -360,21 +360,29 @@ attention_prefix_mma_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ the parts of a row put together
-// A warp per (token, head), a lane two columns in every 64; with the keys of the member's own tokens that the items leave out, a lane a key.
-constexpr int MERGE_THREADS = 128;
+// WARPS warps per (token, head), each of them every WARPS-th part, a lane two columns in every 64; the first warp also adds the keys of the
+// member's own tokens that the items leave out, a lane a key.  One warp for a row of few parts; a row of 35 parts in one warp is a chain
+// of five waits for memory.
+#ifndef PREFIX_MERGE_FROM
+#define PREFIX_MERGE_FROM 24
+#endif
+constexpr int MERGE_THREADS = 128, MERGE_SPLIT = 4, MERGE_FROM = PREFIX_MERGE_FROM;      // MERGE_FROM: parts a row, on average
 
-template <typename T, int PAIRS>
+template <typename T, int PAIRS, int WARPS>
 __global__ void __launch_bounds__(MERGE_THREADS)
 attention_prefix_merge_kernel(const Params p) {
+  constexpr int ROWS = MERGE_THREADS / 32 / WARPS;     // of a block
+  __shared__ float s_max[MERGE_THREADS / 32];
+  __shared__ float s_sum[WARPS > 1 ? WARPS : 1][PAIRS * 64 + 1];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, group = p.heads / p.kv_heads;
-  const long long row = (long long)blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5);
-  if (row >= (long long)p.tokens * p.heads) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WARPS, group = p.heads / p.kv_heads;
+  const long long row = (long long)blockIdx.x * ROWS + warp / WARPS;
+  if (row >= (long long)p.tokens * p.heads) return;    // whole blocks where warps share a row
   const int head = (int)(row % p.heads), place = (int)(row / p.heads), token = p.order[place], g = head / group;
   const int first = p.part_start[place], end = p.part_start[place + 1];
-  const int seen = p.seen[place], extra = p.extra[place];
-  if (p.positions[token] != seen + extra - 1 && head == 0 && lane == 0) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);      // another step's plan
+  const int seen = p.seen[place], extra = share == 0 ? p.extra[place] : 0;
+  if (share == 0 && head == 0 && lane == 0 && p.positions[token] != seen + extra - 1) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);      // another step's plan
   float m = -INFINITY, l = 0.f, sum[PAIRS][2];
 #pragma unroll
   for (int k = 0; k < PAIRS; k++) sum[k][0] = sum[k][1] = 0.f;
@@ -398,13 +406,19 @@ attention_prefix_merge_kernel(const Params p) {
     }
   }
   m = warp_max(fmaxf(m, score));
-  // 32 parts at a time, a lane a part's factor; their outputs AHEAD at a time on their way
+  if (WARPS > 1) {                                     // the extra keys' may be the largest
+    if (lane == 0) s_max[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) m = fmaxf(m, s_max[w]);
+  }
+  // 32 of the warp's parts at a time, a lane a part's factor; their outputs AHEAD at a time on their way
   constexpr int AHEAD = 8 / PAIRS;
-  for (int base = first; base < end; base += 32) {
-    const int count = min(32, end - base);
+  for (int base = first + share; base < end; base += 32 * WARPS) {
+    const int count = min(32, (end - base + WARPS - 1) / WARPS);
     float factor = 0.f;
     if (lane < count) {
-      const float2 ml = __ldcg(&p.part_sum[(size_t)(base + lane) * p.heads + head]);
+      const float2 ml = __ldcg(&p.part_sum[(size_t)(base + lane * WARPS) * p.heads + head]);
       factor = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
       l = fmaf(ml.y, factor, l);
     }
@@ -416,7 +430,7 @@ attention_prefix_merge_kernel(const Params p) {
 #pragma unroll
         for (int k = 0; k < PAIRS; k++) {
           const int c = k * 64 + lane * 2;
-          t[i][k] = part + i < count && c < p.head_dim ? __ldcg((const float2*)(from + (size_t)(part + i) * p.heads * p.head_dim + c)) : make_float2(0.f, 0.f);
+          t[i][k] = part + i < count && c < p.head_dim ? __ldcg((const float2*)(from + (size_t)(part + i) * WARPS * p.heads * p.head_dim + c)) : make_float2(0.f, 0.f);
         }
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
@@ -441,6 +455,19 @@ attention_prefix_merge_kernel(const Params p) {
       }
     }
     l += e;
+  }
+  if (WARPS > 1) {
+#pragma unroll
+    for (int k = 0; k < PAIRS; k++) { s_sum[share][k * 64 + lane * 2] = sum[k][0]; s_sum[share][k * 64 + lane * 2 + 1] = sum[k][1]; }
+    if (lane == 0) s_sum[share][PAIRS * 64] = l;
+    __syncthreads();
+    if (share != 0) return;
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) {
+#pragma unroll
+      for (int k = 0; k < PAIRS; k++) { sum[k][0] += s_sum[w][k * 64 + lane * 2]; sum[k][1] += s_sum[w][k * 64 + lane * 2 + 1]; }
+      l += s_sum[w][PAIRS * 64];
+    }
   }
   const float inv = l != 0.f ? 1.0f / l : 0.f;         // no key at all (every page outside the pool): zero
   T* to = (T*)p.out + (size_t)token * p.out_stride + (size_t)head * p.head_dim;
@@ -487,13 +514,14 @@ int launch_mma_any(const Params& p, int items, cudaStream_t stream) {
   return sprout_fail("attention_shared_prefix: head_dim %d is not the tensor cores'", p.head_dim);
 }
 
-template <typename T>
+template <typename T, int WARPS>
 int launch_merge(const Params& p, cudaStream_t stream) {
-  const long long blocks = ((long long)p.tokens * p.heads + MERGE_THREADS / 32 - 1) / (MERGE_THREADS / 32);
+  constexpr int rows = MERGE_THREADS / 32 / WARPS;
+  const long long blocks = ((long long)p.tokens * p.heads + rows - 1) / rows;
   SPROUT_REQUIRE(blocks <= 0x7fffffffLL, "attention_shared_prefix: too many tokens");
-  if (p.head_dim <= 64) sprout_launch(attention_prefix_merge_kernel<T, 1>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
-  else if (p.head_dim <= 128) sprout_launch(attention_prefix_merge_kernel<T, 2>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
-  else sprout_launch(attention_prefix_merge_kernel<T, 4>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
+  if (p.head_dim <= 64) sprout_launch(attention_prefix_merge_kernel<T, 1, WARPS>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
+  else if (p.head_dim <= 128) sprout_launch(attention_prefix_merge_kernel<T, 2, WARPS>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
+  else sprout_launch(attention_prefix_merge_kernel<T, 4, WARPS>, dim3((unsigned)blocks), dim3(MERGE_THREADS), 0, stream, p);
   return sprout_check_launch("attention_prefix_merge");
 }
 
@@ -510,11 +538,11 @@ SPROUT_API int sprout_attention_prefix_mma_supported(int head_dim) { return head
 // partial results in all; part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
 SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
                                        const int* positions, const int* items, int simple_items, int matrix_items, int narrow_items, int wide_items, const int* order,
-                                       const int* part_start, const int* seen, const int* extra, const int* table_of, float* part_out, float* part_sum, void* out, long long out_stride, int dtype, int tokens,
+                                       const int* part_start, const int* seen, const int* extra, const int* table_of, float* part_out, float* part_sum, void* out, long long out_stride, int dtype, int tokens, int parts,
                                        int heads, int kv_heads, int head_dim, int page_tokens, int num_pages, int* status, cudaStream_t stream) {
   SPROUT_REQUIRE(q && k_cache && v_cache && block_table && positions && items && order && part_start && seen && extra && table_of && part_out && part_sum && out && status,
                  "attention_shared_prefix: null pointer");
-  SPROUT_REQUIRE(tokens > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
+  SPROUT_REQUIRE(tokens > 0 && parts > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
                  "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
   SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
@@ -542,5 +570,7 @@ SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const 
       if (boxes ? sprout_attention_prefix_stream(p, narrow_items, stream) : launch_mma_any<true>(p, narrow_items, stream)) return 1;
     }
   }
-  return dtype == SPROUT_F32 ? launch_merge<float>(p, stream) : launch_merge<__nv_bfloat16>(p, stream);
+  const bool split = parts >= (long long)MERGE_FROM * tokens;
+  if (dtype == SPROUT_F32) return split ? launch_merge<float, MERGE_SPLIT>(p, stream) : launch_merge<float, 1>(p, stream);
+  return split ? launch_merge<__nv_bfloat16, MERGE_SPLIT>(p, stream) : launch_merge<__nv_bfloat16, 1>(p, stream);
 }

@@ -41,7 +41,7 @@ _SIGNATURES = {
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "sprout_attention_prefix_tc_supported": [_I, _I],
-    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_attention_prefix_mma_supported": [_I],
     "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
@@ -973,8 +973,9 @@ class SharedPrefixPlan:
         self.host, self.page_tokens, self.heads, self.kv_heads, self.head_dim, self.dtype, self.buffer = host, page_tokens, heads, kv_heads, head_dim, dtype, buffer
         base = buffer.data_ptr()
         self.pointers = [base + 4 * at for at, _ in host.offsets]
-        # maxima and sums of the partial results, then the results
-        self.scratch_floats = host.parts * heads * (head_dim + 2)
+        self.scratch_floats = host.parts * heads * (head_dim + 2)          # the partial results, then their maxima and sums
+        # what a call's tensors have to be
+        self.rows, self.page, self.token_shape, self.dtype_code = (host.tokens, heads * head_dim), (kv_heads, page_tokens, head_dim), (host.tokens,), _dtype_code(dtype)
 
 
 def _prefix_slots(head_dim: int, tensor_cores: bool) -> tuple[int, int, int]:
@@ -1001,28 +1002,21 @@ def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, 
     if head_dim not in (64, 128) or not (page_tokens in (8, 16, 32, 64) or page_tokens % 128 == 0):
         matrix_slots = 0
     try:
-        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, slots, matrix_slots, narrow_slots)
+        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, slots, matrix_slots, narrow_slots, head_dim)
     except PlanError as error:
         raise KernelError(f"shared_prefix_plan: {error}") from None
     packed = torch.from_numpy(host.pack())
     return SharedPrefixPlan(host, page_tokens, heads, kv_heads, head_dim, dtype, packed.to(device if device is not None else "cuda"))
 
 
-def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: SharedPrefixPlan, out, status, scratch=None):
-    """Causal attention of a step's tokens over their requests' pages, a run of pages that several requests hold read once for all of
-    them.  ``q`` and ``out`` [tokens, heads * head_dim] (rows may lie apart), the caches [pages, kv_heads, page_tokens, head_dim], all
-    of the plan's type; ``block_table`` int32 [requests, pages] holds what the plan was made of; ``positions`` int32 [tokens]: a token
-    sees the keys up to its own, and a position other than the plan's sets a status bit (another step's plan).  float32 runs on CUDA
-    cores with 32-bit products, bfloat16 on tensor cores for head sizes up to 128 in steps of 16.  ``scratch``: float32 memory of
-    ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own."""
-    name = "attention_shared_prefix"
-    host = plan.host
+def _refuse_shared_prefix(q, k_cache, v_cache, block_table, positions, plan, out, status, scratch):
+    """Says what is wrong with the arguments of ``attention_shared_prefix``."""
+    name, host, width = "attention_shared_prefix", plan.host, plan.heads * plan.head_dim
     _one_device(name, (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table), ("positions", positions), ("plan", plan.buffer),
                        ("out", out), ("status", status), ("scratch", scratch)))
     _rows_contiguous(q, "q")
     _rows_contiguous(out, "out")
     _rows_contiguous(block_table, "block_table")
-    width = plan.heads * plan.head_dim
     if q.shape != (host.tokens, width) or out.shape != (host.tokens, width):
         raise KernelError(f"{name}: q and out must be [{host.tokens}, {width}], the plan's tokens and heads")
     if k_cache.shape != v_cache.shape or k_cache.dim() != 4 or k_cache.shape[1:] != (plan.kv_heads, plan.page_tokens, plan.head_dim) or k_cache.shape[0] < 1 \
@@ -1034,18 +1028,39 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
         raise KernelError(f"{name}: block_table must hold the plan's {host.requests} requests and {host.pages} pages")
     if positions.dtype != torch.int32 or positions.shape != (host.tokens,) or not positions.is_contiguous():
         raise KernelError(f"{name}: positions must be contiguous int32 [{host.tokens}]")
+    _ptr(block_table, "block_table", torch.int32)
+    _ptr(status, "status", torch.int32)
+    raise KernelError(f"{name}: arguments that do not fit the plan")
+
+
+def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: SharedPrefixPlan, out, status, scratch=None):
+    """Causal attention of a step's tokens over their requests' pages, a run of pages that several requests hold read once for all of
+    them.  ``q`` and ``out`` [tokens, heads * head_dim] (rows may lie apart), the caches [pages, kv_heads, page_tokens, head_dim], all
+    of the plan's type; ``block_table`` int32 [requests, pages] holds what the plan was made of; ``positions`` int32 [tokens]: a token
+    sees the keys up to its own, and a position other than the plan's sets a status bit (another step's plan).  float32 runs on CUDA
+    cores with 32-bit products, bfloat16 on tensor cores for head sizes up to 128 in steps of 16.  ``scratch``: float32 memory of
+    ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own."""
+    host, pages, index = plan.host, k_cache.shape, q.get_device()
+    if not (0 <= index == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == positions.get_device() == plan.buffer.get_device()
+            == out.get_device() == status.get_device() == torch.cuda.current_device() and (scratch is None or scratch.get_device() == index)
+            and q.shape == plan.rows and out.shape == plan.rows and q.stride(1) == 1 and out.stride(1) == 1 and pages == v_cache.shape
+            and pages[1:] == plan.page and pages[0] > 0 and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == plan.dtype and block_table.dim() == 2 and block_table.stride(1) == 1
+            and block_table.shape[0] >= host.requests and block_table.shape[1] >= host.pages and block_table.dtype == torch.int32
+            and positions.dtype == torch.int32 and positions.shape == plan.token_shape and positions.is_contiguous() and status.dtype == torch.int32):
+        _refuse_shared_prefix(q, k_cache, v_cache, block_table, positions, plan, out, status, scratch)
     if _overlap(q, out):
-        raise KernelError(f"{name}: q and out share memory")
+        raise KernelError("attention_shared_prefix: q and out share memory")
     if scratch is None:
-        scratch = torch.empty(plan.scratch_floats, dtype=torch.float32, device=q.device)
+        scratch = q.new_empty(plan.scratch_floats, dtype=torch.float32)
     elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < plan.scratch_floats or scratch.data_ptr() % 16:
-        raise KernelError(f"{name}: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
+        raise KernelError(f"attention_shared_prefix: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
     items, order, part_start, seen, extra, table_of = plan.pointers
     at = scratch.data_ptr()
-    _run("sprout_attention_prefix", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(block_table, "block_table", torch.int32),
+    _run("sprout_attention_prefix", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
          block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.matrix_items, host.narrow_items, host.wide_items, order, part_start, seen, extra, table_of,
-         at, at + 4 * host.parts * plan.heads * plan.head_dim, out.data_ptr(), out.stride(0), _dtype_code(q.dtype), host.tokens, plan.heads, plan.kv_heads,
-         plan.head_dim, plan.page_tokens, k_cache.shape[0], _ptr(status, "status", torch.int32), _stream())
+         at, at + 4 * host.parts * plan.heads * plan.head_dim, out.data_ptr(), out.stride(0), plan.dtype_code, host.tokens, host.parts, plan.heads, plan.kv_heads,
+         plan.head_dim, plan.page_tokens, pages[0], status.data_ptr(), _stream())
 
 
 def sample(logits, out, status, temperature=None, uniform=None):
@@ -1087,22 +1102,8 @@ def _overlap(a, b) -> bool:
     return gap < (sum((n - 1) * s for n, s in zip(low.shape, low.stride())) + 1) * low.element_size()
 
 
-def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperatures=None, accept=None, draw=None, out=None, accepted=None):
-    """Which drafted tokens stand against the target's probabilities, and the token after the last that does: ``(out, accepted)``.
-
-    Request r has rows ``row_start[r]`` to ``row_start[r + 1] - 1`` (int32 [requests + 1]) of ``logits`` (float32 [rows, vocab]), one more
-    than it has drafts: row i is what the target says at the place of its i-th draft, the last what it says behind all of them.
-    ``drafts`` (int32 [rows]) holds the tokens in the same places (a request's last entry is not read).  ``draft_logits`` (float32
-    [rows - requests, vocab]): the draft model's rows, one a draft, request by request; without it a draft counts as drawn with
-    probability 1 (looked up).  ``temperatures`` (float32 [requests]), ``accept`` and ``draw`` (float32 [rows], uniform in [0, 1)):
-    a request with a temperature T > 0 keeps draft x of row i with probability min(1, p(x) / q(x)), p and q the softmax of the two logits
-    over T: where ``accept[i] * q(x) < p(x)``; at the first that is not kept the token is drawn at ``draw[i]`` from max(p - q, 0),
-    behind the last one from p.  Temperature 0 (or no temperatures): drafts stand while they are the row's argmax (the lowest index among
-    ties), then the argmax follows.
-
-    ``out`` (int32 [rows]): the drafts that stand, the token after them, and -1 in the rest of the request's rows; ``accepted`` (int32
-    [requests]): how many stand; both are made here unless given.  A row that is reached and holds a non-finite logit, or a draft outside
-    the vocabulary, sets a status bit and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
+def _check_verify(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw, out, accepted):
+    """Refuses arguments of ``verify_drafts`` that do not fit."""
     name = "verify_drafts"
     _one_device(name, (("logits", logits), ("drafts", drafts), ("row_start", row_start), ("status", status), ("draft_logits", draft_logits),
                        ("temperatures", temperatures), ("accept", accept), ("draw", draw), ("out", out), ("accepted", accepted)))
@@ -1119,12 +1120,14 @@ def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperat
     for what, t, n in (("temperatures", temperatures, requests), ("accept", accept, rows), ("draw", draw, rows)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous()):
             raise KernelError(f"{name}: {what} must be contiguous float32 [{n}]")
-    draft_rows = 0
     if draft_logits is not None:
         _rows_contiguous(draft_logits, "draft_logits")
-        draft_rows = rows - requests                       # none where nobody drafted anything
+        draft_rows = rows - requests
         if draft_logits.shape != (draft_rows, vocab):
             raise KernelError(f"{name}: draft_logits must be [{draft_rows}, {vocab}], a row per draft (got {tuple(draft_logits.shape)})")
+    for what, t in (("logits", logits), ("draft_logits", draft_logits)):
+        _ptr(t, what, torch.float32, allow_none=what != "logits")
+    _ptr(status, "status", torch.int32)
     if out is not None or accepted is not None:
         inputs = [(w, t) for w, t in (("logits", logits), ("drafts", drafts), ("row_start", row_start), ("draft_logits", draft_logits), ("status", status),
                                       ("temperatures", temperatures), ("accept", accept), ("draw", draw)) if t is not None]
@@ -1132,15 +1135,47 @@ def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperat
             for other, s in others:
                 if t is not None and s is not None and _overlap(t, s):
                     raise KernelError(f"{name}: {what} and {other} share memory")
+
+
+def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperatures=None, accept=None, draw=None, out=None, accepted=None):
+    """Which drafted tokens stand against the target's probabilities, and the token after the last that does: ``(out, accepted)``.
+
+    Request r has rows ``row_start[r]`` to ``row_start[r + 1] - 1`` (int32 [requests + 1]) of ``logits`` (float32 [rows, vocab]), one more
+    than it has drafts: row i is what the target says at the place of its i-th draft, the last what it says behind all of them.
+    ``drafts`` (int32 [rows]) holds the tokens in the same places (a request's last entry is not read).  ``draft_logits`` (float32
+    [rows - requests, vocab]): the draft model's rows, one a draft, request by request; without it a draft counts as drawn with
+    probability 1 (looked up).  ``temperatures`` (float32 [requests]), ``accept`` and ``draw`` (float32 [rows], uniform in [0, 1)):
+    a request with a temperature T > 0 keeps draft x of row i with probability min(1, p(x) / q(x)), p and q the softmax of the two logits
+    over T: where ``accept[i] * q(x) < p(x)``; at the first that is not kept the token is drawn at ``draw[i]`` from max(p - q, 0),
+    behind the last one from p.  Temperature 0 (or no temperatures): drafts stand while they are the row's argmax (the lowest index among
+    ties), then the argmax follows.
+
+    ``out`` (int32 [rows]): the drafts that stand, the token after them, and -1 in the rest of the request's rows; ``accepted`` (int32
+    [requests]): how many stand; both are made here unless given.  A row that is reached and holds a non-finite logit, or a draft outside
+    the vocabulary, sets a status bit and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
+    name, rows, requests = "verify_drafts", drafts.numel(), row_start.numel() - 1
+    draws = temperatures is not None
+    if not (0 <= logits.get_device() == drafts.get_device() == row_start.get_device() == status.get_device() == torch.cuda.current_device()
+            and logits.dim() == 2 and logits.shape[0] == rows >= requests >= 1 <= logits.shape[1] and logits.stride(1) == 1 and logits.dtype == torch.float32
+            and drafts.dtype == row_start.dtype == status.dtype == torch.int32 and drafts.dim() == row_start.dim() == 1 and drafts.is_contiguous()
+            and row_start.is_contiguous() and out is None and accepted is None and draws == (accept is not None) == (draw is not None)
+            and (not draws or (temperatures.get_device() == accept.get_device() == draw.get_device() == logits.get_device()
+                               and temperatures.dtype == accept.dtype == draw.dtype == torch.float32 and temperatures.shape == (requests,)
+                               and accept.shape == draw.shape == (rows,) and temperatures.is_contiguous() and accept.is_contiguous() and draw.is_contiguous()))
+            and (draft_logits is None or (draft_logits.get_device() == logits.get_device() and draft_logits.dtype == torch.float32
+                                          and draft_logits.shape == (rows - requests, logits.shape[1]) and draft_logits.stride(1) == 1))):
+        _check_verify(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw, out, accepted)
+    vocab = logits.shape[1]
+    draft_rows = rows - requests if draft_logits is not None else 0          # none where nobody drafted anything
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+        out = drafts.new_empty(rows)
     if accepted is None:
-        accepted = torch.empty(requests, dtype=torch.int32, device=logits.device)
-    scratch = torch.empty((_lib or load_library()).sprout_verify_scratch_bytes(rows + draft_rows, requests, vocab), dtype=torch.uint8, device=logits.device)
-    _run("sprout_verify", _ptr(logits, "logits", torch.float32), logits.stride(0), _ptr(draft_logits, "draft_logits", torch.float32, True) if draft_rows else None,
+        accepted = drafts.new_empty(requests)
+    scratch = logits.new_empty((_lib or load_library()).sprout_verify_scratch_bytes(rows + draft_rows, requests, vocab), dtype=torch.uint8)
+    _run("sprout_verify", logits.data_ptr(), logits.stride(0), draft_logits.data_ptr() if draft_rows else None,
          draft_logits.stride(0) if draft_rows else 0, drafts.data_ptr(), row_start.data_ptr(), temperatures.data_ptr() if temperatures is not None else None,
          accept.data_ptr() if accept is not None else None, draw.data_ptr() if draw is not None else None, out.data_ptr(), accepted.data_ptr(),
-         scratch.data_ptr(), rows, draft_rows, requests, vocab, _ptr(status, "status", torch.int32), _stream())
+         scratch.data_ptr(), rows, draft_rows, requests, vocab, status.data_ptr(), _stream())
     return out, accepted
 
 

@@ -16,7 +16,7 @@ import numpy as np
 MEMBER_TOKENS = 16          # attention_prefix.cuh: MEMBER_TOKENS
 KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole steps
 NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS, MATRIX_ROWS = 16, 64, 16, 256      # rows of an item of each kind
-MATRIX_FROM = 128           # rows of a segment
+MATRIX_FROM = 48            # rows of a segment
 ITEM_STEPS = 0.5            # what an item of few rows costs beside its steps
 MAX_RANGES = 64             # of a segment
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
@@ -94,6 +94,43 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
     return segments, parents, np.repeat(first[leaves], lengths) + within, np.repeat(sees[leaves], lengths), within, np.repeat(request[leaves], lengths)
 
 
+def choose_kinds(rows, steps, whole, kv_heads: int, head_dim: int, slots: int, matrix_slots: int, narrow_slots: int) -> np.ndarray:
+    """The kind of every segment: 0 where ``whole`` allows it (tiles of 256 rows on tcgen05), 1 (tiles of 16 rows) or 2 (of 64).  Segments of
+    up to 16 rows are 1; of the four ways for the rest (0 or not where it may be, and 1 or 2 for all others) the one that a rough model of
+    the launches finds shortest.  Its constants are microseconds on a B200 at head size 64 and 128: a CTA's time for a step of 128 keys,
+    what it takes beside, and the partial results' way through memory.  Measured with it, head size 128: 20 requests over 16,384 keys
+    (28 heads over 4) as 0, 1, 2: 25.8, 48.4, 40.2 us; 32 over 1,024 (40 over 8): 20.7, 16.3, 20.5; head size 64 (14 over 2): 64 over
+    4,096: 19.4, 18.5, 19.5; 90 pairs of tokens over 1,000: 20.3, 17.5, 16.8."""
+    few = rows <= NARROW_ROWS
+    if few.all():
+        return np.ones(len(rows), dtype=np.int64)
+    wide_head = head_dim > 64
+    best = None
+    for matrix in ((True, False) if whole.any() else (False,)):
+        for others in (1, 2):
+            kind = np.where(few, 1, others)
+            if matrix:
+                kind[whole] = 0
+            cost, busy = 0.0, 0.0
+            for which, tile, places, beside, step in ((0, MATRIX_ROWS, matrix_slots, 6.5, 2.0 if wide_head else 1.4), (2, WIDE_ROWS, slots, 3.5, 5.0 if wide_head else 2.0),
+                                                      (1, NARROW_ROWS, narrow_slots, 2.0, 2.7 if wide_head else 2.2)):
+                of = kind == which
+                if not of.any():
+                    continue
+                tiles = -(-rows[of] // tile) * kv_heads
+                share = float((tiles * steps[of]).sum()) / places
+                length = max(1.0, share)
+                time = beside + step * (length + 0.75 if which == 1 else np.ceil(length))      # items of few rows are walked: some CTA has more
+                # SMs that the matrix items leave run the others meanwhile
+                cost += 1.0 + time * (1.0 if which == 0 or not busy else 0.3 + 0.7 * busy)
+                if which == 0:
+                    busy = min(1.0, float((tiles * -(-steps[of] // np.ceil(length))).sum()) / places)
+                cost += float((rows[of] * -(-steps[of] // np.ceil(length))).sum()) * kv_heads * head_dim * 8 / 6e6
+            if best is None or cost < best[0]:
+                best = cost, kind
+    return best[1]
+
+
 def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int, start: float, step: float) -> np.ndarray:
     """Into how many ranges each segment's keys go (``steps`` key steps, ``tiles`` tiles of rows), on a device that runs ``slots`` items at
     once, an item of n steps taking ``start + n * step``: ranges of the length that makes the fewest full rounds of items the shortest."""
@@ -155,7 +192,7 @@ class HostPlan:
     """The plan's arrays on the host: ``items`` [n, 8] (simple ones, or matrix, narrow and wide ones), ``order``, ``part_start``, ``seen``,
     ``extra``, ``table_of``."""
 
-    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0, narrow_slots: int | None = None):
+    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0, narrow_slots: int | None = None, head_dim: int = 64):
         tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
         if tables.ndim != 2 or q_start.ndim != 1 or contexts.ndim != 1 or len(contexts) == 0 or len(q_start) != len(contexts) + 1 or len(tables) < len(contexts):
             raise PlanError("a block table row and a context per request, and where each request's tokens start")
@@ -179,9 +216,8 @@ class HostPlan:
         rows = (np.array([s.token_end for s in segments]) - token_begin) * group
         # the kinds: 0 a matrix product's worth of rows over whole pages, 1 few rows, 2 more; all of 1 on the CUDA cores
         if tensor_cores:
-            kind = np.where(rows <= NARROW_ROWS, 1, 2)
-            if matrix_slots:
-                kind[(rows >= MATRIX_FROM) & (end % page_tokens == 0) & (begin % page_tokens == 0)] = 0
+            whole = (rows >= MATRIX_FROM) & (end % page_tokens == 0) & (begin % page_tokens == 0) if matrix_slots else np.zeros(len(segments), dtype=bool)
+            kind = choose_kinds(rows, -(-(end - begin) // KEY_STEP), whole, kv_heads, head_dim, slots, matrix_slots, narrow_slots or slots)
             tile_rows = np.array([MATRIX_ROWS, NARROW_ROWS, WIDE_ROWS])[kind]
         else:
             kind, tile_rows = np.ones(len(segments), dtype=np.int64), np.full(len(segments), SIMPLE_ROWS)

@@ -171,7 +171,7 @@ def test_later_tokens_do_not_reach_earlier_ones(dtype, status):
 
 def test_nan_in_a_seen_key_is_not_lost(status):
     """A NaN in a key or value that a row sees makes the row NaN, wherever in a tile it lies: a shared key every row, an own key its request's."""
-    step = Step(28, 4, 128, BF16, 16, [0] * 24, [40], [30] * 24, [1] * 24, seed=15)
+    step = Step(28, 4, 128, BF16, 16, [0] * 24, [600], [30] * 24, [1] * 24, seed=15)
     assert step.plan().host.matrix_items > 0
     for key in range(0, 64):
         saved = step.k[step.pages[0][key // 16], 1, key % 16, 5].clone()
@@ -179,7 +179,7 @@ def test_nan_in_a_seen_key_is_not_lost(status):
         out = step.run(status).view(24, 28, 128)
         step.k[step.pages[0][key // 16], 1, key % 16, 5] = saved
         assert bool(out[:, 7:14].isnan().all()) and not bool(out[:, :7].isnan().any()) and not bool(out[:, 14:].isnan().any())
-    step.v[step.pages[3][41], 0, 3, 9] = float("nan")
+    step.v[step.pages[3][601], 0, 3, 9] = float("nan")
     out = step.run(status).view(24, 28, 128)
     assert bool(out[3, :7, 9].isnan().all()) and int(out.isnan().sum()) == 7
 
