@@ -290,10 +290,10 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
 }
 
 template <int HD>
-int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, int items, int box_rows, cudaStream_t stream) {
+int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, int items, int ctas, int box_rows, cudaStream_t stream) {
   using L = Layout<HD>;
   if (reserve_shared<attention_prefix_stream_kernel<HD>>(L::SMEM, "attention_shared_prefix (few rows)")) return 1;
-  const long long pairs = (long long)items * p.kv_heads, slots = (long long)L::CTAS * sprout_sm_count();
+  const long long pairs = (long long)items * p.kv_heads, most = (long long)L::CTAS * sprout_sm_count(), slots = ctas < most ? ctas : most;
   SPROUT_REQUIRE(pairs <= 0x7fffffffLL, "attention_shared_prefix: too many items");
   sprout_launch(attention_prefix_stream_kernel<HD>, dim3((unsigned)(pairs < slots ? pairs : slots)), dim3(THREADS), L::SMEM, stream, map_k, map_v, p, (int)pairs, box_rows);
   return sprout_check_launch("attention_shared_prefix (few rows)");
@@ -302,12 +302,12 @@ int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, 
 }  // namespace
 
 // Items of up to 16 rows; the sizes are sprout_attention_prefix_tc_supported's.
-int sprout_attention_prefix_stream(const Params& p, int items, cudaStream_t stream) {
+int sprout_attention_prefix_stream(const Params& p, int items, int ctas, cudaStream_t stream) {
   const long long cache_rows = (long long)p.num_pages * p.kv_heads * p.page_tokens;
   SPROUT_REQUIRE(cache_rows <= 0x7fffffffLL && (p.head_dim == 64 || p.head_dim == 128), "attention_shared_prefix (few rows): sizes that are not taken");
   const int box_rows = p.page_tokens < KEYS ? p.page_tokens : KEYS;
   CUtensorMap map_k, map_v;
   if (tensor_map(p.k_cache, (int)cache_rows, p.head_dim, p.head_dim, box_rows, &map_k)) return 1;
   if (tensor_map(p.v_cache, (int)cache_rows, p.head_dim, p.head_dim, box_rows, &map_v)) return 1;
-  return p.head_dim == 64 ? launch<64>(map_k, map_v, p, items, box_rows, stream) : launch<128>(map_k, map_v, p, items, box_rows, stream);
+  return p.head_dim == 64 ? launch<64>(map_k, map_v, p, items, ctas, box_rows, stream) : launch<128>(map_k, map_v, p, items, ctas, box_rows, stream);
 }

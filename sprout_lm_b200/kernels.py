@@ -41,7 +41,7 @@ _SIGNATURES = {
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "sprout_attention_prefix_tc_supported": [_I, _I],
-    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_attention_prefix_mma_supported": [_I],
     "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
@@ -1058,7 +1058,7 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     items, order, part_start, seen, extra, table_of = plan.pointers
     at = scratch.data_ptr()
     _run("sprout_attention_prefix", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-         block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.matrix_items, host.narrow_items, host.wide_items, order, part_start, seen, extra, table_of,
+         block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.matrix_items, host.narrow_items, host.narrow_ctas, host.wide_items, order, part_start, seen, extra, table_of,
          at, at + 4 * host.parts * plan.heads * plan.head_dim, out.data_ptr(), out.stride(0), plan.dtype_code, host.tokens, host.parts, plan.heads, plan.kv_heads,
          plan.head_dim, plan.page_tokens, pages[0], status.data_ptr(), _stream())
 

@@ -17,6 +17,7 @@ MEMBER_TOKENS = 16          # attention_prefix.cuh: MEMBER_TOKENS
 KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole steps
 NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS, MATRIX_ROWS = 16, 64, 16, 256      # rows of an item of each kind
 MATRIX_FROM = 48            # rows of a segment
+MATRIX_US, MATRIX_STEP_US, NARROW_STEP_US = 8.0, 2.0, 2.0      # of items beside one another: a matrix item's start and step, a step of few rows
 ITEM_STEPS = 0.5            # what an item of few rows costs beside its steps
 MAX_RANGES = 64             # of a segment
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
@@ -98,9 +99,9 @@ def choose_kinds(rows, steps, whole, kv_heads: int, head_dim: int, slots: int, m
     """The kind of every segment: 0 where ``whole`` allows it (tiles of 256 rows on tcgen05), 1 (tiles of 16 rows) or 2 (of 64).  Segments of
     up to 16 rows are 1; of the four ways for the rest (0 or not where it may be, and 1 or 2 for all others) the one that a rough model of
     the launches finds shortest.  Its constants are microseconds on a B200 at head size 64 and 128: a CTA's time for a step of 128 keys,
-    what it takes beside, and the partial results' way through memory.  Measured with it, head size 128: 20 requests over 16,384 keys
-    (28 heads over 4) as 0, 1, 2: 25.8, 48.4, 40.2 us; 32 over 1,024 (40 over 8): 20.7, 16.3, 20.5; head size 64 (14 over 2): 64 over
-    4,096: 19.4, 18.5, 19.5; 90 pairs of tokens over 1,000: 20.3, 17.5, 16.8."""
+    what it takes beside, and the partial results' way through memory.  Measured, head size 128: 20 requests over 16,384 keys
+    (28 heads over 4) as 0, 1, 2: 23.1, 48.4, 40.3 us; 24 of 4 tokens over 2,000: 26.4, 40.3, 33.4; 6 over 30,000 (40 over 8): -, 42.8,
+    56.0; head size 64 (14 over 2): 64 over 1,024: 12.0, 9.7, 11.3; 90 pairs of tokens over 1,000: 20.4, 17.6, 16.8."""
     few = rows <= NARROW_ROWS
     if few.all():
         return np.ones(len(rows), dtype=np.int64)
@@ -111,8 +112,8 @@ def choose_kinds(rows, steps, whole, kv_heads: int, head_dim: int, slots: int, m
             kind = np.where(few, 1, others)
             if matrix:
                 kind[whole] = 0
-            cost, busy = 0.0, 0.0
-            for which, tile, places, beside, step in ((0, MATRIX_ROWS, matrix_slots, 6.5, 2.0 if wide_head else 1.4), (2, WIDE_ROWS, slots, 3.5, 5.0 if wide_head else 2.0),
+            cost = 0.0
+            for which, tile, places, beside, step in ((0, MATRIX_ROWS, matrix_slots, 6.5 if wide_head else 7.5, 2.0 if wide_head else 1.4), (2, WIDE_ROWS, slots, 3.5, 7.5 if wide_head else 3.5),
                                                       (1, NARROW_ROWS, narrow_slots, 2.0, 2.7 if wide_head else 2.2)):
                 of = kind == which
                 if not of.any():
@@ -121,10 +122,12 @@ def choose_kinds(rows, steps, whole, kv_heads: int, head_dim: int, slots: int, m
                 share = float((tiles * steps[of]).sum()) / places
                 length = max(1.0, share)
                 time = beside + step * (length + 0.75 if which == 1 else np.ceil(length))      # items of few rows are walked: some CTA has more
-                # SMs that the matrix items leave run the others meanwhile
-                cost += 1.0 + time * (1.0 if which == 0 or not busy else 0.3 + 0.7 * busy)
                 if which == 0:
-                    busy = min(1.0, float((tiles * -(-steps[of] // np.ceil(length))).sum()) / places)
+                    ctas = float((tiles * -(-steps[of] // np.ceil(length))).sum())
+                    alone, free = time, max(0.0, 1.0 - ctas / places)
+                elif matrix and free > 0:                # on the SMs that the matrix items leave, or behind them
+                    time = min(time, max(0.0, beside + step * (max(1.0, share / free) + 0.75) - alone))
+                cost += 1.0 + time
                 cost += float((rows[of] * -(-steps[of] // np.ceil(length))).sum()) * kv_heads * head_dim * 8 / 6e6
             if best is None or cost < best[0]:
                 best = cost, kind
@@ -160,9 +163,10 @@ def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int, star
 
 def spread(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> np.ndarray:
     """The same for items that ``slots`` CTAs walk, each taking one of every ``slots`` of them, longest first, forwards and backwards in
-    turn: ranges of the length with which the CTA that has most to do has least (an item costs ``ITEM_STEPS`` steps beside its own)."""
+    turn: ranges of the length with which the CTA that has most to do has least (an item costs ``ITEM_STEPS`` steps beside its own), and
+    how much that is."""
     if not len(tiles):
-        return steps
+        return steps, 0.0
 
     def busiest(length):
         ranges = np.minimum(-(-steps // length), MAX_RANGES)
@@ -184,8 +188,8 @@ def spread(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> n
             middle = (low + high) // 2
             low, high = (low, middle) if count(middle) <= slots else (middle + 1, high)
         lengths.add(low)
-    best = min(sorted(lengths, reverse=True), key=busiest)
-    return np.minimum(-(-steps // best), MAX_RANGES)
+    most, best = min((busiest(n), -n) for n in lengths)
+    return np.minimum(-(-steps // -best), MAX_RANGES), float(most)
 
 
 class HostPlan:
@@ -206,6 +210,7 @@ class HostPlan:
             raise PlanError("a context reaches beyond its block table")
         if kv_heads < 1 or heads < 1 or heads % kv_heads:
             raise PlanError(f"heads ({heads}) must be a multiple of the key/value heads ({kv_heads})")
+        self.narrow_ctas = 0                             # that walk the narrow items
         self.tokens, self.requests = int(q_start[-1]), len(contexts)
         self.pages = int(-(-contexts.max() // page_tokens))
         group = heads // kv_heads
@@ -228,7 +233,16 @@ class HostPlan:
         if tensor_cores:
             wide, narrow = kind == 2, kind == 1
             ranges[wide] = divide(tiles[wide], steps[wide], kv_heads, slots, 4.0, 1.5)
-            ranges[narrow] = spread(tiles[narrow], steps[narrow], kv_heads, narrow_slots or slots)
+            self.narrow_ctas = narrow_slots or slots
+            ranges[narrow], most = spread(tiles[narrow], steps[narrow], kv_heads, self.narrow_ctas)
+            ctas = int((tiles[matrix] * ranges[matrix]).sum()) * kv_heads
+            if narrow.any() and 0 < ctas < matrix_slots:
+                # beside matrix items that leave some SMs: all there, if that is done before both one behind the other would be
+                beside = (matrix_slots - ctas) * self.narrow_ctas // matrix_slots
+                alone_us = -(-steps[matrix] // ranges[matrix]).max() * MATRIX_STEP_US + MATRIX_US
+                apart, there = spread(tiles[narrow], steps[narrow], kv_heads, beside)
+                if max(alone_us, there * NARROW_STEP_US) < alone_us + most * NARROW_STEP_US:
+                    ranges[narrow], self.narrow_ctas = apart, beside
         else:
             ranges[:] = divide(tiles, steps, kv_heads, slots, 4.0, 1.5)
         per_range = -(-steps // ranges)                  # steps of a range
