@@ -20,7 +20,7 @@ namespace {
 
 // ------------------------------------------------------------------ CUDA cores
 // 16 rows, 64 keys at a time in shared memory as float32.  A thread has 2 rows x 4 keys of the scores, and 2 rows x 4 columns in
-// every 64 of the output.
+// every 64 of the output: six 16-byte reads of shared memory for 32 fused multiply-adds, which bound it.
 constexpr int SIMPLE_ROWS = 16, SIMPLE_KEYS = 64, SIMPLE_THREADS = 128;
 
 __host__ __device__ constexpr int simple_width(int head_dim) { return (head_dim + 3) / 4 * 4; }
@@ -29,8 +29,23 @@ size_t simple_smem(int head_dim) {
   return ((w + 4) * (SIMPLE_KEYS + SIMPLE_ROWS) + w * SIMPLE_KEYS + SIMPLE_ROWS * (SIMPLE_KEYS + 4) + SIMPLE_ROWS * 3) * sizeof(float) + SIMPLE_KEYS * sizeof(long long);
 }
 
+// Four elements of a row from column c on, zero from head_dim on; FOURS: rows are whole fours and start on their boundaries.
+template <bool FOURS> __device__ __forceinline__ float4 load_elements(const float* row, int c, int head_dim) {
+  if (FOURS) return c < head_dim ? *(const float4*)(row + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  return make_float4(c < head_dim ? row[c] : 0.f, c + 1 < head_dim ? row[c + 1] : 0.f, c + 2 < head_dim ? row[c + 2] : 0.f, c + 3 < head_dim ? row[c + 3] : 0.f);
+}
+template <bool FOURS> __device__ __forceinline__ float4 load_elements(const __nv_bfloat16* row, int c, int head_dim) {
+  if (FOURS) {
+    if (c >= head_dim) return make_float4(0.f, 0.f, 0.f, 0.f);
+    const uint2 t = *(const uint2*)(row + c);
+    return make_float4(__uint_as_float(t.x << 16), __uint_as_float(t.x & 0xffff0000u), __uint_as_float(t.y << 16), __uint_as_float(t.y & 0xffff0000u));
+  }
+  return make_float4(c < head_dim ? to_float(row[c]) : 0.f, c + 1 < head_dim ? to_float(row[c + 1]) : 0.f, c + 2 < head_dim ? to_float(row[c + 2]) : 0.f,
+                     c + 3 < head_dim ? to_float(row[c + 3]) : 0.f);
+}
+
 // COLUMNS: of 64, that hold head_dim
-template <typename T, int COLUMNS>
+template <typename T, int COLUMNS, bool FOURS>
 __global__ void __launch_bounds__(SIMPLE_THREADS)
 attention_prefix_simple_kernel(const Params p) {
   extern __shared__ __align__(16) float simple_shared[];
@@ -47,12 +62,15 @@ attention_prefix_simple_kernel(const Params p) {
   const Item item = p.items[blockIdx.x];
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
-  for (int idx = tid; idx < SIMPLE_ROWS * w; idx += SIMPLE_THREADS) {
-    const int i = idx / w, c = idx % w;
-    float v = 0.f;
-    if (i < item.rows && c < p.head_dim)
-      v = to_float(((const T*)p.q)[(size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * p.head_dim + c]);
-    sQ[i * ks + c] = v;
+  // a thread keeps its four columns and walks down the rows
+  constexpr int PIECES = 16 * COLUMNS, AT_ONCE = SIMPLE_THREADS / PIECES;
+  const int own_c = tid % PIECES * 4, own_row = tid / PIECES;
+#pragma unroll
+  for (int i = own_row; i < SIMPLE_ROWS; i += AT_ONCE) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < item.rows)
+      v = load_elements<FOURS>((const T*)p.q + (size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * p.head_dim, own_c, p.head_dim);
+    if (own_c < w) *(float4*)(sQ + i * ks + own_c) = v;
   }
   if (tid < SIMPLE_ROWS) { s_m[tid] = -INFINITY; s_l[tid] = 0.f; }
   const int r0 = tid / 16 * 2, c0 = tid % 16 * 4;
@@ -67,12 +85,23 @@ attention_prefix_simple_kernel(const Params p) {
     __syncthreads();                                   // the pass before is done with the keys and values
     if (tid < SIMPLE_KEYS) rows[tid] = base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1;
     __syncthreads();
-    for (int idx = tid; idx < SIMPLE_KEYS * w; idx += SIMPLE_THREADS) {
-      const int j = idx / w, c = idx % w;
-      const long long at = rows[j];
-      const bool has = at >= 0 && c < p.head_dim;
-      sK[j * ks + c] = has ? to_float(((const T*)p.k_cache)[at + c]) : 0.f;
-      sV[j * w + c] = has ? to_float(((const T*)p.v_cache)[at + c]) : 0.f;
+    if (own_c < w) {
+      constexpr int BATCH = 8;                         // rows of keys and values on their way at a time
+#pragma unroll
+      for (int j0 = 0; j0 < SIMPLE_KEYS; j0 += BATCH * AT_ONCE) {
+        float4 k[BATCH], v[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) {
+          const long long at = rows[j0 + j * AT_ONCE + own_row];
+          k[j] = at >= 0 ? load_elements<FOURS>((const T*)p.k_cache + at, own_c, p.head_dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[j] = at >= 0 ? load_elements<FOURS>((const T*)p.v_cache + at, own_c, p.head_dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) {
+          *(float4*)(sK + (j0 + j * AT_ONCE + own_row) * ks + own_c) = k[j];
+          *(float4*)(sV + (j0 + j * AT_ONCE + own_row) * w + own_c) = v[j];
+        }
+      }
     }
     __syncthreads();
     float s[2][4] = {};
@@ -119,16 +148,21 @@ attention_prefix_simple_kernel(const Params p) {
     for (int b = 0; b < COLUMNS; b++)
 #pragma unroll
       for (int c = 0; c < 4; c++) { acc[0][b][c] *= a0; acc[1][b][c] *= a1; }
-    for (int j = 0; j < SIMPLE_KEYS; j++) {
-      const float p0 = sP[r0 * (SIMPLE_KEYS + 4) + j], p1 = sP[(r0 + 1) * (SIMPLE_KEYS + 4) + j];
+    for (int j = 0; j < SIMPLE_KEYS; j += 4) {
+      float p0[4], p1[4];
+      *(float4*)p0 = *(const float4*)(sP + r0 * (SIMPLE_KEYS + 4) + j);
+      *(float4*)p1 = *(const float4*)(sP + (r0 + 1) * (SIMPLE_KEYS + 4) + j);
 #pragma unroll
       for (int b = 0; b < COLUMNS; b++) {
         if (b * 64 + c0 >= w) break;
-        const float4 v = *(const float4*)(sV + j * w + b * 64 + c0);
-        acc[0][b][0] = fmaf(p0, v.x, acc[0][b][0]); acc[0][b][1] = fmaf(p0, v.y, acc[0][b][1]);
-        acc[0][b][2] = fmaf(p0, v.z, acc[0][b][2]); acc[0][b][3] = fmaf(p0, v.w, acc[0][b][3]);
-        acc[1][b][0] = fmaf(p1, v.x, acc[1][b][0]); acc[1][b][1] = fmaf(p1, v.y, acc[1][b][1]);
-        acc[1][b][2] = fmaf(p1, v.z, acc[1][b][2]); acc[1][b][3] = fmaf(p1, v.w, acc[1][b][3]);
+#pragma unroll
+        for (int jj = 0; jj < 4; jj++) {
+          const float4 v = *(const float4*)(sV + (j + jj) * w + b * 64 + c0);
+          acc[0][b][0] = fmaf(p0[jj], v.x, acc[0][b][0]); acc[0][b][1] = fmaf(p0[jj], v.y, acc[0][b][1]);
+          acc[0][b][2] = fmaf(p0[jj], v.z, acc[0][b][2]); acc[0][b][3] = fmaf(p0[jj], v.w, acc[0][b][3]);
+          acc[1][b][0] = fmaf(p1[jj], v.x, acc[1][b][0]); acc[1][b][1] = fmaf(p1[jj], v.y, acc[1][b][1]);
+          acc[1][b][2] = fmaf(p1[jj], v.z, acc[1][b][2]); acc[1][b][3] = fmaf(p1[jj], v.w, acc[1][b][3]);
+        }
       }
     }
   }
@@ -479,17 +513,17 @@ attention_prefix_merge_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ launches
-template <typename T, int COLUMNS>
+template <typename T, int COLUMNS, bool FOURS>
 int launch_simple(const Params& p, int items, cudaStream_t stream) {
-  if (reserve_shared<attention_prefix_simple_kernel<T, COLUMNS>>(simple_smem(COLUMNS * 64), "attention_shared_prefix")) return 1;
-  sprout_launch(attention_prefix_simple_kernel<T, COLUMNS>, dim3(items, p.kv_heads), dim3(SIMPLE_THREADS), simple_smem(p.head_dim), stream, p);
+  if (reserve_shared<attention_prefix_simple_kernel<T, COLUMNS, FOURS>>(simple_smem(COLUMNS * 64), "attention_shared_prefix")) return 1;
+  sprout_launch(attention_prefix_simple_kernel<T, COLUMNS, FOURS>, dim3(items, p.kv_heads), dim3(SIMPLE_THREADS), simple_smem(p.head_dim), stream, p);
   return sprout_check_launch("attention_prefix_simple");
 }
-template <typename T>
+template <typename T, bool FOURS>
 int launch_simple_any(const Params& p, int items, cudaStream_t stream) {
-  if (p.head_dim <= 64) return launch_simple<T, 1>(p, items, stream);
-  if (p.head_dim <= 128) return launch_simple<T, 2>(p, items, stream);
-  return launch_simple<T, 4>(p, items, stream);
+  if (p.head_dim <= 64) return launch_simple<T, 1, FOURS>(p, items, stream);
+  if (p.head_dim <= 128) return launch_simple<T, 2, FOURS>(p, items, stream);
+  return launch_simple<T, 4, FOURS>(p, items, stream);
 }
 
 template <int HD, bool NARROW>
@@ -550,7 +584,11 @@ SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const 
   Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, (const Item*)items, order, part_start, seen, extra, table_of, part_out, (float2*)part_sum, out, out_stride,
            tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, 1};
   if (simple_items > 0) {
-    if (dtype == SPROUT_F32 ? launch_simple_any<float>(p, simple_items, stream) : launch_simple_any<__nv_bfloat16>(p, simple_items, stream)) return 1;
+    // rows that are whole fours on their boundaries
+    const int row = dtype == SPROUT_F32 ? 16 : 8;
+    const bool fours = head_dim % 4 == 0 && q_stride % 4 == 0 && (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & (row - 1)) == 0;
+    if (dtype == SPROUT_F32 ? (fours ? launch_simple_any<float, true>(p, simple_items, stream) : launch_simple_any<float, false>(p, simple_items, stream))
+                            : (fours ? launch_simple_any<__nv_bfloat16, true>(p, simple_items, stream) : launch_simple_any<__nv_bfloat16, false>(p, simple_items, stream))) return 1;
   } else {
     SPROUT_REQUIRE(dtype == SPROUT_BF16 && sprout_attention_prefix_mma_supported(head_dim), "attention_shared_prefix: these sizes run on the CUDA cores");
     SPROUT_REQUIRE(((uintptr_t)q & 15) == 0 && q_stride % 8 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0,

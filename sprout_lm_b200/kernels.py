@@ -983,7 +983,7 @@ def _prefix_slots(head_dim: int, tensor_cores: bool) -> tuple[int, int, int]:
     that walk those of up to 16."""
     sms = sm_count() if torch.cuda.is_available() else 148
     if not tensor_cores:
-        return 2 * sms, 0, 0
+        return sms * (4 if head_dim <= 64 else 2 if head_dim <= 128 else 1), 0, 0
     return sms * (3 if head_dim > 96 else 4), sms, sms * (2 if head_dim > 64 else 3 if head_dim > 48 else 4)
 
 

@@ -141,12 +141,13 @@ def test_branching_prefixes(status):
     step.check(status)
 
 
-def test_strided_rows(status):
-    step = Step(14, 2, 64, BF16, 16, [0] * 5, [20], [5, 9, 0, 30, 100], [2, 1, 1, 3, 1], seed=6)
-    wide = torch.full((step.q.shape[0], step.q.shape[1] + 256), float("nan"), dtype=BF16, device=DEV)
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F32, 64), (F32, 34), (BF16, 40)])
+def test_strided_rows(dtype, dim, status):
+    step = Step(14, 2, dim, dtype, 16, [0] * 5, [20], [5, 9, 0, 30, 100], [2, 1, 1, 3, 1], seed=6)
+    wide = torch.full((step.q.shape[0], step.q.shape[1] + (256 if dim == 64 and dtype == BF16 else 3)), float("nan"), dtype=dtype, device=DEV)
     wide[:, :step.q.shape[1]] = step.q
     step.q = wide[:, :step.q.shape[1]]
-    out = torch.full((step.q.shape[0], step.q.shape[1] + 3), 7.0, dtype=BF16, device=DEV)
+    out = torch.full((step.q.shape[0], step.q.shape[1] + 3), 7.0, dtype=dtype, device=DEV)
     step.check(status, out[:, :step.q.shape[1]])
     assert bool((out[:, step.q.shape[1]:] == 7.0).all())
 
