@@ -45,6 +45,7 @@ class StepContext:
     # captured graph, that of the steps it is replayed for (0: max_context)
     planned_context: int = 0
     context_total: int = 0          # the requests' contexts together, as the step was staged (0: not known)
+    shared: dict | None = None      # plans of the requests' shared pages by attention sizes (``engine.shared``), for parts that take them
 
     @property
     def all_decode(self) -> bool:

@@ -13,7 +13,8 @@ from .step import ModelRunner
 def make_engine(model, options: EngineOptions | None = None) -> Engine:
     options = options or EngineOptions()
     runner = ModelRunner(model, num_pages=options.num_blocks, page_tokens=options.block_size,
-                         max_requests=options.max_sequences, prefix_caching=options.prefix_caching)
+                         max_requests=options.max_sequences, prefix_caching=options.prefix_caching,
+                         shared_prefix=options.shared_prefix)
     return Engine(runner, options)
 
 

@@ -43,10 +43,12 @@ class EngineOptions:
     # Not in the reference either: start the next decode step before this step's tokens are read,
     # when it is already known what that step will be (see Engine._next_step).
     launch_ahead: bool = True
+    # Not in the reference: pages that running requests share are read once for all of them by steps where that pays (engine/shared.py).
+    shared_prefix: bool = False
 
     def validate(self):
         for name, value in asdict(self).items():
-            if name in ("prefix_caching", "record_trace", "admit_within_pool", "launch_ahead"):
+            if name in ("prefix_caching", "record_trace", "admit_within_pool", "launch_ahead", "shared_prefix"):
                 if not isinstance(value, bool):
                     raise ValueError(f"{name} must be a boolean.")
             elif not isinstance(value, int) or isinstance(value, bool) or value <= 0:

@@ -15,6 +15,7 @@ from .. import kernels, sampling
 from ..cache.manager import CacheManager
 from ..cache.storage import CacheStorage, check_capacity, plan_groups, state_slot_count
 from .batch import BatchStager, StepContext, StepEntry
+from .shared import SharedPrefixSteps
 
 
 class StepError(RuntimeError):
@@ -23,7 +24,9 @@ class StepError(RuntimeError):
 
 class ModelRunner:
     def __init__(self, model, num_pages: int, page_tokens: int = 16, max_requests: int = 64,
-                 prefix_caching: bool = True):
+                 prefix_caching: bool = True, shared_prefix: bool = False):
+        """``shared_prefix``: steps of few tokens a request read pages that requests share once for all of them where that pays
+        (``engine.shared``; bfloat16 attention with grouped queries)."""
         if model.runtime is None:
             raise StepError("the model has no weights loaded")
         self.model = model
@@ -55,6 +58,7 @@ class ModelRunner:
         from .graphs import GraphCache, StepGraphs
         self.graphs = GraphCache(self)
         self.step_graphs = StepGraphs(self)
+        self.shared_prefix = SharedPrefixSteps(self) if shared_prefix else None
 
     # ------------------------------------------------------------------ requests' caches
     def new_sequence(self, tokens=None):
@@ -164,8 +168,10 @@ class ModelRunner:
         lengths are advanced."""
         self._take_ahead(None, None, None)
         self.validate(entries)
-        key, width = self.step_graphs.plan(entries, sample=False)
+        shared = self.shared_prefix.plans(entries, replayed=False) if self.shared_prefix else None
+        key, width = self.step_graphs.plan(entries, sample=False) if shared is None else (None, None)
         ctx = self.stager.stage(entries, self.page_tokens, fixed_pages=width)
+        ctx.shared = shared
         if key is None:
             logits = self.forward(ctx)
         else:
@@ -186,7 +192,8 @@ class ModelRunner:
         self.validate(entries)
         decode_only = self.graphs.enabled and all(len(e.tokens) == 1 and e.want == [0] for e in entries)
         taken = self._take_ahead(entries, temperatures, uniforms)
-        if decode_only:
+        shared = self.shared_prefix.plans(entries, replayed=decode_only) if self.shared_prefix and taken is None else None
+        if decode_only and shared is None:
             if taken is None:
                 graph = self.graphs.get(entries)
                 if graph.graph is None:
@@ -210,8 +217,9 @@ class ModelRunner:
             self.steps_run += 1
             return sampled
         floats = {"temperature": temperatures, "uniform": uniforms} if temperatures else None
-        key, width = self.step_graphs.plan(entries, sample=bool(temperatures))
+        key, width = self.step_graphs.plan(entries, sample=bool(temperatures)) if shared is None else (None, None)
         ctx = self.stager.stage(entries, self.page_tokens, fixed_pages=width, floats=floats)
+        ctx.shared = shared
         self.stats["h2d_bytes"] += self.stager.last_bytes
         if key is not None:
             _, tokens = self.step_graphs.run(key, ctx, sample=bool(temperatures))
@@ -228,6 +236,50 @@ class ModelRunner:
             return []
         self.stats["d2h_bytes"] += tokens.numel() * 4
         return tokens.tolist()
+
+    def step_and_verify(self, entries: list[StepEntry], temperatures, accept, draw, draft_logits: torch.Tensor | None = None) -> list[list[int]]:
+        """Run one batch of drafted tokens and keep what the model confirms.  An entry's ``tokens`` are the request's last token and, behind it,
+        its drafts (none: a plain step); ``want`` is not read.  Returns per entry the drafts that stand and the token after them, at least one
+        token; the request's length advances past its last token and the drafts that stand, and what the rest left in the cache is
+        written again by what comes next.
+
+        ``temperatures``: per entry (0: greedy); ``accept`` and ``draw``: uniform numbers in [0, 1), one per token of the batch, the
+        first for whether the draft behind the token stands, the second for the token drawn there (``sampling.verify_uniforms`` makes
+        them).  ``draft_logits``: the draft model's float32 rows [drafts, vocab] entry by entry, None for drafts that were looked up.
+        A request whose logits are not finite gets -1 (``check_status`` says why).  Models that keep per-request state cannot take
+        tokens back: refused."""
+        self._take_ahead(None, None, None)
+        if self.manager.state_slot_count:
+            raise StepError("a model with per-request state cannot take drafted tokens back")
+        counts = [len(e.tokens) for e in entries]
+        total = sum(counts)
+        if len(temperatures) != len(entries) or len(accept) != total or len(draw) != total:
+            raise StepError("a temperature per request, and two uniform numbers per token")
+        entries = [StepEntry(e.seq, e.tokens, list(range(n))) for e, n in zip(entries, counts)]
+        self.validate(entries)
+        if draft_logits is not None and tuple(draft_logits.shape) != (total - len(entries), self.vocab_size):
+            raise StepError(f"draft_logits must be [{total - len(entries)}, {self.vocab_size}], a row per draft")
+        drafts = [t for e in entries for t in (*e.tokens[1:], 0)]
+        floats = {"temperature": temperatures, "accept": accept, "draw": draw, "drafts": np.asarray(drafts, dtype=np.int32).view(np.float32)}
+        shared = self.shared_prefix.plans(entries, replayed=False) if self.shared_prefix else None
+        ctx = self.stager.stage(entries, self.page_tokens, floats=floats)
+        ctx.shared = shared
+        self.stats["h2d_bytes"] += self.stager.last_bytes
+        logits = self.forward(ctx)
+        values = ctx.floats
+        drawn = any(t > 0 for t in temperatures)
+        tokens, accepted = sampling.verify(logits, values["drafts"].view(torch.int32), ctx.q_start, self.runtime.status, draft_logits if drawn else None,
+                                           *((values[name] for name in ("temperature", "accept", "draw")) if drawn else (None, None, None)))
+        both = torch.cat([tokens, accepted]).tolist()
+        self.stats["d2h_bytes"] += 4 * len(both)
+        result, at = [], 0
+        for e, n, kept in zip(entries, counts, both[total:]):
+            result.append(both[at:at + kept + 1])
+            at += n
+            e.seq.length += 1 + kept
+            self.manager.trim(e.seq)
+        self.steps_run += 1
+        return result
 
     def decode_loop(self, entries, temperatures, uniforms, max_steps: int):
         """A device-side run of decode steps (see ``graphs.DecodeLoop``): pages for ``max_steps``

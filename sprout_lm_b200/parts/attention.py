@@ -55,6 +55,10 @@ class PagedGQAttention(Part):
         return kernels.decode_attention_plan(requests, self.heads, self.kv_heads, self.head_dim, page_tokens, max_keys,
                                              planned_context)
 
+    def shared_prefix_sizes(self):
+        """(query heads, key/value heads, head size): what a plan of shared pages (``kernels.shared_prefix_plan``) is made for."""
+        return self.heads, self.kv_heads, self.head_dim
+
     # ---- weights
     def tensor_decls(self):
         q_width, kv_width = self.heads * self.head_dim, self.kv_heads * self.head_dim
@@ -115,7 +119,7 @@ class PagedGQAttention(Part):
     def _decodes_fused(self, tokens, ctx, cache) -> bool:
         """One token per request, the projection's tail inside the attention kernel: then that kernel
         can also apply the norm's scale, and the q/k/v product takes the rows as they are."""
-        return tokens <= self.SPLIT_TOKENS and ctx.max_q_len == 1 and cache.write and \
+        return tokens <= self.SPLIT_TOKENS and ctx.max_q_len == 1 and cache.write and ctx.shared is None and \
             kernels.decode_fusable(tokens, self.heads, self.kv_heads, self.head_dim, cache.block_table.shape[1] * cache.page_tokens)
 
     def forward(self, h, x, ctx, cache: CacheView, state=None, norm=None):
@@ -134,7 +138,7 @@ class PagedGQAttention(Part):
                 self.qkv.accumulate(h if h is not None else norm.forward(x), acc)
             attended = torch.empty((tokens, self.heads * self.head_dim), dtype=dtype, device=x.device)
             max_keys = cache.block_table.shape[1] * cache.page_tokens
-            if ctx.max_q_len == 1 and cache.write and kernels.decode_fusable(tokens, self.heads, self.kv_heads,
+            if ctx.max_q_len == 1 and cache.write and ctx.shared is None and kernels.decode_fusable(tokens, self.heads, self.kv_heads,
                                                                              self.head_dim, max_keys):
                 # one token per request: bias, rotation and the cache append happen inside the attention kernel
                 planned = ctx.planned_context or ctx.max_context
@@ -165,6 +169,10 @@ class PagedGQAttention(Part):
                                 self.runtime.status, interleaved=self.interleaved)
         q = qkv[:, :self.heads * self.head_dim]
         attended = torch.empty((tokens, self.heads * self.head_dim), dtype=qkv.dtype, device=qkv.device)
-        kernels.paged_attention(q, cache, ctx, attended, self.heads, self.kv_heads, self.head_dim,
-                                self.runtime.status)
+        plan = ctx.shared.get(self.shared_prefix_sizes()) if ctx.shared is not None else None
+        if plan is not None:
+            kernels.attention_shared_prefix(q, cache.k, cache.v, cache.block_table, ctx.positions, plan, attended, self.runtime.status)
+        else:
+            kernels.paged_attention(q, cache, ctx, attended, self.heads, self.kv_heads, self.head_dim,
+                                    self.runtime.status)
         self.out.forward(attended, residual=x)

@@ -25,6 +25,13 @@ def uniform_for(seed: int, request_id: str, index: int) -> float:
     return (int.from_bytes(digest, "little") >> 40) / float(1 << 24)
 
 
+def verify_uniforms(seed: int, request_id: str, index: int, tokens: int) -> tuple[list, list]:
+    """The numbers that check ``tokens`` - 1 drafts from output token ``index`` of a request on: (accept, draw), one each per token of its
+    step.  Functions of (seed, request id, index of the output token) alone; the draws are those of plain sampling (``uniform_for``)."""
+    return ([uniform_for(seed, f"{request_id}:accept", index + i) for i in range(tokens)],
+            [uniform_for(seed, request_id, index + i) for i in range(tokens)])
+
+
 def sample(logits: torch.Tensor, status: torch.Tensor, temperatures: torch.Tensor | None = None,
            uniforms: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Token ids (int32, on the device) from float32 logits [rows, vocab].
