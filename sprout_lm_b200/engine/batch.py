@@ -92,10 +92,10 @@ class BatchStager:
             at += _pad4(max(n, 1))
         return offsets, at
 
-    def stage(self, entries, page_tokens: int, fixed_pages: int | None = None, floats=None) -> StepContext:
+    def stage(self, entries, page_tokens: int, fixed_pages: int | None = None, floats=None, tables=None) -> StepContext:
         """Pack and copy.  ``fixed_pages`` fixes the block tables' width (a replayed CUDA graph
         needs the same layout every time); ``floats`` are extra float32 arrays (name -> values)
-        that travel in the same copy."""
+        that travel in the same copy; ``tables``: block tables that are at hand as arrays, by group."""
         R = len(entries)
         counts = [len(e.tokens) for e in entries]
         T = sum(counts)
@@ -136,9 +136,12 @@ class BatchStager:
             put(f"float:{name}", np.asarray(values, dtype=np.float32).view(np.int32))
         for g in range(self.num_groups):
             table = np.full((R, max_pages), -1, dtype=np.int32)
-            for i, e in enumerate(entries):
-                pages = e.seq.tables[g]
-                table[i, :len(pages)] = pages
+            if tables is not None and g in tables:
+                table[:, :tables[g].shape[1]] = tables[g]
+            else:
+                for i, e in enumerate(entries):
+                    pages = e.seq.tables[g]
+                    table[i, :len(pages)] = pages
             put(f"table{g}", table.reshape(-1))
         self._device_buf[:total].copy_(host[:total], non_blocking=True)
         self.last_bytes = total * 4

@@ -8,6 +8,8 @@ then differ from the other kernels' in the order of float32 additions, as betwee
 """
 from __future__ import annotations
 
+import weakref
+
 import numpy as np
 import torch
 
@@ -15,27 +17,21 @@ from .. import kernels
 from ..prefix_plan import MEMBER_TOKENS
 
 BYTES_PER_US = 6.4e6               # what attention streams keys and values at
-PLAN_US, PLAN_REQUEST_US = 400.0, 10.0         # a plan, and for each request of it
-EAGER_LAYER_US = 90.0              # a layer's launches one by one beside a replay of them
+# A plan, for each request of it, and a layer's launches one by one beside a replay of them (measured: 64 requests of the 0.5B shape over
+# 4,096 shared keys take 1.55 ms a step as a replay and 4.3 with a plan; over 32,768, 4.3 and 4.5; its 24 layers' attention alone 0.6 and 0.5, 4.0 and 0.9)
+PLAN_US, PLAN_REQUEST_US, EAGER_LAYER_US = 600.0, 10.0, 130.0
 
 
-def shared_keys(tables, page_tokens: int) -> int:
-    """Key reads that reading common leading pages once saves, at least: over the requests with the same first page, what all of them hold.
-    The lists between the least and the greatest in order share what those two do."""
-    groups: dict = {}
-    for table in tables:
-        if table:
-            groups.setdefault(table[0], []).append(table)
+def shared_keys(table: np.ndarray, whole: np.ndarray, page_tokens: int) -> int:
+    """Key reads that reading common leading pages once saves, at least: over the requests with the same first page, the pages that all of
+    them hold; ``whole``: a request's pages that its tokens all see in full."""
     saved = 0
-    for group in groups.values():
+    for first in np.unique(table[:, 0]):
+        group = np.flatnonzero((table[:, 0] == first) & (whole > 0))
         if len(group) > 1:
-            low, high = min(group), max(group)
-            common = 0
-            for a, b in zip(low, high):
-                if a != b:
-                    break
-                common += 1
-            saved += (len(group) - 1) * common * page_tokens
+            rows = table[group, :int(whole[group].min())]
+            same = (rows == rows[0]).all(axis=0)
+            saved += (len(group) - 1) * (int(same.argmin()) if not same.all() else rows.shape[1]) * page_tokens
     return saved
 
 
@@ -46,8 +42,10 @@ class SharedPrefixSteps:
         self.runner = runner
         self.always = False
         self.steps = 0                     # steps that took a plan
+        self.tables: dict = {}             # the last such step's block tables as arrays, by group
         manager, runtime = runner.manager, runner.runtime
         self.group = next((g for g in runner._groups_in_use if manager.groups[g].kind == "full"), None)
+        self._tables = weakref.WeakKeyDictionary()          # request's cache -> its block table as an array (a full group's only grows)
         # how many layer calls have attention of which sizes
         self.sizes: dict = {}
         if runtime.dtype == torch.bfloat16 and self.group is not None:
@@ -56,25 +54,36 @@ class SharedPrefixSteps:
                 if sizes is not None and runner.storage.slot_group[call.cache] == self.group:
                     self.sizes[sizes] = self.sizes.get(sizes, 0) + 1
 
+    def _table(self, seq) -> np.ndarray:
+        pages, held = seq.tables[self.group], self._tables.get(seq)
+        known = 0 if held is None else len(held)
+        if known > len(pages):
+            known = 0                      # given back meanwhile
+        if held is None or known != len(pages):
+            new = np.array(pages[known:], dtype=np.int32)
+            held = self._tables[seq] = np.concatenate([held[:known], new]) if known else new
+        return held
+
     def plans(self, entries, replayed: bool):
         """{sizes: plan} for a step, or None; ``replayed``: the step would be a capture's replay otherwise."""
         if not self.sizes or len(entries) < 2 or max(len(e.tokens) for e in entries) > MEMBER_TOKENS:
             return None
-        tables = [e.seq.tables[self.group] for e in entries]
-        saved = shared_keys(tables, self.runner.page_tokens)
-        if not saved:
+        counts = np.array([len(e.tokens) for e in entries])
+        contexts = np.array([e.seq.length for e in entries]) + counts
+        per_key = sum(n * kv_heads * head_dim * 4 for (_, kv_heads, head_dim), n in self.sizes.items())
+        cost = PLAN_US + PLAN_REQUEST_US * len(entries) + (EAGER_LAYER_US * sum(self.sizes.values()) if replayed else 0.0)
+        page_tokens = self.runner.page_tokens
+        if not self.always and int(contexts.sum()) * per_key / BYTES_PER_US < cost:
+            return None                    # not if every key were shared
+        rows = [self._table(e.seq) for e in entries]
+        table = np.full((len(entries), max(map(len, rows))), -1, dtype=np.int32)
+        for at, row in zip(table, rows):
+            at[:len(row)] = row
+        saved = shared_keys(table, (contexts - counts + 1) // page_tokens, page_tokens)
+        if not saved or (not self.always and saved * per_key / BYTES_PER_US < cost):
             return None
-        if not self.always:
-            layers = sum(self.sizes.values())
-            won = saved * sum(n * kv_heads * head_dim * 4 for (_, kv_heads, head_dim), n in self.sizes.items()) / BYTES_PER_US
-            if won < PLAN_US + PLAN_REQUEST_US * len(entries) + (EAGER_LAYER_US * layers if replayed else 0.0):
-                return None
-        counts = [len(e.tokens) for e in entries]
-        table = np.full((len(entries), max(map(len, tables))), -1, dtype=np.int32)
-        for row, pages in zip(table, tables):
-            row[:len(pages)] = pages
         q_start = np.concatenate([[0], np.cumsum(counts)])
-        contexts = np.array([e.seq.length + n for e, n in zip(entries, counts)])
         self.steps += 1
-        return {sizes: kernels.shared_prefix_plan(table, q_start, contexts, self.runner.page_tokens, *sizes, torch.bfloat16, self.runner.runtime.device)
+        self.tables = {self.group: table}
+        return {sizes: kernels.shared_prefix_plan(table, q_start, contexts, page_tokens, *sizes, torch.bfloat16, self.runner.runtime.device)
                 for sizes in self.sizes}

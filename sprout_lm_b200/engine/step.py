@@ -170,7 +170,7 @@ class ModelRunner:
         self.validate(entries)
         shared = self.shared_prefix.plans(entries, replayed=False) if self.shared_prefix else None
         key, width = self.step_graphs.plan(entries, sample=False) if shared is None else (None, None)
-        ctx = self.stager.stage(entries, self.page_tokens, fixed_pages=width)
+        ctx = self.stager.stage(entries, self.page_tokens, fixed_pages=width, tables=shared and self.shared_prefix.tables)
         ctx.shared = shared
         if key is None:
             logits = self.forward(ctx)
@@ -218,7 +218,7 @@ class ModelRunner:
             return sampled
         floats = {"temperature": temperatures, "uniform": uniforms} if temperatures else None
         key, width = self.step_graphs.plan(entries, sample=bool(temperatures)) if shared is None else (None, None)
-        ctx = self.stager.stage(entries, self.page_tokens, fixed_pages=width, floats=floats)
+        ctx = self.stager.stage(entries, self.page_tokens, fixed_pages=width, floats=floats, tables=shared and self.shared_prefix.tables)
         ctx.shared = shared
         self.stats["h2d_bytes"] += self.stager.last_bytes
         if key is not None:
@@ -262,7 +262,7 @@ class ModelRunner:
         drafts = [t for e in entries for t in (*e.tokens[1:], 0)]
         floats = {"temperature": temperatures, "accept": accept, "draw": draw, "drafts": np.asarray(drafts, dtype=np.int32).view(np.float32)}
         shared = self.shared_prefix.plans(entries, replayed=False) if self.shared_prefix else None
-        ctx = self.stager.stage(entries, self.page_tokens, floats=floats)
+        ctx = self.stager.stage(entries, self.page_tokens, floats=floats, tables=shared and self.shared_prefix.tables)
         ctx.shared = shared
         self.stats["h2d_bytes"] += self.stager.last_bytes
         logits = self.forward(ctx)
