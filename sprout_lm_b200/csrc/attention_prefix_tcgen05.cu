@@ -4,12 +4,16 @@
 // A CTA owns an item of up to 256 rows, two Q tiles of 128, and walks its keys in tiles of 64:
 //
 //   S = Q K^T    tcgen05.mma, Q and K K-major in shared memory, S [128 x 64] in tensor memory, two buffers per Q tile
-//   softmax      a warpgroup per Q tile, one thread per row: S into registers, P = exp2(..) as bfloat16 back into tensor memory, over the
-//                first half of S's columns
+//   softmax      two warpgroups per Q tile, half a row a thread: S into registers, the halves' maxima through shared memory, P = exp2(..)
+//                as bfloat16 back into tensor memory, over the first half of S's columns
 //   O += P V     tcgen05.mma with P from tensor memory, V as it lies in the cache (MN-major); O stays in tensor memory
 //
 // as the prompt kernel of attention_maps_tcgen05.cu does, but every row sees every key, the rows are gathered from many requests, and O
-// leaves unnormalised with its maximum and sum.  A row's O and sum follow its maximum only once it has grown by 2^GROWTH.
+// leaves unnormalised with its maximum and sum.  A row's O and sum follow its maximum only once it has grown by 2^GROWTH.  What bounds
+// it: the chain S, maximum, exponentials, P, products of a tile, two tiles deep; the products alone are 1,000 cycles for 256 x 64 at head
+// size 128, the exponentials 1,024, a tile takes 1,700 to 1,900.  A warp for both tiles' products took 2,300 (its waits are 150 cycles
+// each, and 24 products 1,400 to issue); one warpgroup a Q tile is 3 % faster over 32,768 keys and 8 % slower over 2,000, where a CTA has
+// few tiles; a quarter of the exponentials as polynomials gained 5 % there and costs 5 % here.
 //
 // K and V come by TMA, one box per page, through a ring of stages.  Every mbarrier wait is bounded: on a timeout the CTA sets
 // the status word, waits (bounded) for its copies in flight, frees its tensor memory and returns.
@@ -23,7 +27,8 @@ using namespace sprout_prefix;
 namespace {
 
 constexpr int ROWS = 128, KEYS = 64;        // rows of a Q tile (tensor-memory lanes), keys of a tile
-constexpr int THREADS = 384;                // warpgroup 0: key copies, MMA, value copies, MMA; 1, 2: softmax of Q tile 0, 1
+constexpr int THREADS = 640;                // warpgroup 0: key copies, MMA, value copies, MMA; 1, 2: softmax of Q tile 0's columns' halves; 3, 4: of Q tile 1's
+constexpr int HALF = KEYS / 2;              // columns of S that a softmax thread has
 constexpr int ATOM = 128 * 128;             // bytes of a [128 rows, 64 bf16] swizzled tile
 constexpr int KV_ATOM = KEYS * 128;         // and of [KEYS rows, 64 bf16]
 constexpr int TMEM_COLS = 512;
@@ -33,37 +38,22 @@ constexpr int MARKS = 16;                   // tiles whose missing boxes are rem
 template <int DIM>
 struct Layout {
   static constexpr int Q_BYTES = DIM / 64 * ATOM, KV_BYTES = DIM / 64 * KV_ATOM;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = 4;
   static constexpr int OFF_K = 2 * Q_BYTES, OFF_V = OFF_K + STAGES * KV_BYTES, OFF_BAR = OFF_V + STAGES * KV_BYTES;
-  static constexpr int OFF_ROWS = OFF_BAR + 512, SMEM = OFF_ROWS + 2 * ROWS * 8;       // the query rows' addresses
+  static constexpr int OFF_ROWS = OFF_BAR + 512, OFF_MAX = OFF_ROWS + 2 * ROWS * 8;    // the query rows' addresses
+  static constexpr int SMEM = OFF_MAX + (2 * 2 * 2 + 2) * ROWS * 4;        // the halves' maxima (two tiles), the second halves' sums
   static constexpr int O_COLUMN = 4 * KEYS;                        // tensor memory: S of the Q tiles, two buffers each, then their O
   static_assert(O_COLUMN + 2 * DIM <= TMEM_COLS, "tensor memory columns");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
+// A barrier of some of the CTA's threads, and whether all of them say so.
+__device__ __forceinline__ bool named_barrier_and(int id, int threads, bool mine) {
+  uint32_t all;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.cta.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
+               : "=r"(all) : "r"(id), "r"(threads), "r"((uint32_t)mine) : "memory");
+  return all != 0;
 }
-// 2^x0 and 2^x1 for x <= 8 by packed products in place of the special function unit, to 4e-6 (the weights that they become have 2^-8): x = n + f
-// with |f| <= 1/2, 2^f by its Taylor polynomial, n into the exponent; results below 2^-126 are 2^-126.
-__device__ __forceinline__ void exp2_by_products(float x0, float x1, float& p0, float& p1) {
-  const uint64_t x = pair(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t t = add2(x, pair(12582912.f, 12582912.f));        // 1.5 * 2^23: the sum's low bits are x rounded to a whole number
-  const uint64_t f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
-  uint64_t r = fma2(f, pair(1.3333558e-3f, 1.3333558e-3f), pair(9.6181291e-3f, 9.6181291e-3f));
-  r = fma2(r, f, pair(5.5504109e-2f, 5.5504109e-2f));
-  r = fma2(r, f, pair(0.24022651f, 0.24022651f));
-  r = fma2(r, f, pair(0.69314718f, 0.69314718f));
-  r = fma2(r, f, pair(1.f, 1.f));
-  float r0, r1, t0, t1;
-  unpair(r, r0, r1);
-  unpair(t, t0, t1);
-  p0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
-  p1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
-}
-
 template <int DIM>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p, const int box_rows) {
@@ -79,7 +69,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   uint64_t* v_full = k_empty + NS;
   uint64_t* v_empty = v_full + NS;
   uint64_t* s_full = v_empty + NS;     // [2 Q tiles][2 buffers] S is complete in tensor memory
-  uint64_t* p_full = s_full + 4;       // [2][2] P is in tensor memory (4 warps arrive)
+  uint64_t* p_full = s_full + 4;       // [2][2] P is in tensor memory (8 warps arrive)
   uint64_t* o_done = p_full + 4;       // [2][2] P V of a Q tile's key tile is complete, for even and odd tiles (a waiter may be two behind)
   constexpr int BARS = 4 * NS + 12;
   uint32_t* tmem_slot = (uint32_t*)(bars + BARS);
@@ -114,7 +104,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   if (tid == THREADS - 1) {
     for (int i = 0; i < BARS; i++) {
       const bool writes_p = &bars[i] >= p_full && &bars[i] < o_done, empty = (&bars[i] >= k_empty && &bars[i] < v_full) || (&bars[i] >= v_empty && &bars[i] < s_full);
-      mbar_init(&bars[i], writes_p ? 4 : empty && two ? 2 : 1);
+      mbar_init(&bars[i], writes_p ? 8 : empty && two ? 2 : 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -144,7 +134,8 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   }
   const uint32_t tmem_base = *tmem_slot;
   if (warp < 4) {
-    warpgroup_regs_give<104>();
+    // the launch's 640 x 96 registers as 128 x 64 and 512 x 104
+    warpgroup_regs_give<64>();
     if (warp == 0 || warp == 2) {
       // ---------------- copies, keys by warp 0 and values by warp 2: one TMA box per page (or per KEYS keys of a larger page); lane b
       // issues box b's copies, lane 0 waits for the stage and posts the bytes.  The page of a tile is looked up while the tile before
@@ -251,15 +242,18 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       if (!ok && lane == 0) gave_up();
     }
   } else {
-    // ---------------- softmax: a warpgroup per Q tile, one thread per row
-    warpgroup_regs_take<200>();
-    const int q = (warp >> 2) - 1, quarter = warp & 3, row = quarter * 32 + lane;       // a warp reads tensor-memory lanes 32 * (warp % 4) on
+    // ---------------- softmax: two warpgroups per Q tile, half a row a thread
+    warpgroup_regs_take<104>();
+    const int q = ((warp >> 2) - 1) >> 1, half = ((warp >> 2) - 1) & 1, quarter = warp & 3, row = quarter * 32 + lane;       // a warp reads tensor-memory lanes 32 * (warp % 4) on
     const int i = q * ROWS + row;                      // of the item
     const int my_tiles = q == 0 || two ? n_tiles : 0;
     const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t o_addr = lane_addr + L::O_COLUMN + q * DIM;
     const float scale_log2 = p.scale_log2;
     const uint64_t scale2 = pair(scale_log2, scale_log2);
+    float* maxima = (float*)(smem + L::OFF_MAX) + q * 2 * ROWS + row;        // [2 tiles][2 Q tiles][2 halves][128]
+    float* second = (float*)(smem + L::OFF_MAX) + 8 * ROWS + q * ROWS + row; // [2 Q tiles][128]
+    const int meet = 2 + q * 4 + quarter;              // the barrier of the two warps that share 32 rows
     float m = -INFINITY;                               // the maximum that the sums stand for (unscaled scores)
     uint64_t l2 = 0ull;                                // the sum, as two partial sums
     bool ok = true;
@@ -267,32 +261,28 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       const uint32_t s_addr = lane_addr + (q * 2 + (j & 1)) * KEYS;
       ok = !*abort_flag && mbar_wait(&s_full[q * 2 + (j & 1)], (j >> 1) & 1, abort_flag);
       if (!ok) gave_up();
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      ok = __all_sync(0xffffffffu, ok);                // one that gave up goes on to where it meets the other half
       tc_fence_after();
-      uint32_t sc[KEYS / 32][32];
-#pragma unroll
-      for (int c = 0; c < KEYS / 32; c++) tmem_load32_issue(s_addr + c * 32, sc[c]);
-#pragma unroll
-      for (int c = 0; c < KEYS / 32; c++) tmem_load_wait(sc[c]);
-      const int there = item.key_end - item.key_begin - j * KEYS;        // keys of the tile before the range's end
+      uint32_t sc[HALF];
+      tmem_load32_issue(s_addr + half * HALF, sc);
+      tmem_load_wait(sc);
+      const int there = item.key_end - item.key_begin - j * KEYS - half * HALF;        // of this half's keys before the range's end
       const uint32_t marks = missing[j % MARKS];
-      if (there < KEYS || marks != 0) {
+      if (there < HALF || marks != 0) {
 #pragma unroll
-        for (int c = 0; c < KEYS / 32; c++)
-#pragma unroll
-          for (int k = 0; k < 32; k++)
-            if (c * 32 + k >= there || (marks >> ((c * 32 + k) / box_rows) & 1)) sc[c][k] = 0xff800000u;          // -inf
+        for (int k = 0; k < HALF; k++) if (k >= there || (marks >> ((half * HALF + k) / box_rows) & 1)) sc[k] = 0xff800000u;          // -inf
       }
-      // the maximum, NaN if there is one (the exponentials by products would lose it)
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < KEYS / 32; c++)
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) mx[(k >> 1) & 3] = max3_nan(mx[(k >> 1) & 3], __uint_as_float(sc[c][k]), __uint_as_float(sc[c][k + 1]));
-      const float n = max3_nan(max3_nan(m, mx[0], mx[1]), mx[2], mx[3]);
+      for (int k = 0; k < HALF; k += 2) mx[(k >> 1) & 3] = max3(mx[(k >> 1) & 3], __uint_as_float(sc[k]), __uint_as_float(sc[k + 1]));
+      float n = max3(max3(m, mx[0], mx[1]), mx[2], mx[3]);
+      float* at = maxima + (j & 1) * 4 * ROWS;
+      at[half * ROWS] = n;
+      ok = named_barrier_and(meet, 64, ok);            // both halves are in registers: P may go over S
+      if (!ok) break;
+      n = max3(n, at[(half ^ 1) * ROWS], n);
       // it moved: bring O and the sum to it (by less than 2^GROWTH: they stay, and weights are up to that large)
-      const bool moved = m == -INFINITY ? n != m : !((n - m) * scale_log2 <= GROWTH);
+      const bool moved = m == -INFINITY ? n != m : (n - m) * scale_log2 > GROWTH;
       if (__any_sync(0xffffffffu, moved)) {
         const float alpha = !moved ? 1.0f : m == -INFINITY ? 0.f : exp2_fast((m - n) * scale_log2);
         if (moved) m = n;
@@ -300,12 +290,11 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
         unpair(l2, lo2, hi2);
         l2 = pair(lo2 * alpha, hi2 * alpha);
         if (j > 0) {
-          ok = !*abort_flag && mbar_wait(&o_done[q * 2 + ((j - 1) & 1)], ((j - 1) >> 1) & 1, abort_flag);
-          if (!ok) gave_up();
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          // a timeout here shows in the status word and the abort flag; the halves go on in step, to the next wait for S
+          if (*abort_flag || !mbar_wait(&o_done[q * 2 + ((j - 1) & 1)], ((j - 1) >> 1) & 1, abort_flag)) gave_up();
+          __syncwarp();
           tc_fence_after();
-          for (int c = 0; c < DIM; c += 16) {
+          for (int c = half * (DIM / 2); c < (half + 1) * (DIM / 2); c += 16) {
             uint32_t o[16];
             tmem_load16(o_addr + c, o);
 #pragma unroll
@@ -318,22 +307,17 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       const uint64_t nbase2 = pair(-base, -base);
       // probabilities, their sum, and P as bfloat16 into tensor memory
       uint64_t sums[2] = {0ull, 0ull};
+      uint32_t packed[HALF / 2];
 #pragma unroll
-      for (int c = 0; c < KEYS / 32; c++) {
-        uint32_t packed[16];
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float x0, x1;
-          unpair(fma2(pair(sc[c][k], sc[c][k + 1]), scale2, nbase2), x0, x1);
-          float p0, p1;
-          if ((k & 6) == 6) exp2_by_products(x0, x1, p0, p1);
-          else { p0 = exp2_fast(x0); p1 = exp2_fast(x1); }
-          __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-          packed[k >> 1] = *(uint32_t*)&h;
-          sums[(k >> 1) & 1] = add2(sums[(k >> 1) & 1], pair(p0, p1));
-        }
-        tmem_store16(s_addr + c * 16, packed);
+      for (int k = 0; k < HALF; k += 2) {
+        float x0, x1;
+        unpair(fma2(pair(sc[k], sc[k + 1]), scale2, nbase2), x0, x1);
+        const float p0 = exp2_fast(x0), p1 = exp2_fast(x1);
+        __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+        packed[k >> 1] = *(uint32_t*)&h;
+        sums[(k >> 1) & 1] = add2(sums[(k >> 1) & 1], pair(p0, p1));
       }
+      tmem_store16(s_addr + half * (HALF / 2), packed);
       l2 = add2(l2, add2(sums[0], sums[1]));
       tmem_store_wait();
       tc_fence_before();
@@ -346,33 +330,37 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
-    if (ok && my_tiles > 0) {
-      // O leaves by way of the Q tile's room, which no product reads any more: a warp's 32 rows, 64 columns at a time, so that its
-      // stores are rows of 256 bytes
+    if (my_tiles > 0) {
+      // O leaves by way of the Q tile's room, which no product reads any more: a warp's 32 rows, COLUMNS columns at a time, so that its
+      // stores are whole lines
+      constexpr int COLUMNS = DIM / 4, CHUNKS16 = COLUMNS / 4, AT_ONCE = 32 / CHUNKS16;        // 16-byte chunks of a row, rows a store
       float l_lo, l_hi;
       unpair(l2, l_lo, l_hi);
+      if (half == 1) *second = l_lo + l_hi;
+      ok = named_barrier_and(meet, 64, ok);            // both halves have their outputs, or both leave
       size_t slot = 0;
-      const bool mine = i < item.rows;
+      const bool mine = ok && i < item.rows;
       if (mine) {
         slot = (size_t)(p.part_start[place_of_row(item, i, group)] + item.part) * p.heads + head_of_row(item, i, group, g);
-        p.part_sum[slot] = make_float2(m == -INFINITY ? -INFINITY : m * scale_log2, l_lo + l_hi);
+        if (half == 0) p.part_sum[slot] = make_float2(m == -INFINITY ? -INFINITY : m * scale_log2, l_lo + l_hi + *second);
       }
       const unsigned long long to = mine ? (unsigned long long)(p.part_out + slot * DIM) : 0ull;
-      float* dst[8];                                   // of the rows whose 16-byte chunk lane % 8 this lane stores
+      float* dst[CHUNKS16];                            // of the rows that this lane stores a chunk of
 #pragma unroll
-      for (int k = 0; k < 8; k++) dst[k] = (float*)__shfl_sync(0xffffffffu, to, k * 4 + (lane >> 3));
-      float* room = (float*)(sQ + q * L::Q_BYTES) + quarter * (32 * 32);       // 4 KB: 32 rows of 32 columns, 16-byte chunk c of row r at c ^ (r & 7)
-      for (int c = 0; c < DIM; c += 32) {
-        uint32_t o[32];
-        tmem_load32(o_addr + c, o);
+      for (int k = 0; k < CHUNKS16; k++) dst[k] = (float*)__shfl_sync(0xffffffffu, to, k * AT_ONCE + lane / CHUNKS16);
+      float* room = (float*)(sQ + q * L::Q_BYTES) + (half * 4 + quarter) * (32 * COLUMNS);       // chunk c of row r at c ^ (r & (CHUNKS16 - 1))
+      for (int c = half * (DIM / 2); c < (half + 1) * (DIM / 2); c += COLUMNS) {
+        uint32_t o[COLUMNS];
+        if constexpr (COLUMNS == 32) tmem_load32(o_addr + c, o);
+        else tmem_load16(o_addr + c, o);
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 8; k++) *(uint4*)(room + lane * 32 + ((k ^ (lane & 7)) << 2)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        for (int k = 0; k < CHUNKS16; k++) *(uint4*)(room + lane * COLUMNS + ((k ^ (lane & (CHUNKS16 - 1))) << 2)) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         __syncwarp();
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int r = k * 4 + (lane >> 3), chunk = lane & 7;
-          if (dst[k] != nullptr) *(uint4*)(dst[k] + c + chunk * 4) = *(const uint4*)(room + r * 32 + ((chunk ^ (r & 7)) << 2));
+        for (int k = 0; k < CHUNKS16; k++) {
+          const int r = k * AT_ONCE + lane / CHUNKS16, chunk = lane % CHUNKS16;
+          if (dst[k] != nullptr) *(uint4*)(dst[k] + c + chunk * 4) = *(const uint4*)(room + r * COLUMNS + ((chunk ^ (r & (CHUNKS16 - 1))) << 2));
         }
       }
     }

@@ -18,7 +18,7 @@ from ..prefix_plan import MEMBER_TOKENS
 
 BYTES_PER_US = 6.4e6               # what attention streams keys and values at
 # A plan, for each request of it, and a layer's launches one by one beside a replay of them (measured: 64 requests of the 0.5B shape over
-# 4,096 shared keys take 1.55 ms a step as a replay and 4.3 with a plan; over 32,768, 4.3 and 4.5; its 24 layers' attention alone 0.6 and 0.5, 4.0 and 0.9)
+# 4,096 shared keys take 1.55 ms a step as a replay and 4.3 with a plan; over 32,768, 4.3 and 4.5)
 PLAN_US, PLAN_REQUEST_US, EAGER_LAYER_US = 600.0, 10.0, 130.0
 
 
