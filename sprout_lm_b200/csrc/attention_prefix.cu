@@ -397,10 +397,9 @@ attention_prefix_mma_kernel(const Params p) {
 // WARPS warps per (token, head), each of them every WARPS-th part, a lane two columns in every 64; the first warp also adds the keys of the
 // member's own tokens that the items leave out, a lane a key.  One warp for a row of few parts; a row of 35 parts in one warp is a chain
 // of five waits for memory.
-#ifndef PREFIX_MERGE_FROM
-#define PREFIX_MERGE_FROM 24
-#endif
-constexpr int MERGE_THREADS = 128, MERGE_SPLIT = 4, MERGE_FROM = PREFIX_MERGE_FROM;      // MERGE_FROM: parts a row, on average
+// MERGE_FROM: parts a row, on average.  35 parts (64 tokens of 14 heads of 64): 20.5 us a call with four warps, 21.5 with one; 14 parts (135
+// tokens): 27.4 and 24.4; 10 parts (90 tokens of 28 heads of 128): 33.2 and 29.7.
+constexpr int MERGE_THREADS = 128, MERGE_SPLIT = 4, MERGE_FROM = 24;
 
 template <typename T, int PAIRS, int WARPS>
 __global__ void __launch_bounds__(MERGE_THREADS)
@@ -581,6 +580,7 @@ SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const 
                  "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
   SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (narrow_items == 0 || narrow_ctas > 0) && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
+  SPROUT_REQUIRE(((uintptr_t)part_out & 15) == 0 && ((uintptr_t)part_sum & 7) == 0, "attention_shared_prefix: the partial results must start on 16- and 8-byte boundaries");
   Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, (const Item*)items, order, part_start, seen, extra, table_of, part_out, (float2*)part_sum, out, out_stride,
            tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, 1};
   if (simple_items > 0) {

@@ -31,15 +31,11 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int PER_THREAD = 16, RUN = THREADS * PER_THREAD;       // logits of a run
-#ifndef VERIFY_ROWS
-#define VERIFY_ROWS 2
-#define VERIFY_ITEMS 8
-#define VERIFY_PIECE 1024
-#endif
-constexpr int ROW_BLOCKS = VERIFY_ROWS;    // of the first kernel, an SM
-constexpr int MAX_ITEMS = VERIFY_ITEMS;    // pieces that one of its warps takes
-constexpr int PIECE = VERIFY_PIECE;        // logits of a piece
+// The first kernel: blocks an SM, pieces that a warp takes at most, logits of a piece.  616 rows of 152,064 (a third of the drafts' greedy and
+// not read, 320 MB): 71 us; 3 blocks an SM 76, 16 pieces a warp 79, pieces of 512 logits in 4 blocks 71 but 10 % more in what merges them.
+constexpr int ROW_BLOCKS = 2, MAX_ITEMS = 8, PIECE = 1024;
 constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_LOGITS = RUN / DRAW_THREADS;
+constexpr int MAX_HELD = 256;              // runs whose sums the last kernel keeps in shared memory
 
 struct PieceSum { double sum; float max; int index; int bad; int pad; };     // sum: of 2^((v - max) log2(e) / T)
 
@@ -109,7 +105,7 @@ struct Chosen {
 
 // 64-bit sums of a run of the row that is drawn from: the exponentials of the target's and the draft's logits, and both again over the
 // tokens where the difference is positive.
-struct Sums { double a, b, above_a, above_b; };
+struct __align__(16) Sums { double a, b, above_a, above_b; };
 
 struct Args {
   const float* logits; const float* draft_logits;      // [rows, vocab], [draft_rows, vocab]
@@ -232,20 +228,35 @@ verify_rows_kernel(const Args p) {
 // What a row's pieces add up to: its maximum, first index and (with `sums`) sum relative to the maximum, in every lane of the warp.
 struct RowSum { double sum; float max; int index; int bad; };
 __device__ __forceinline__ RowSum merge_pieces(const PieceSum* pieces, int count, bool sums, double c) {
+  constexpr int HELD = 8;                              // of a lane, all on their way at a time
   const int lane = threadIdx.x & 31;
-  float best = -INFINITY;
-  int best_i = 0x7fffffff, bad = 0;
-  for (int i = lane; i < count; i += 32) {
-    better(best, best_i, pieces[i].max, pieces[i].index);
-    bad |= pieces[i].bad;
-  }
+  RowSum row{0.0, -INFINITY, 0x7fffffff, 0};
+  for (int base = 0; base < count; base += 32 * HELD) {
+    PieceSum held[HELD];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) better(best, best_i, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, best_i, o));
-  bad = __any_sync(0xffffffffu, bad);
-  double sum = 0.0;
-  if (sums && !bad)
-    for (int i = lane; i < count; i += 32) sum += pieces[i].sum * pow2(((double)pieces[i].max - (double)best) * c);
-  return RowSum{warp_sum_d(sum), best, best_i, bad};
+    for (int k = 0; k < HELD; k++) {
+      const int i = base + k * 32 + lane;
+      held[k] = i < count ? pieces[i] : PieceSum{0.0, -INFINITY, 0x7fffffff, 0, 0};
+    }
+    float best = row.max;
+    int index = row.index, bad = row.bad;
+#pragma unroll
+    for (int k = 0; k < HELD; k++) {
+      better(best, index, held[k].max, held[k].index);
+      bad |= held[k].bad;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) better(best, index, __shfl_xor_sync(0xffffffffu, best, o), __shfl_xor_sync(0xffffffffu, index, o));
+    double sum = 0.0;
+    if (sums) {
+#pragma unroll
+      for (int k = 0; k < HELD; k++) if (held[k].sum > 0.0) sum += held[k].sum * pow2(((double)held[k].max - (double)best) * c);
+      sum = warp_sum_d(sum);
+      if (row.sum > 0.0) sum += row.sum * pow2(((double)row.max - (double)best) * c);
+    }
+    row = RowSum{sum, best, index, __any_sync(0xffffffffu, bad)};
+  }
+  return row;
 }
 
 __global__ void __launch_bounds__(THREADS)
@@ -367,12 +378,18 @@ __global__ void __launch_bounds__(DRAW_THREADS)
 verify_draw_kernel(const Args p) {
   __shared__ double s_sum[DRAW_WARPS], s_before, s_target, s_rho;
   __shared__ int s_run, s_from_p, s_first, s_last;
+  __shared__ Sums s_sums[MAX_HELD];
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Chosen at = p.chosen[r];
   if (at.row < 0) return;
   const Sums* sums = p.sums + (size_t)r * p.runs;
+  if (p.runs <= MAX_HELD) {                            // gone through three times
+    for (int i = tid; i < p.runs * 2; i += DRAW_THREADS) ((double2*)s_sums)[i] = ((const double2*)sums)[i];
+    __syncthreads();
+    sums = s_sums;
+  }
   if (warp == 0) {
     // the run in which the draw falls, a lane a run
     double rho = 1.0, total = 0.0;
@@ -476,6 +493,8 @@ int runs_of(int vocab) { return (vocab + RUN - 1) / RUN; }
 long long aligned16(long long bytes) { return (bytes + 15) & ~15LL; }
 }  // namespace
 
+static_assert(sizeof(Sums) == 32 && alignof(Sums) == 16 && sizeof(Chosen) % 8 == 0 && sizeof(PieceSum) % 8 == 0, "the scratch's parts start on their boundaries");
+
 // Bytes of scratch, 16-byte aligned, for `rows` rows (target's and draft's together) of `vocab` logits.
 SPROUT_API long long sprout_verify_scratch_bytes(int rows, int requests, int vocab) {
   return aligned16(rows * (long long)pieces_of(vocab) * (long long)sizeof(PieceSum)) + aligned16(requests * (long long)sizeof(Chosen)) +
@@ -491,6 +510,7 @@ SPROUT_API int sprout_verify(const float* logits, long long ld, const float* dra
   SPROUT_REQUIRE(rows > 0 && requests > 0 && requests <= rows && vocab > 0 && vocab <= 1 << 30 && ld >= 0, "verify: bad sizes rows=%d requests=%d vocab=%d ld=%lld", rows, requests, vocab, ld);
   SPROUT_REQUIRE(draft_rows == 0 || (draft_rows == rows - requests && draft_logits && draft_ld >= 0), "verify: a draft row per drafted token");
   SPROUT_REQUIRE(logits && drafts && row_start && out && accepted && scratch && status, "verify: null pointer");
+  SPROUT_REQUIRE(((uintptr_t)scratch & 15) == 0, "verify: scratch must start on a 16-byte boundary");
   SPROUT_REQUIRE((temperature == nullptr) == (accept == nullptr) && (accept == nullptr) == (draw == nullptr), "verify: temperatures and both kinds of uniform numbers go together");
   const long long per_row = pieces_of(vocab), runs = runs_of(vocab), all = per_row * (rows + (long long)draft_rows);
   SPROUT_REQUIRE(rows + (long long)draft_rows <= 0x7fffffffLL && runs * requests <= 0x7fffffffLL, "verify: too many rows");
