@@ -256,6 +256,61 @@ def test_captured_and_on_another_stream(status):
     assert torch.equal(again, eager[-1]) and int(status.item()) == 0
 
 
+def test_launches_one_behind_the_other(status):
+    """Without programmatic dependent launch the items' launches follow one another; the results are the same bits."""
+    from sprout_lm_b200 import kernels
+    step = Step(28, 4, 128, BF16, 16, [0] * 30, [600], list(range(0, 600, 20)), [1, 2, 3] * 10, seed=14)
+    plan = step.plan()
+    assert plan.host.matrix_items > 0 and plan.host.narrow_items > 0
+    want = step.run(status, plan=plan)
+    try:
+        kernels.set_pdl(False)
+        assert torch.equal(step.run(status, plan=plan), want)
+    finally:
+        kernels.set_pdl(True)
+    step.check(status)
+
+
+def test_two_calls_at_once(status):
+    """Calls of one plan on two streams, each with scratch of its own, while a third runs on the current one."""
+    step = Step(28, 4, 128, BF16, 16, [0] * 20, [300], list(range(0, 400, 20)), [1] * 20, seed=16)
+    plan = step.plan()
+    want = step.run(status, plan=plan)
+    torch.cuda.synchronize()
+    outs = []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                outs.append(step.run(status, plan=plan))
+        outs.append(step.run(status, plan=plan))
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs) and int(status.item()) == 0
+
+
+@pytest.mark.parametrize("shape", [(128, 1, 64), (64, 1, 128), (17, 1, 16)])
+def test_many_query_heads_a_key_value_head(shape, status):
+    """More query rows a token than an item of few rows holds."""
+    Step(*shape, BF16, 16, [0] * 5, [30], [5, 70, 0, 33, 200], [1, 3, 1, 2, 1], seed=17).check(status)
+
+
+def test_every_kind_of_item(status):
+    """Each kind alone and all of them in one call, whatever the plan's model would pick."""
+    import sprout_lm_b200.prefix_plan as prefix_plan
+    step = Step(14, 2, 64, BF16, 16, [0] * 20, [100], [7 * i for i in range(20)], [1 + i % 6 for i in range(20)], seed=18)
+    want, tol = step.exact()
+    pick, seen = prefix_plan.choose_kinds, set()
+    try:
+        for ways in ((1, 1), (2, 2), (0, 1), (0, 2)):
+            prefix_plan.choose_kinds = lambda rows, steps, whole, *rest, ways=ways: np.where(rows <= 16, 1, np.where(whole, *ways))
+            plan = step.plan()
+            seen.add((plan.host.matrix_items > 0, plan.host.narrow_items > 0, plan.host.wide_items > 0))
+            assert bool(((step.run(status, plan=plan).double() - want).abs() <= tol).all())
+    finally:
+        prefix_plan.choose_kinds = pick
+    assert seen == {(False, True, False), (False, True, True), (True, True, False), (True, True, True)}
+
+
 def test_refusals(status):
     from sprout_lm_b200 import kernels
     step = Step(14, 2, 64, BF16, 16, [0] * 3, [10], [5, 9, 0], [1, 2, 1], seed=13)
