@@ -23,6 +23,7 @@ MAX_RANGES = 64             # of a segment
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
 # the members read it themselves.
 MIN_SAVED_KEYS = 64
+PART_KEYS = 2               # and more than its rows' partial results cost: float32 written and read, the bytes of two bfloat16 keys and values a row
 
 
 class PlanError(ValueError):
@@ -39,10 +40,10 @@ class Segment:
         self.part, self.ranges = 0, 1
 
 
-def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray, page_tokens: int):
+def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray, page_tokens: int, group: int = 1):
     """(segments, order, seen, extra, table_of): the trie's segments, parents before their children; per place of the plan's order the
     step's token there, the keys that its member's tokens all see, the further ones that it sees itself, and its request.  The
-    parent of a segment is in ``parents`` of the result (-1: none)."""
+    parent of a segment is in ``parents`` of the result (-1: none).  ``group``: query heads of a key/value head."""
     counts = np.diff(q_start)
     # members: request, first token, tokens, keys that all of them see
     blocks = -(-counts // MEMBER_TOKENS)
@@ -51,44 +52,42 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
     tokens = np.minimum(MEMBER_TOKENS, counts[request] - offset)
     first = q_start[request] + offset
     sees = contexts[request] - counts[request] + offset + 1
-    whole = sees // page_tokens                          # full pages among them: what may be shared
+    whole = np.minimum(sees, contexts[request] - counts[request]) // page_tokens       # full pages of earlier steps: what may be shared
     segments, parents, leaves = [], [], []               # leaves: members in the plan's order
     placed = 0
-
-    def own(member, start, parent):
-        nonlocal placed
-        if int(sees[member]) > start * page_tokens:      # else all it sees lies in shared runs
-            segments.append(Segment(int(request[member]), int(start) * page_tokens, int(sees[member]), placed, placed + int(tokens[member])))
-            parents.append(parent)
-        leaves.append(member)
-        placed += int(tokens[member])
-
-    def walk(members, start, depth, parent):
-        # all of `members` (two or more) hold the same pages up to `depth`; those from `start` on are in no segment yet
-        rows = tables[request[members], depth:int(whole[members].min())]
-        same = (rows == rows[0]).all(axis=0)
-        end = depth + (int(same.argmin()) if not same.all() else rows.shape[1])
-        mine = None
-        if (len(members) - 1) * (end - start) * page_tokens >= MIN_SAVED_KEYS:
-            mine = Segment(int(request[members[0]]), start * page_tokens, end * page_tokens, placed)
-            segments.append(mine)
-            parents.append(parent)
-            parent, start = len(segments) - 1, end
-        branch(members, start, end, parent)
-        if mine is not None:
-            mine.token_end = placed
+    # Work that is left, the next last: members that hold the same pages up to ``depth``, of which those from ``start`` on are in no
+    # segment yet; or a segment whose members are all placed.
+    left = []
 
     def branch(members, start, depth, parent):
         groups = {}
         for member in members:
             groups.setdefault(int(tables[request[member], depth]) if whole[member] > depth else -1 - int(member), []).append(member)
-        for group in groups.values():
-            if len(group) > 1:
-                walk(np.asarray(group), start, depth, parent)
-            else:
-                own(group[0], start, parent)
+        left.extend((group, start, depth, parent) for group in reversed(groups.values()))
 
     branch(np.arange(len(request)), 0, 0, -1)
+    while left:
+        members, start, depth, parent = left.pop()
+        if members is None:
+            segments[parent].token_end = placed
+        elif len(members) == 1:
+            member = members[0]
+            if int(sees[member]) > start * page_tokens:      # else all it sees lies in shared runs
+                segments.append(Segment(int(request[member]), int(start) * page_tokens, int(sees[member]), placed, placed + int(tokens[member])))
+                parents.append(parent)
+            leaves.append(member)
+            placed += int(tokens[member])
+        else:
+            members = np.asarray(members)
+            rows = tables[request[members], depth:int(whole[members].min())]
+            same = (rows == rows[0]).all(axis=0)
+            end = depth + (int(same.argmin()) if not same.all() else rows.shape[1])
+            if (len(members) - 1) * (end - start) * page_tokens >= max(MIN_SAVED_KEYS, PART_KEYS * group * int(tokens[members].sum())):
+                segments.append(Segment(int(request[members[0]]), start * page_tokens, end * page_tokens, placed))
+                parents.append(parent)
+                parent, start = len(segments) - 1, end
+                left.append((None, 0, 0, parent))
+            branch(members, start, end, parent)
     leaves = np.asarray(leaves)
     lengths = tokens[leaves]
     within = np.arange(placed) - np.repeat(np.cumsum(lengths) - lengths, lengths)
@@ -214,7 +213,7 @@ class HostPlan:
         self.tokens, self.requests = int(q_start[-1]), len(contexts)
         self.pages = int(-(-contexts.max() // page_tokens))
         group = heads // kv_heads
-        segments, parents, order, seen, extra, table_of = find_segments(tables, q_start, contexts, page_tokens)
+        segments, parents, order, seen, extra, table_of = find_segments(tables, q_start, contexts, page_tokens, group)
         begin = np.array([s.key_begin for s in segments])
         end = np.array([s.key_end for s in segments])
         token_begin = np.array([s.token_begin for s in segments])

@@ -102,6 +102,34 @@ def test_no_range_is_much_longer_than_an_even_share(matrix_slots):
     assert int(lengths.max()) * (matrix_slots or 444) <= 1.3 * int(lengths.sum()) * 4
 
 
+@pytest.mark.parametrize("tokens, context", [(20000, 20000), (5000, 30000)])
+def test_a_long_prompt_among_the_requests(tokens, context):
+    """A request's pages of the step itself are read by its members, each with one result: no chain of a segment a page."""
+    page, cached = 16, context - tokens
+    tables = np.arange(3 * (context // page), dtype=np.int32).reshape(3, -1)
+    tables[:, :cached // page] = tables[0, :cached // page]
+    plan = HostPlan(tables, [0, tokens, tokens + 1, tokens + 2], [context, cached + 1, cached + 1], page, 28, 4, True, 592, 148, 296, 128)
+    assert plan.tokens == tokens + 2 and len(plan.segments) <= -(-tokens // MEMBER_TOKENS) + 3
+    assert plan.parts <= 12 * plan.tokens        # a segment of the cached pages in ranges, and the member's own
+
+
+@pytest.mark.parametrize("group", [1, 7])
+def test_many_requests_that_leave_a_document_page_by_page(group):
+    """Request i holds i pages of a document: as many branches one inside the other."""
+    page, requests = 16, 1300
+    tables = np.full((requests, requests + 1), -1, dtype=np.int32)
+    for i in range(requests):
+        tables[i, :i] = np.arange(i)
+        tables[i, i] = 10000 + i
+    contexts = np.arange(requests) * page + 3
+    plan = HostPlan(tables, np.arange(requests + 1), contexts, page, group, 1, True, 592, 148, 296, 128)
+    keys = np.zeros(plan.tokens * group, dtype=np.int64)
+    for table, begin, end, token_begin, row_begin, rows, _, _ in plan.items.tolist():
+        keys[token_begin * group + row_begin:][:rows] += end - begin
+        assert (tables[table, begin // page:-(-end // page)] >= 0).all()
+    assert (keys.reshape(-1, group) == contexts[plan.table_of][:, None]).all()
+
+
 def test_one_token_of_context():
     plan = HostPlan([[3]], [0, 1], [1], 16, 4, 2, True, 592)
     assert plan.items[:, :7].tolist() == [[0, 0, 1, 0, 0, 2, 0]] and plan.parts == 1
