@@ -567,21 +567,29 @@ extern "C" int sprout_attention_prefix_tc_supported(int head_dim, int page_token
 // Whether bfloat16 items of this head size run on the tensor cores.
 SPROUT_API int sprout_attention_prefix_mma_supported(int head_dim) { return head_dim % 16 == 0 && head_dim > 0 && head_dim <= 128; }
 
-// items: `simple_items` for the CUDA cores, or `matrix_items` of up to 256 rows, `narrow_items` of up to 16 (walked by `narrow_ctas` CTAs
-// where they stream) and `wide_items` of up to 64.  `parts`: the
-// partial results in all; part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
-SPROUT_API int sprout_attention_prefix(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
-                                       const int* positions, const int* items, int simple_items, int matrix_items, int narrow_items, int narrow_ctas, int wide_items, const int* order,
-                                       const int* part_start, const int* seen, const int* extra, const int* table_of, float* part_out, float* part_sum, void* out, long long out_stride, int dtype, int tokens, int parts,
-                                       int heads, int kv_heads, int head_dim, int page_tokens, int num_pages, int* status, cudaStream_t stream) {
-  SPROUT_REQUIRE(q && k_cache && v_cache && block_table && positions && items && order && part_start && seen && extra && table_of && part_out && part_sum && out && status,
-                 "attention_shared_prefix: null pointer");
+// What a plan is to its calls (kernels.py: _PrefixPlan): its arrays on the device; `simple_items` for the CUDA cores, or `matrix_items` of up
+// to 256 rows, `narrow_items` of up to 16 (walked by `narrow_ctas` CTAs where they stream) and `wide_items` of up to 64; the partial results
+// in all; and the sizes.
+struct PrefixPlan {
+  const Item* items;
+  const int* order; const int* part_start; const int* seen; const int* extra; const int* table_of;
+  int simple_items, matrix_items, narrow_items, narrow_ctas, wide_items, dtype, tokens, parts, heads, kv_heads, head_dim, page_tokens;
+};
+static_assert(sizeof(PrefixPlan) == 6 * 8 + 12 * 4, "as ctypes lays it out");
+
+// part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
+SPROUT_API int sprout_attention_prefix(const PrefixPlan* plan, const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
+                                       const int* positions, float* part_out, float* part_sum, void* out, long long out_stride, int num_pages, int* status, cudaStream_t stream) {
+  SPROUT_REQUIRE(plan && q && k_cache && v_cache && block_table && positions && plan->items && plan->order && plan->part_start && plan->seen && plan->extra && plan->table_of && part_out &&
+                 part_sum && out && status, "attention_shared_prefix: null pointer");
+  const int simple_items = plan->simple_items, matrix_items = plan->matrix_items, narrow_items = plan->narrow_items, narrow_ctas = plan->narrow_ctas, wide_items = plan->wide_items;
+  const int dtype = plan->dtype, tokens = plan->tokens, parts = plan->parts, heads = plan->heads, kv_heads = plan->kv_heads, head_dim = plan->head_dim, page_tokens = plan->page_tokens;
   SPROUT_REQUIRE(tokens > 0 && parts > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
                  "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
   SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (narrow_items == 0 || narrow_ctas > 0) && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
   SPROUT_REQUIRE(((uintptr_t)part_out & 15) == 0 && ((uintptr_t)part_sum & 7) == 0, "attention_shared_prefix: the partial results must start on 16- and 8-byte boundaries");
-  Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, (const Item*)items, order, part_start, seen, extra, table_of, part_out, (float2*)part_sum, out, out_stride,
+  Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, plan->items, plan->order, plan->part_start, plan->seen, plan->extra, plan->table_of, part_out, (float2*)part_sum, out, out_stride,
            tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, 1};
   if (simple_items > 0) {
     // rows that are whole fours on their boundaries

@@ -17,9 +17,10 @@
 // logits (some 15 64-bit operations, two cycles each), 1.09 T a second, while memory delivers 1.6 T logits a second: only the row that is
 // drawn from takes them.  Whether a draft stands is decided by float32 exponentials, whose sums are good to 1e-8.
 //
-// Four launches.  verify_rows_kernel: every row in pieces of PIECE logits, a warp each, their maxima and sums of exponentials (greedy:
-// the maximum's first index).  verify_decide_kernel: a block per request merges its rows' pieces, a warp a row, and finds the first row that does not stand.  verify_sums_kernel: the 64-bit sums of that row's
-// runs, a block each.  verify_draw_kernel: a block per request finds the run in which the draw falls and looks through it.
+// Three launches.  verify_rows_kernel: every row in pieces of PIECE logits, a warp each, their maxima and sums of exponentials (greedy:
+// the maximum's first index).  verify_decide_kernel: a block per request merges its rows' pieces, a warp a row, and finds the first row
+// that does not stand.  verify_sums_kernel: the 64-bit sums of that row's runs, a block each; where there are few, the request's last
+// block to be done also finds the run in which the draw falls and looks through it, else a fourth launch does.
 //
 // The difference in one pass: max(p - q, 0) needs both rows' sums before a single element of it is known.  With a_j, b_j the
 // exponentials and Za, Zb their sums, (p_j - q_j) Zb = a_j rho - b_j, rho = Zb / Za.  The float32 sums give rho to 1e-8, and so the set
@@ -34,8 +35,8 @@ constexpr int PER_THREAD = 16, RUN = THREADS * PER_THREAD;       // logits of a 
 // The first kernel: blocks an SM, pieces that a warp takes at most, logits of a piece.  616 rows of 152,064 (a third of the drafts' greedy and
 // not read, 320 MB): 71 us; 3 blocks an SM 76, 16 pieces a warp 79, pieces of 512 logits in 4 blocks 71 but 10 % more in what merges them.
 constexpr int ROW_BLOCKS = 2, MAX_ITEMS = 8, PIECE = 1024;
-constexpr int DRAW_THREADS = 512, DRAW_WARPS = DRAW_THREADS / 32, DRAW_LOGITS = RUN / DRAW_THREADS;
-constexpr int MAX_HELD = 256;              // runs whose sums the last kernel keeps in shared memory
+constexpr int DRAW_THREADS = 512;          // of a block that draws and did not sum
+constexpr int MAX_HELD = 256;              // runs whose sums the drawing block keeps in shared memory
 
 struct PieceSum { double sum; float max; int index; int bad; int pad; };     // sum: of 2^((v - max) log2(e) / T)
 
@@ -99,7 +100,7 @@ struct Chosen {
   int draft_row;                                       // whose probabilities are taken away, -1: none
   int without;                                         // a token that is left out, -1: none
   float top, top_q;                                    // the rows' maxima
-  int pad;
+  unsigned done;                                       // blocks of the draw whose sums are there
   double c, rho;                                       // log2(e) / T; the ratio of the rows' sums, from the float32 ones
 };
 
@@ -327,15 +328,11 @@ verify_decide_kernel(const Args p) {
   }
 }
 
-__global__ void __launch_bounds__(THREADS)
-verify_sums_kernel(const Args p) {
+// The run's sums of this block, by a thread per sum, the first four.
+template <bool COUNTED>
+__device__ __forceinline__ void sum_run(const Args& p, const Chosen& at, int run, Sums* to) {
   __shared__ Sums s_sums[WARPS];
-  pdl_launch_dependents();
-  pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = blockIdx.x / p.runs, run = blockIdx.x % p.runs;
-  const Chosen at = p.chosen[r];
-  if (at.row < 0) return;
   const int begin = run * RUN, count = min(RUN, p.vocab - begin);
   const bool difference = at.draft_row >= 0;
   float v[PER_THREAD], d[PER_THREAD];
@@ -366,27 +363,28 @@ verify_sums_kernel(const Args p) {
   sum.a = warp_sum_d(sum.a);
   if (lane == 0) s_sums[warp] = sum;
   __syncthreads();
-  if (tid < 4) {                                       // a thread per sum
+  if (tid < 4) {
     double total = 0.0;
 #pragma unroll
     for (int w = 0; w < WARPS; w++) total += ((const double*)&s_sums[w])[tid];
-    ((double*)&p.sums[(size_t)r * p.runs + run])[tid] = total;
+    ((double*)to)[tid] = total;
+    if (COUNTED) {                                     // there before the block counts as done
+      __threadfence();
+      __syncwarp(0xf);
+    }
   }
 }
 
-__global__ void __launch_bounds__(DRAW_THREADS)
-verify_draw_kernel(const Args p) {
-  __shared__ double s_sum[DRAW_WARPS], s_before, s_target, s_rho;
+// A request's draw, by a block of N threads: from the sums of its runs, the run in which it falls, then its place there.
+template <int N>
+__device__ __forceinline__ void draw_token(const Args& p, const Chosen& at, const Sums* sums, int* out) {
+  constexpr int LOGITS = RUN / N;
+  __shared__ double s_sum[N / 32], s_before, s_target, s_rho;
   __shared__ int s_run, s_from_p, s_first, s_last;
   __shared__ Sums s_sums[MAX_HELD];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Chosen at = p.chosen[r];
-  if (at.row < 0) return;
-  const Sums* sums = p.sums + (size_t)r * p.runs;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (p.runs <= MAX_HELD) {                            // gone through three times
-    for (int i = tid; i < p.runs * 2; i += DRAW_THREADS) ((double2*)s_sums)[i] = ((const double2*)sums)[i];
+    for (int i = tid; i < p.runs * 2; i += N) ((double2*)s_sums)[i] = __ldcg((const double2*)sums + i);
     __syncthreads();
     sums = s_sums;
   }
@@ -433,7 +431,7 @@ verify_draw_kernel(const Args p) {
   __syncthreads();
   const int run = s_run;
   if (run < 0) {
-    if (tid == 0) p.out[at.row] = at.without;
+    if (tid == 0) *out = at.without;
     return;
   }
   const bool from_p = s_from_p != 0;
@@ -442,18 +440,18 @@ verify_draw_kernel(const Args p) {
   const float* logits = p.logits + (size_t)at.row * p.ld + begin;
   const float* draft = from_p ? nullptr : p.draft_logits + (size_t)at.draft_row * p.draft_ld + begin;
   const bool aligned = ((uintptr_t)logits & 15) == 0, aligned_q = ((uintptr_t)draft & 15) == 0;
-  float v[DRAW_LOGITS], d[DRAW_LOGITS];
+  float v[LOGITS], d[LOGITS];
 #pragma unroll
-  for (int i = 0; i < DRAW_LOGITS; i += 4) {           // side by side in every thread
-    const int place = tid * DRAW_LOGITS + i;
+  for (int i = 0; i < LOGITS; i += 4) {           // side by side in every thread
+    const int place = tid * LOGITS + i;
     const float4 t = load_four(logits, place, count, aligned), q = from_p ? t : load_four(draft, place, count, aligned_q);
     v[i] = t.x; v[i + 1] = t.y; v[i + 2] = t.z; v[i + 3] = t.w;
     d[i] = q.x; d[i + 1] = q.y; d[i + 2] = q.z; d[i + 3] = q.w;
   }
-  double w[DRAW_LOGITS], own = 0.0;
+  double w[LOGITS], own = 0.0;
 #pragma unroll
-  for (int i = 0; i < DRAW_LOGITS; i++) {
-    const int place = tid * DRAW_LOGITS + i;
+  for (int i = 0; i < LOGITS; i++) {
+    const int place = tid * LOGITS + i;
     double e = pow2(((double)v[i] - top) * at.c);
     if (!from_p) e = fmax(0.0, fma(e, rho, -pow2(((double)d[i] - top_q) * at.c)));
     w[i] = place < count && begin + place != at.without ? e : 0.0;
@@ -472,17 +470,44 @@ verify_draw_kernel(const Args p) {
   running += sum - own;
   int first = 0x7fffffff, last = -1;
 #pragma unroll
-  for (int i = 0; i < DRAW_LOGITS; i++) {
+  for (int i = 0; i < LOGITS; i++) {
     running += w[i];
     if (w[i] > 0.0) {
-      last = begin + tid * DRAW_LOGITS + i;
+      last = begin + tid * LOGITS + i;
       if (running > target && first == 0x7fffffff) first = last;
     }
   }
   if (first != 0x7fffffff) atomicMin(&s_first, first);
   if (last >= 0) atomicMax(&s_last, last);
   __syncthreads();
-  if (tid == 0) p.out[at.row] = s_first != 0x7fffffff ? s_first : s_last;      // none by rounding: the last with any weight
+  if (tid == 0) *out = s_first != 0x7fffffff ? s_first : s_last;      // none by rounding: the last with any weight
+}
+
+// FEW: the request's last block to be done draws.
+template <bool FEW>
+__global__ void __launch_bounds__(THREADS, FEW ? 2 : 3)
+verify_sums_kernel(const Args p) {
+  __shared__ int s_draws;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x / p.runs;
+  const Chosen at = p.chosen[r];
+  if (at.row < 0) return;
+  sum_run<FEW>(p, at, blockIdx.x % p.runs, p.sums + blockIdx.x);
+  if (!FEW) return;
+  if (threadIdx.x == 0) s_draws = atomicAdd(&p.chosen[r].done, 1u) == (unsigned)p.runs - 1;
+  __syncthreads();
+  if (!s_draws) return;
+  __threadfence();                                     // the other blocks' sums
+  draw_token<THREADS>(p, at, p.sums + (size_t)r * p.runs, p.out + at.row);
+}
+
+__global__ void __launch_bounds__(DRAW_THREADS)
+verify_draw_kernel(const Args p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const Chosen at = p.chosen[blockIdx.x];
+  if (at.row >= 0) draw_token<DRAW_THREADS>(p, at, p.sums + (size_t)blockIdx.x * p.runs, p.out + at.row);
 }
 
 }  // namespace
@@ -531,8 +556,14 @@ SPROUT_API int sprout_verify(const float* logits, long long ld, const float* dra
   if (sprout_check_launch("verify_rows")) return 1;
   sprout_launch(verify_decide_kernel, dim3(requests), dim3(THREADS), 0, stream, p);
   if (sprout_check_launch("verify_decide") || temperature == nullptr) return sprout_check_launch("verify_decide");
-  sprout_launch(verify_sums_kernel, dim3((unsigned)(runs * requests)), dim3(THREADS), 0, stream, p);
-  if (sprout_check_launch("verify_sums")) return 1;
+  // A launch less where the sums are one round of blocks on the device, half a block an SM where they have a draft's as well: calls of so
+  // few wait for the host, beyond it the drawing block's work behind its sum takes longer than the launch.  Without draft logits, 3 and 4 launches:
+  // 38 blocks 18.8 and 20.4 us a call, 228 18.9 and 21.0, 320 19.9 and 21.1, 342 22.9 and 21.2, 640 26.1 and 22.8; with them: 38 20.5 and
+  // 21.3, 64 20.0 and 21.9, 76 21.8 and 21.6, 96 22.4 and 21.9, 256 27.6 and 26.4.
+  const bool few = runs * requests * (draft_rows ? 4 : 1) <= 2 * sprout_sm_count();
+  if (few) sprout_launch(verify_sums_kernel<true>, dim3((unsigned)(runs * requests)), dim3(THREADS), 0, stream, p);
+  else sprout_launch(verify_sums_kernel<false>, dim3((unsigned)(runs * requests)), dim3(THREADS), 0, stream, p);
+  if (sprout_check_launch("verify_sums") || few) return sprout_check_launch("verify_sums");
   sprout_launch(verify_draw_kernel, dim3(requests), dim3(DRAW_THREADS), 0, stream, p);
   return sprout_check_launch("verify_draw");
 }

@@ -41,7 +41,7 @@ _SIGNATURES = {
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "sprout_attention_prefix_tc_supported": [_I, _I],
-    "sprout_attention_prefix": [_P, _L, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
+    "sprout_attention_prefix": [_P, _P, _L, _P, _P, _P, _I, _P, _P, _P, _P, _L, _I, _P, _P],
     "sprout_attention_prefix_mma_supported": [_I],
     "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
@@ -966,16 +966,26 @@ def paged_attention(q, cache, ctx, out, heads, kv_heads, head_dim, status):
 
 # ---------------------------------------------------------------------------------- attention over shared prefixes
 
+class _PrefixPlan(ctypes.Structure):
+    """csrc/attention_prefix.cu: PrefixPlan."""
+    _fields_ = [(name, c_void_p) for name in ("items", "order", "part_start", "seen", "extra", "table_of")] + \
+               [(name, c_int) for name in ("simple_items", "matrix_items", "narrow_items", "narrow_ctas", "wide_items", "dtype", "tokens", "parts", "heads",
+                                           "kv_heads", "head_dim", "page_tokens")]
+
+
 class SharedPrefixPlan:
     """A step's plan on the device (``shared_prefix_plan``): the arrays that ``attention_shared_prefix`` walks, for all layers of the step."""
 
     def __init__(self, host: HostPlan, page_tokens: int, heads: int, kv_heads: int, head_dim: int, dtype, buffer: torch.Tensor):
         self.host, self.page_tokens, self.heads, self.kv_heads, self.head_dim, self.dtype, self.buffer = host, page_tokens, heads, kv_heads, head_dim, dtype, buffer
         base = buffer.data_ptr()
-        self.pointers = [base + 4 * at for at, _ in host.offsets]
+        self.arguments = _PrefixPlan(*(base + 4 * at for at, _ in host.offsets), host.simple_items, host.matrix_items, host.narrow_items, host.narrow_ctas,
+                                     host.wide_items, _dtype_code(dtype), host.tokens, host.parts, heads, kv_heads, head_dim, page_tokens)
+        self.address, self.device_index = ctypes.addressof(self.arguments), buffer.get_device()
         self.scratch_floats = host.parts * heads * (head_dim + 2)          # the partial results, then their maxima and sums
+        self.sums_at = 4 * host.parts * heads * head_dim                   # bytes
         # what a call's tensors have to be
-        self.rows, self.page, self.token_shape, self.dtype_code = (host.tokens, heads * head_dim), (kv_heads, page_tokens, head_dim), (host.tokens,), _dtype_code(dtype)
+        self.rows, self.page, self.token_shape, self.item_bytes = (host.tokens, heads * head_dim), (kv_heads, page_tokens, head_dim), (host.tokens,), dtype.itemsize
 
 
 def _prefix_slots(head_dim: int, tensor_cores: bool) -> tuple[int, int, int]:
@@ -1040,27 +1050,28 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     sees the keys up to its own, and a position other than the plan's sets a status bit (another step's plan).  float32 runs on CUDA
     cores with 32-bit products, bfloat16 on tensor cores for head sizes up to 128 in steps of 16.  ``scratch``: float32 memory of
     ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own."""
-    host, pages, index = plan.host, k_cache.shape, q.get_device()
-    if not (0 <= index == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == positions.get_device() == plan.buffer.get_device()
+    pages, index, dtype = k_cache.shape, q.get_device(), plan.dtype
+    q_stride, out_stride, table_stride, table = q.stride(), out.stride(), block_table.stride(), block_table.shape
+    if not (0 <= index == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == positions.get_device() == plan.device_index
             == out.get_device() == status.get_device() == torch.cuda.current_device() and (scratch is None or scratch.get_device() == index)
-            and q.shape == plan.rows and out.shape == plan.rows and q.stride(1) == 1 and out.stride(1) == 1 and pages == v_cache.shape
-            and pages[1:] == plan.page and pages[0] > 0 and k_cache.is_contiguous() and v_cache.is_contiguous()
-            and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype == plan.dtype and block_table.dim() == 2 and block_table.stride(1) == 1
-            and block_table.shape[0] >= host.requests and block_table.shape[1] >= host.pages and block_table.dtype == torch.int32
-            and positions.dtype == torch.int32 and positions.shape == plan.token_shape and positions.is_contiguous() and status.dtype == torch.int32):
+            and q.shape == plan.rows == out.shape and q_stride[1] == 1 == out_stride[1] and pages == v_cache.shape and pages[1:] == plan.page and pages[0] > 0
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and q.dtype is dtype and out.dtype is dtype and k_cache.dtype is dtype and v_cache.dtype is dtype
+            and len(table) == 2 and table_stride[1] == 1 and table[0] >= plan.host.requests and table[1] >= plan.host.pages and block_table.dtype is torch.int32
+            and positions.dtype is torch.int32 and positions.shape == plan.token_shape and positions.is_contiguous() and status.dtype is torch.int32):
         _refuse_shared_prefix(q, k_cache, v_cache, block_table, positions, plan, out, status, scratch)
-    if _overlap(q, out):
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    # the one that starts first ends before the other (its last row is `width` elements)
+    tokens, width = plan.rows
+    gap = out_at - q_at
+    if (gap if gap >= 0 else -gap) < ((tokens - 1) * (q_stride if gap >= 0 else out_stride)[0] + width) * plan.item_bytes:
         raise KernelError("attention_shared_prefix: q and out share memory")
     if scratch is None:
         scratch = q.new_empty(plan.scratch_floats, dtype=torch.float32)
     elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < plan.scratch_floats or scratch.data_ptr() % 16:
         raise KernelError(f"attention_shared_prefix: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
-    items, order, part_start, seen, extra, table_of = plan.pointers
     at = scratch.data_ptr()
-    _run("sprout_attention_prefix", q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-         block_table.stride(0), positions.data_ptr(), items, host.simple_items, host.matrix_items, host.narrow_items, host.narrow_ctas, host.wide_items, order, part_start, seen, extra, table_of,
-         at, at + 4 * host.parts * plan.heads * plan.head_dim, out.data_ptr(), out.stride(0), plan.dtype_code, host.tokens, host.parts, plan.heads, plan.kv_heads,
-         plan.head_dim, plan.page_tokens, pages[0], status.data_ptr(), _stream())
+    _run("sprout_attention_prefix", plan.address, q_at, q_stride[0], k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), table_stride[0],
+         positions.data_ptr(), at, at + plan.sums_at, out_at, out_stride[0], pages[0], status.data_ptr(), _stream())
 
 
 def sample(logits, out, status, temperature=None, uniform=None):
@@ -1153,28 +1164,30 @@ def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperat
     ``out`` (int32 [rows]): the drafts that stand, the token after them, and -1 in the rest of the request's rows; ``accepted`` (int32
     [requests]): how many stand; both are made here unless given.  A row that is reached and holds a non-finite logit, or a draft outside
     the vocabulary, sets a status bit and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
-    name, rows, requests = "verify_drafts", drafts.numel(), row_start.numel() - 1
-    draws = temperatures is not None
-    if not (0 <= logits.get_device() == drafts.get_device() == row_start.get_device() == status.get_device() == torch.cuda.current_device()
-            and logits.dim() == 2 and logits.shape[0] == rows >= requests >= 1 <= logits.shape[1] and logits.stride(1) == 1 and logits.dtype == torch.float32
-            and drafts.dtype == row_start.dtype == status.dtype == torch.int32 and drafts.dim() == row_start.dim() == 1 and drafts.is_contiguous()
-            and row_start.is_contiguous() and out is None and accepted is None and draws == (accept is not None) == (draw is not None)
-            and (not draws or (temperatures.get_device() == accept.get_device() == draw.get_device() == logits.get_device()
-                               and temperatures.dtype == accept.dtype == draw.dtype == torch.float32 and temperatures.shape == (requests,)
-                               and accept.shape == draw.shape == (rows,) and temperatures.is_contiguous() and accept.is_contiguous() and draw.is_contiguous()))
-            and (draft_logits is None or (draft_logits.get_device() == logits.get_device() and draft_logits.dtype == torch.float32
-                                          and draft_logits.shape == (rows - requests, logits.shape[1]) and draft_logits.stride(1) == 1))):
+    rows, requests, index, shape, strides = drafts.numel(), row_start.numel() - 1, logits.get_device(), logits.shape, logits.stride()
+    draws, per_row, per_request = temperatures is not None, (rows,), (requests,)
+    if not (0 <= index == drafts.get_device() == row_start.get_device() == status.get_device() == torch.cuda.current_device()
+            and len(shape) == 2 and shape[0] == rows >= requests >= 1 <= shape[1] and strides[1] == 1 and logits.dtype is torch.float32
+            and drafts.dtype is torch.int32 and row_start.dtype is torch.int32 and status.dtype is torch.int32 and drafts.shape == per_row
+            and row_start.dim() == 1 and drafts.is_contiguous() and row_start.is_contiguous() and out is None and accepted is None
+            and draws == (accept is not None) == (draw is not None)
+            and (not draws or (temperatures.get_device() == accept.get_device() == draw.get_device() == index
+                               and temperatures.dtype is torch.float32 and accept.dtype is torch.float32 and draw.dtype is torch.float32
+                               and temperatures.shape == per_request and accept.shape == per_row == draw.shape
+                               and temperatures.is_contiguous() and accept.is_contiguous() and draw.is_contiguous()))
+            and (draft_logits is None or (draft_logits.get_device() == index and draft_logits.dtype is torch.float32
+                                          and draft_logits.shape == (rows - requests, shape[1]) and draft_logits.stride(1) == 1))):
         _check_verify(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw, out, accepted)
-    vocab = logits.shape[1]
+    vocab = shape[1]
     draft_rows = rows - requests if draft_logits is not None else 0          # none where nobody drafted anything
     if out is None:
         out = drafts.new_empty(rows)
     if accepted is None:
         accepted = drafts.new_empty(requests)
     scratch = logits.new_empty((_lib or load_library()).sprout_verify_scratch_bytes(rows + draft_rows, requests, vocab), dtype=torch.uint8)
-    _run("sprout_verify", logits.data_ptr(), logits.stride(0), draft_logits.data_ptr() if draft_rows else None,
-         draft_logits.stride(0) if draft_rows else 0, drafts.data_ptr(), row_start.data_ptr(), temperatures.data_ptr() if temperatures is not None else None,
-         accept.data_ptr() if accept is not None else None, draw.data_ptr() if draw is not None else None, out.data_ptr(), accepted.data_ptr(),
+    _run("sprout_verify", logits.data_ptr(), strides[0], draft_logits.data_ptr() if draft_rows else None,
+         draft_logits.stride(0) if draft_rows else 0, drafts.data_ptr(), row_start.data_ptr(), temperatures.data_ptr() if draws else None,
+         accept.data_ptr() if draws else None, draw.data_ptr() if draws else None, out.data_ptr(), accepted.data_ptr(),
          scratch.data_ptr(), rows, draft_rows, requests, vocab, status.data_ptr(), _stream())
     return out, accepted
 

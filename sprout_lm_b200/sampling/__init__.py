@@ -45,9 +45,6 @@ def sample(logits: torch.Tensor, status: torch.Tensor, temperatures: torch.Tenso
     return out
 
 
-__all__ = ["sample", "uniform_for"]
-
-
 def verify(logits: torch.Tensor, drafts: torch.Tensor, row_start: torch.Tensor, status: torch.Tensor, draft_logits: torch.Tensor | None = None,
            temperatures: torch.Tensor | None = None, accept: torch.Tensor | None = None, draw: torch.Tensor | None = None):
     """Drafted tokens against the target's probabilities: ``(tokens, accepted)``, int32 on the device.
@@ -56,3 +53,6 @@ def verify(logits: torch.Tensor, drafts: torch.Tensor, row_start: torch.Tensor, 
     how many stand.  What is emitted is distributed as if drawn from the target alone; a greedy request (temperature 0, or none given)
     gets the target's argmax at every place.  The arguments are those of ``kernels.verify_drafts`` (csrc/verify.cu), which this launches."""
     return kernels.verify_drafts(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw)
+
+
+__all__ = ["sample", "uniform_for", "verify", "verify_uniforms"]

@@ -140,6 +140,24 @@ def test_many_requests_and_long_drafts(model, status):
     assert any(a == n for a, n in zip(accepted, counts) if n) and any(a < n for a, n in zip(accepted, counts))
 
 
+@pytest.mark.parametrize("model", [True, False])
+def test_a_vocabulary_of_a_million(model, status):
+    """More runs of a row than the drawing block holds in shared memory."""
+    check(case([2, 0, 1], 1100003, 41, model=model, spread=0.5), status)
+
+
+@pytest.mark.parametrize("counts", [[4, 0, 8, 1], [4, 0, 8, 1, 3, 2, 6, 5] * 3])
+def test_the_same_call_many_times(counts, status):
+    """Which block is done last, where that one draws, changes from call to call; nothing else does."""
+    from sprout_lm_b200 import sampling
+    c = case(counts, 50021, 42)
+    args, more = on_device(c)
+    calls = [sampling.verify(*args, status, **more) for _ in range(200)]
+    want_tokens, want_accepted, bits = plain(c["logits"], c["drafts"], c["counts"], c["draft_logits"], c["temperatures"], c["accept"], c["draw"])
+    assert int(status.item()) == bits == 0
+    assert all(tokens.tolist() == want_tokens and accepted.tolist() == want_accepted for tokens, accepted in calls)
+
+
 def test_all_stand_and_none_stands(status):
     """Drafts that the target would draw for certain stand to the end over several batches of rows; drafts it cannot draw never do."""
     vocab, n = 200, 21
