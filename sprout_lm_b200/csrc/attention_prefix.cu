@@ -59,7 +59,7 @@ attention_prefix_simple_kernel(const Params p) {
   float* s_l = s_m + SIMPLE_ROWS;
   float* s_a = s_l + SIMPLE_ROWS;
   begin_items(p);
-  const Item item = p.items[blockIdx.x];
+  const Item item = item_at(p, blockIdx.x);
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
   // a thread keeps its four columns and walks down the rows
@@ -213,7 +213,7 @@ attention_prefix_mma_kernel(const Params p) {
   __nv_bfloat16* sK = sQ + L::ROWS * STRIDE;           // [KEYS][STRIDE]
   __nv_bfloat16* sV = sK + KEYS * STRIDE;
   begin_items(p);
-  const Item item = p.items[blockIdx.x];
+  const Item item = item_at(p, blockIdx.x);
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
   auto look_up = [&](int base) { return tid < KEYS && base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1ll; };
@@ -414,8 +414,10 @@ attention_prefix_merge_kernel(const Params p) {
   if (row >= (long long)p.tokens * p.heads) return;    // whole blocks where warps share a row
   const int head = (int)(row % p.heads), place = (int)(row / p.heads), token = p.order[place], g = head / group;
   const int first = p.part_start[place], end = p.part_start[place + 1];
-  const int seen = p.seen[place], extra = share == 0 ? p.extra[place] : 0;
-  if (share == 0 && head == 0 && lane == 0 && p.positions[token] != seen + extra - 1) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);      // another step's plan
+  // how far the step is behind the plan's own; outside what the plan serves it is another step's
+  const int all_extra = p.extra[place], ahead = p.positions[token] - (p.seen[place] + all_extra - 1), extra = share == 0 ? all_extra : 0;
+  const int seen = p.seen[place] + min(max(ahead, 0), p.stretch);
+  if (share == 0 && head == 0 && lane == 0 && (ahead < 0 || ahead > p.stretch)) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);
   float m = -INFINITY, l = 0.f, sum[PAIRS][2];
 #pragma unroll
   for (int k = 0; k < PAIRS; k++) sum[k][0] = sum[k][1] = 0.f;
@@ -573,9 +575,9 @@ SPROUT_API int sprout_attention_prefix_mma_supported(int head_dim) { return head
 struct PrefixPlan {
   const Item* items;
   const int* order; const int* part_start; const int* seen; const int* extra; const int* table_of;
-  int simple_items, matrix_items, narrow_items, narrow_ctas, wide_items, dtype, tokens, parts, heads, kv_heads, head_dim, page_tokens;
+  int simple_items, matrix_items, narrow_items, narrow_ctas, wide_items, dtype, tokens, parts, heads, kv_heads, head_dim, page_tokens, stretch, unused;
 };
-static_assert(sizeof(PrefixPlan) == 6 * 8 + 12 * 4, "as ctypes lays it out");
+static_assert(sizeof(PrefixPlan) == 6 * 8 + 14 * 4, "as ctypes lays it out");
 
 // part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
 SPROUT_API int sprout_attention_prefix(const PrefixPlan* plan, const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
@@ -584,13 +586,13 @@ SPROUT_API int sprout_attention_prefix(const PrefixPlan* plan, const void* q, lo
                  part_sum && out && status, "attention_shared_prefix: null pointer");
   const int simple_items = plan->simple_items, matrix_items = plan->matrix_items, narrow_items = plan->narrow_items, narrow_ctas = plan->narrow_ctas, wide_items = plan->wide_items;
   const int dtype = plan->dtype, tokens = plan->tokens, parts = plan->parts, heads = plan->heads, kv_heads = plan->kv_heads, head_dim = plan->head_dim, page_tokens = plan->page_tokens;
-  SPROUT_REQUIRE(tokens > 0 && parts > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
+  SPROUT_REQUIRE(tokens > 0 && parts > 0 && plan->stretch >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
                  "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
   SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (narrow_items == 0 || narrow_ctas > 0) && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
   SPROUT_REQUIRE(((uintptr_t)part_out & 15) == 0 && ((uintptr_t)part_sum & 7) == 0, "attention_shared_prefix: the partial results must start on 16- and 8-byte boundaries");
   Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, plan->items, plan->order, plan->part_start, plan->seen, plan->extra, plan->table_of, part_out, (float2*)part_sum, out, out_stride,
-           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, 1};
+           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, plan->stretch, 1};
   if (simple_items > 0) {
     // rows that are whole fours on their boundaries
     const int row = dtype == SPROUT_F32 ? 16 : 8;

@@ -19,7 +19,7 @@ struct Item {
   int token_begin;                     // the segment's first token, in the plan's order
   int row_begin, rows;                 // of the segment's rows: (token - token_begin) * group + head within the group
   int part;                            // the place of this range among the token's ranges
-  int pad;
+  int open;                            // the range grows with the member: it ends with what its tokens all see (see Params::stretch)
 };
 
 struct Params {
@@ -39,6 +39,9 @@ struct Params {
   int tokens, heads, kv_heads, head_dim, page_tokens, num_pages;
   float scale_log2;                    // log2(e) / sqrt(head_dim)
   int* status;
+  // The plan serves steps whose tokens stand up to this many positions behind those that it was made for; the member's last own range is
+  // open then.
+  int stretch;
   int first;                           // the call's first launch (see begin_items)
 };
 
@@ -51,6 +54,13 @@ __device__ __forceinline__ void begin_items(const Params& p) {
 }
 __device__ __forceinline__ void end_items(const Params& p) { if (!p.first) pdl_wait(); }
 
+// An item as it is in this step: an open range ends with the member's first token, within the plan's bounds and never empty, whatever the
+// positions say.
+__device__ __forceinline__ Item item_at(const Params& p, int index) {
+  Item item = p.items[index];
+  if (item.open) item.key_end = max(item.key_begin + 1, min(item.key_end, p.positions[p.order[item.token_begin]] + 1));
+  return item;
+}
 // An item's row i, 0 <= i < rows: its place in the plan's order, and its query head.
 __device__ __forceinline__ int place_of_row(const Item& item, int i, int group) { return item.token_begin + (item.row_begin + i) / group; }
 __device__ __forceinline__ int head_of_row(const Item& item, int i, int group, int g) { return g * group + (item.row_begin + i) % group; }

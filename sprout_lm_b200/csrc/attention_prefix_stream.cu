@@ -86,7 +86,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     const uint32_t stages = smem_u32(smem);
     const int boxes = KEYS / box_rows;
     int round = 0, pair = pair_of(0), next_pair = pair_of(1);
-    Item item = p.items[pair / p.kv_heads], next_item = p.items[max(next_pair, 0) / p.kv_heads];
+    Item item = item_at(p, pair / p.kv_heads), next_item = item_at(p, max(next_pair, 0) / p.kv_heads);
     int base = item.key_begin;
     auto box_key = [&]() {
       const int key = base + lane * box_rows;
@@ -107,7 +107,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
         item = next_item;
         base = item.key_begin;
         next_pair = pair_of(round + 1);
-        next_item = p.items[max(next_pair, 0) / p.kv_heads];
+        next_item = item_at(p, max(next_pair, 0) / p.kv_heads);
       }
       key = box_key();
       page = page_of(key);
@@ -152,7 +152,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     }
   };
   int pair = pair_of(0);                               // the grid has at most as many CTAs as there are pairs
-  Item item = p.items[pair / p.kv_heads];
+  Item item = item_at(p, pair / p.kv_heads);
   uint4 q[EACH];
   query(item, pair % p.kv_heads, q);
   bool ok = true;
@@ -169,7 +169,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     for (int k = 0; k < EACH; k++) { const int idx = tid + k * COMPUTE; *(uint4*)(sQ + idx / PIECES * L::Q_STRIDE + idx % PIECES * 8) = q[k]; }
     compute_barrier();
     const int next_pair = pair_of(round + 1);
-    const Item next_item = p.items[max(next_pair, 0) / p.kv_heads];
+    const Item next_item = item_at(p, max(next_pair, 0) / p.kv_heads);
     if (next_pair >= 0) query(next_item, next_pair % p.kv_heads, q);
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[2 * MINE][4];
 #pragma unroll

@@ -90,7 +90,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
   begin_items(p);
 
-  const Item item = p.items[blockIdx.x];
+  const Item item = p.items[blockIdx.x];               // whole pages: never open
   const int g = blockIdx.y, group = p.heads / p.kv_heads;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
   const bool two = item.rows > ROWS;                   // the second Q tile has rows

@@ -66,7 +66,8 @@ class DecodeGraph:
 
     RING = 3            # pinned buffers per graph: more launches than two are never in flight
 
-    def __init__(self, runner, requests: int, table_pages: int, planned_context: int = 0):
+    def __init__(self, runner, requests: int, table_pages: int, planned_context: int = 0, shared=None):
+        """``shared``: plans of shared pages by attention sizes, for all steps that the capture is replayed for (``engine.shared``)."""
         self.runner = runner
         self.requests = R = requests
         self.table_pages = table_pages
@@ -106,7 +107,7 @@ class DecodeGraph:
             block_tables=[view(f"table{g}").view(R, table_pages) for g in range(self.groups)],
             page_tokens=runner.page_tokens,
             floats={"temperature": view("temperature").view(torch.float32), "uniform": view("uniform").view(torch.float32)},
-            planned_context=planned_context)
+            planned_context=planned_context, shared=shared)
         self._seqs = None
         self._known = None                # pages of each request's tables already in the host mirror
         self.graph = None

@@ -138,7 +138,11 @@ class ModelRunner:
         for e in entries:
             if e.seq.released or e.seq.length + 2 > self.max_positions or not self.reserve(e.seq, e.seq.length + 2):
                 return False                       # the planner decides what happens when pages run out
-        graph = self.graphs.get(entries, shift=1)
+        graph = self.shared_prefix.captured(entries, shift=1) if self.shared_prefix else None
+        if graph is None:
+            if self.shared_prefix and self.shared_prefix.due(entries, behind=1):
+                return False                       # that step may capture one over shared pages: through the ordinary path
+            graph = self.graphs.get(entries, shift=1)
         if graph.graph is None:
             return False                           # a first use runs eagerly and captures: through the ordinary path
         ticket = graph.launch(entries, temperatures, uniforms, shift=1, feed_rows=list(feed_rows))
@@ -192,10 +196,11 @@ class ModelRunner:
         self.validate(entries)
         decode_only = self.graphs.enabled and all(len(e.tokens) == 1 and e.want == [0] for e in entries)
         taken = self._take_ahead(entries, temperatures, uniforms)
-        shared = self.shared_prefix.plans(entries, replayed=decode_only) if self.shared_prefix and taken is None else None
+        graph = self.shared_prefix.decode_graph(entries, taken is None) if self.shared_prefix and decode_only else None
+        shared = self.shared_prefix.plans(entries, replayed=decode_only) if self.shared_prefix and taken is None and graph is None else None
         if decode_only and shared is None:
             if taken is None:
-                graph = self.graphs.get(entries)
+                graph = graph or self.graphs.get(entries)
                 if graph.graph is None:
                     sampled = graph.run(entries, temperatures, uniforms)      # first use: runs eagerly, then captures
                     ticket = None
@@ -207,6 +212,8 @@ class ModelRunner:
                 if then is not None:
                     self._launch_next(then)
                 sampled = graph.collect(ticket)
+            if graph.ctx.shared is not None:
+                self.shared_prefix.steps += 1
             self.last_decode_graph = graph
             self._last_sampled = sampled
             self.stats["h2d_bytes"] += graph.stager.last_bytes

@@ -970,7 +970,7 @@ class _PrefixPlan(ctypes.Structure):
     """csrc/attention_prefix.cu: PrefixPlan."""
     _fields_ = [(name, c_void_p) for name in ("items", "order", "part_start", "seen", "extra", "table_of")] + \
                [(name, c_int) for name in ("simple_items", "matrix_items", "narrow_items", "narrow_ctas", "wide_items", "dtype", "tokens", "parts", "heads",
-                                           "kv_heads", "head_dim", "page_tokens")]
+                                           "kv_heads", "head_dim", "page_tokens", "stretch", "unused")]
 
 
 class SharedPrefixPlan:
@@ -980,7 +980,7 @@ class SharedPrefixPlan:
         self.host, self.page_tokens, self.heads, self.kv_heads, self.head_dim, self.dtype, self.buffer = host, page_tokens, heads, kv_heads, head_dim, dtype, buffer
         base = buffer.data_ptr()
         self.arguments = _PrefixPlan(*(base + 4 * at for at, _ in host.offsets), host.simple_items, host.matrix_items, host.narrow_items, host.narrow_ctas,
-                                     host.wide_items, _dtype_code(dtype), host.tokens, host.parts, heads, kv_heads, head_dim, page_tokens)
+                                     host.wide_items, _dtype_code(dtype), host.tokens, host.parts, heads, kv_heads, head_dim, page_tokens, host.stretch, 0)
         self.address, self.device_index = ctypes.addressof(self.arguments), buffer.get_device()
         self.scratch_floats = host.parts * heads * (head_dim + 2)          # the partial results, then their maxima and sums
         self.sums_at = 4 * host.parts * heads * head_dim                   # bytes
@@ -997,12 +997,15 @@ def _prefix_slots(head_dim: int, tensor_cores: bool) -> tuple[int, int, int]:
     return sms * (3 if head_dim > 96 else 4), sms, sms * (2 if head_dim > 64 else 3 if head_dim > 48 else 4)
 
 
-def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, head_dim: int, dtype, device=None) -> SharedPrefixPlan:
+def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, head_dim: int, dtype, device=None,
+                       stretch: int = 0) -> SharedPrefixPlan:
     """How ``attention_shared_prefix`` divides the keys of a step.  All on the host: ``tables`` [requests, pages] the requests' pages
     (entries behind a request's last page are not read), ``q_start`` [requests + 1] where each request's tokens start among the step's,
     ``contexts`` [requests] the keys that each request's last token sees.  Runs of leading pages that several requests hold are found in
     the tables, branching ones too; pages that this step still writes are nobody else's.  ``dtype``: of the cache.  The plan depends on
-    nothing else, and one made for a step serves all its layers with these sizes."""
+    nothing else, and one made for a step serves all its layers with these sizes.  ``stretch``: it also serves steps of the same requests
+    with the same numbers of tokens whose contexts are up to this many keys longer, each request's by as many as it likes (a captured
+    decode step, replayed); their block tables are wide enough for all of those."""
     _dtype_code(dtype)
     if not 0 < head_dim <= 256 or head_dim % 2:
         raise KernelError(f"shared_prefix_plan: head_dim must be even and at most 256 (got {head_dim})")
@@ -1012,7 +1015,7 @@ def shared_prefix_plan(tables, q_start, contexts, page_tokens: int, heads: int, 
     if head_dim not in (64, 128) or not (page_tokens in (8, 16, 32, 64) or page_tokens % 128 == 0):
         matrix_slots = 0
     try:
-        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, slots, matrix_slots, narrow_slots, head_dim)
+        host = HostPlan(tables, q_start, contexts, page_tokens, heads, kv_heads, tensor_cores, slots, matrix_slots, narrow_slots, head_dim, stretch)
     except PlanError as error:
         raise KernelError(f"shared_prefix_plan: {error}") from None
     packed = torch.from_numpy(host.pack())
@@ -1047,7 +1050,7 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     """Causal attention of a step's tokens over their requests' pages, a run of pages that several requests hold read once for all of
     them.  ``q`` and ``out`` [tokens, heads * head_dim] (rows may lie apart), the caches [pages, kv_heads, page_tokens, head_dim], all
     of the plan's type; ``block_table`` int32 [requests, pages] holds what the plan was made of; ``positions`` int32 [tokens]: a token
-    sees the keys up to its own, and a position other than the plan's sets a status bit (another step's plan).  float32 runs on CUDA
+    sees the keys up to its own, and a position that the plan does not serve sets a status bit (another step's plan).  float32 runs on CUDA
     cores with 32-bit products, bfloat16 on tensor cores for head sizes up to 128 in steps of 16.  ``scratch``: float32 memory of
     ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own."""
     pages, index, dtype = k_cache.shape, q.get_device(), plan.dtype

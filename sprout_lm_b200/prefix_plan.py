@@ -20,6 +20,7 @@ MATRIX_FROM = 48            # rows of a segment
 MATRIX_US, MATRIX_STEP_US, NARROW_STEP_US = 8.0, 2.0, 2.0      # of items beside one another: a matrix item's start and step, a step of few rows
 ITEM_STEPS = 0.5            # what an item of few rows costs beside its steps
 MAX_RANGES = 64             # of a segment
+MAX_STRETCH = 1024          # positions that a plan's steps may be behind its own: its items are sized for its own
 # A shared run is a segment of its own if reading it once saves this many key reads (a member fewer than hold it, times its keys): below,
 # the members read it themselves.
 MIN_SAVED_KEYS = 64
@@ -32,12 +33,13 @@ class PlanError(ValueError):
 
 class Segment:
     """Keys ``key_begin`` to ``key_end`` of the pages in block table row ``table``, seen by the places ``token_begin`` to ``token_end`` of the
-    plan's order; ``part``: the first of its partial results at each of these places (``ranges`` of them)."""
-    __slots__ = ("table", "key_begin", "key_end", "token_begin", "token_end", "part", "ranges")
+    plan's order; ``part``: the first of its partial results at each of these places (``ranges`` of them); ``own``: one member's, what it
+    sees behind its last shared run."""
+    __slots__ = ("table", "key_begin", "key_end", "token_begin", "token_end", "part", "ranges", "own")
 
-    def __init__(self, table, key_begin, key_end, token_begin=0, token_end=0):
+    def __init__(self, table, key_begin, key_end, token_begin=0, token_end=0, own=False):
         self.table, self.key_begin, self.key_end, self.token_begin, self.token_end = table, key_begin, key_end, token_begin, token_end
-        self.part, self.ranges = 0, 1
+        self.part, self.ranges, self.own = 0, 1, own
 
 
 def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray, page_tokens: int, group: int = 1):
@@ -72,9 +74,9 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
             segments[parent].token_end = placed
         elif len(members) == 1:
             member = members[0]
-            if int(sees[member]) > start * page_tokens:      # else all it sees lies in shared runs
-                segments.append(Segment(int(request[member]), int(start) * page_tokens, int(sees[member]), placed, placed + int(tokens[member])))
-                parents.append(parent)
+            # never empty: what is shared ends before the step's own tokens
+            segments.append(Segment(int(request[member]), int(start) * page_tokens, int(sees[member]), placed, placed + int(tokens[member]), own=True))
+            parents.append(parent)
             leaves.append(member)
             placed += int(tokens[member])
         else:
@@ -192,10 +194,12 @@ def spread(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> n
 
 
 class HostPlan:
-    """The plan's arrays on the host: ``items`` [n, 8] (simple ones, or matrix, narrow and wide ones), ``order``, ``part_start``, ``seen``,
+    """The plan's arrays on the host, for a step and for those of the same requests and numbers of tokens up to ``stretch`` positions behind
+    it: ``items`` [n, 8] (simple ones, or matrix, narrow and wide ones), ``order``, ``part_start``, ``seen``,
     ``extra``, ``table_of``."""
 
-    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0, narrow_slots: int | None = None, head_dim: int = 64):
+    def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0, narrow_slots: int | None = None, head_dim: int = 64,
+                 stretch: int = 0):
         tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
         if tables.ndim != 2 or q_start.ndim != 1 or contexts.ndim != 1 or len(contexts) == 0 or len(q_start) != len(contexts) + 1 or len(tables) < len(contexts):
             raise PlanError("a block table row and a context per request, and where each request's tokens start")
@@ -205,22 +209,24 @@ class HostPlan:
         counts = np.diff(q_start)
         if q_start[0] != 0 or (counts < 1).any() or (contexts < counts).any():
             raise PlanError("every request brings a token or more, and its context holds them")
-        if page_tokens < 1 or int(contexts.max()) > tables.shape[1] * page_tokens or int(contexts.max()) > 0x7fffffff:
+        if page_tokens < 1 or int(contexts.max()) > tables.shape[1] * page_tokens or int(contexts.max()) > 0x7fffffff - MAX_STRETCH:
             raise PlanError("a context reaches beyond its block table")
+        if type(stretch) is not int or not 0 <= stretch <= MAX_STRETCH:
+            raise PlanError(f"stretch must be a whole number up to {MAX_STRETCH} (got {stretch!r})")
         if kv_heads < 1 or heads < 1 or heads % kv_heads:
             raise PlanError(f"heads ({heads}) must be a multiple of the key/value heads ({kv_heads})")
         self.narrow_ctas = 0                             # that walk the narrow items
         self.tokens, self.requests = int(q_start[-1]), len(contexts)
-        self.pages = int(-(-contexts.max() // page_tokens))
+        self.stretch, self.pages = stretch, int(-(-(contexts.max() + stretch) // page_tokens))       # pages: of a call's block tables
         group = heads // kv_heads
         segments, parents, order, seen, extra, table_of = find_segments(tables, q_start, contexts, page_tokens, group)
         begin = np.array([s.key_begin for s in segments])
         end = np.array([s.key_end for s in segments])
-        token_begin = np.array([s.token_begin for s in segments])
+        token_begin, own = np.array([s.token_begin for s in segments]), np.array([s.own for s in segments])
         rows = (np.array([s.token_end for s in segments]) - token_begin) * group
         # the kinds: 0 a matrix product's worth of rows over whole pages, 1 few rows, 2 more; all of 1 on the CUDA cores
         if tensor_cores:
-            whole = (rows >= MATRIX_FROM) & (end % page_tokens == 0) & (begin % page_tokens == 0) if matrix_slots else np.zeros(len(segments), dtype=bool)
+            whole = (rows >= MATRIX_FROM) & ~(own & (stretch > 0)) & (end % page_tokens == 0) & (begin % page_tokens == 0) if matrix_slots else np.zeros(len(segments), dtype=bool)
             kind = choose_kinds(rows, -(-(end - begin) // KEY_STEP), whole, kv_heads, head_dim, slots, matrix_slots, narrow_slots or slots)
             tile_rows = np.array([MATRIX_ROWS, NARROW_ROWS, WIDE_ROWS])[kind]
         else:
@@ -265,6 +271,9 @@ class HostPlan:
         items[:, 4] = tile * tile_rows[of]
         items[:, 5] = np.minimum(rows[of] - items[:, 4], tile_rows[of])
         items[:, 6] = part[of] + rng
+        if stretch:
+            items[:, 7] = own[of] & (rng == ranges[of] - 1)                 # a member's last own range grows with the steps
+            items[:, 2] += items[:, 7] * stretch
         of_kind = kind[of]
         items = items[np.lexsort((items[:, 1] - items[:, 2], of_kind))]     # longest first within a kind
         counts = np.bincount(of_kind, minlength=3).tolist()

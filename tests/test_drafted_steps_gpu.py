@@ -218,6 +218,75 @@ def test_generation_with_shared_prompts(model_dirs):
         assert len(result["output"]) == 10 and nearly_greedy(model, model_dirs["B"], prompt, result["output"], "bfloat16")
 
 
+@pytest.mark.parametrize("name", ["A", "B", "wide"])
+def test_captured_steps_over_a_shared_prompt(model_dirs, name, monkeypatch):
+    """Decode steps of the same requests: one captured over their pages serves as many as its plan does, the next is made behind it, and
+    another request among them ends it."""
+    from sprout_lm_b200 import load_model
+    from sprout_lm_b200.engine import shared
+    from sprout_lm_b200.engine.batch import StepEntry
+    monkeypatch.setattr(shared, "STRETCH", 7)
+    directory = model_dirs[name]
+    model = load_model(directory, dtype="bfloat16")
+    page, vocab = 8, model.spec.vocab_size
+    rng = np.random.default_rng(53)
+    prefix = helpers.random_tokens(rng, 11 * page + 3, vocab)
+    tails = [helpers.random_tokens(rng, n, vocab) for n in (1, 9, 30, 5, 2, 14)]
+    runner, seqs = started(model, prefix, tails, page)
+    steps = runner.shared_prefix
+    steps.after, steps.always = 2, True
+    histories, graphs = [prefix + tail for tail in tails], []
+
+    def decode(which):
+        new = [int(rng.integers(vocab)) for _ in which]
+        runner.step_and_sample([StepEntry(seqs[r], [t], [0]) for r, t in zip(which, new)], [0.0] * len(which), [0.0] * len(which))
+        for r, t in zip(which, new):
+            histories[r].append(t)
+        graph = steps._graph
+        if graph is not None:
+            assert runner.last_decode_graph is graph and graph.ctx.shared is not None
+            if graph not in graphs:
+                graphs.append(graph)
+            logits = graph.last_logits.float().cpu().numpy()
+            for row, r in enumerate(which):
+                assert float(np.abs(logits[row] - helpers.plain_logits(directory, histories[r])[-1]).max()) <= tolerance(model, "bfloat16")
+        return graph
+
+    made = [decode([0, 1, 2, 3, 4, 5]) for _ in range(19)]
+    assert made[0] is None and made[1] is not None                  # the second step of the same requests
+    assert [made.index(g) for g in graphs] == [1, 9, 17]            # a plan serves its own step and seven behind it
+    assert [decode([5, 3, 1]) is None for _ in range(3)] == [True, False, False]
+    assert len(graphs) == 4 and steps.steps == 22
+    # other steps in between, and a request that was taken back further than its plan's first step
+    assert decode([5, 3, 1]) is graphs[3]
+    seqs[3].length -= 5
+    del histories[3][-5:]
+    assert decode([5, 3, 1]) is not graphs[3] and len(graphs) == 5
+    steps.always = False
+    assert decode([0, 1]) is None and decode([0, 1]) is None        # it does not pay here
+    runner.check_status()
+
+
+def test_captured_generation_with_shared_prompts(model_dirs, monkeypatch):
+    """The same through the scheduler, whose steps are launched ahead."""
+    from sprout_lm_b200 import EngineOptions, generate, load_model, make_engine
+    from sprout_lm_b200.engine import shared
+    monkeypatch.setattr(shared, "STRETCH", 11)
+    model = load_model(model_dirs["B"], dtype="bfloat16")
+    rng = np.random.default_rng(59)
+    prefix = helpers.random_tokens(rng, 80, 509)
+    prompts = [prefix + helpers.random_tokens(rng, n, 509) for n in (1, 20, 9, 33)]
+    engine = make_engine(model, EngineOptions(block_size=8, num_blocks=160, max_sequences=4, max_batch_tokens=64, prefill_chunk_size=48, shared_prefix=True))
+    runner = engine.runner
+    runner.shared_prefix.always, runner.shared_prefix.after = True, 2
+    runner.shared_prefix.plans = lambda entries, replayed: None     # captured ones alone
+    generate(model, prompts[:1], max_new_tokens=1, ignore_eos=True, engine=engine)      # publishes the prefix
+    results = generate(model, prompts, max_new_tokens=40, ignore_eos=True, engine=engine)
+    assert runner.shared_prefix.steps >= 30 and runner.ahead_used >= 20
+    for prompt, result in zip(prompts, results):
+        assert len(result["output"]) == 40 and nearly_greedy(model, model_dirs["B"], prompt, result["output"], "bfloat16")
+
+
 def test_plans_are_taken_where_they_pay(model_dirs):
     """Without ``always``: not for a tiny model's short prompt."""
     from sprout_lm_b200 import load_model

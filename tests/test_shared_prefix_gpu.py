@@ -340,3 +340,77 @@ def test_refusals(status):
     refused("unit inner stride", q=step.q.t())
     refused("16-byte", q=torch.empty(step.q.numel() + 1, dtype=BF16, device=DEV)[1:].view_as(step.q))
     assert int(status.item()) == 0
+
+
+# ---------------------------------------------------------------------------------- plans for later steps
+
+LATER = [(14, 2, 64, BF16, 16), (28, 4, 128, BF16, 16), (14, 2, 64, BF16, 5), (5, 1, 48, BF16, 16), (28, 4, 128, BF16, 128), (6, 3, 40, BF16, 8), (14, 2, 64, F32, 16), (3, 1, 144, BF16, 16)]
+
+
+def earlier_plan(step, ahead, stretch):
+    """The plan that the step's requests would have had `ahead` tokens before, good for `stretch` more."""
+    from sprout_lm_b200 import kernels
+    contexts = [c - a for c, a in zip(step.contexts, ahead)]
+    tables = step.tables.copy()
+    for row, c in zip(tables, contexts):
+        row[-(-c // step.page):] = -1                     # pages that the requests did not have yet
+    tables = tables[:, :-(-max(contexts) // step.page)]
+    return kernels.shared_prefix_plan(tables, step.q_start, contexts, step.page, step.heads, step.kv_heads, step.dim, step.dtype, DEV, stretch=stretch)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,page", LATER)
+@pytest.mark.parametrize("tokens", [1, 5, 20])
+def test_a_plan_for_later_steps(heads, kv_heads, dim, dtype, page, tokens, status):
+    rng = np.random.default_rng(tokens)
+    own = [130, 20, 300, 64, 200, 128, 1, 160]
+    ahead = [0, 5, 128, 64, 17, 128, 0, 1]
+    counts = [int(n) for n in rng.integers(1, tokens + 1, len(own))]
+    step = Step(heads, kv_heads, dim, dtype, page, [0] * len(own), [40], own, counts, seed=tokens, table_pad=-(-128 // page))
+    plan = earlier_plan(step, ahead, 128)
+    out = step.run(status, plan=plan)
+    want, tol = step.exact()
+    assert int(status.item()) == 0
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("requests,prefix", [(20, 130), (48, 400)])
+def test_a_captured_step_replayed_for_later_ones(requests, prefix, status):
+    """One capture for decode steps 0 to 70 positions behind its plan: items of few rows and, over the prefix, matrix items."""
+    from sprout_lm_b200 import kernels
+    rng = np.random.default_rng(requests)
+    own = [70 + int(n) for n in rng.integers(0, 200, requests)]
+    last = Step(28, 4, 128, BF16, 16, [0] * requests, [prefix], own, [1] * requests, seed=7, table_pad=5)
+    plan, out, scratch = earlier_plan(last, [70] * requests, 70), torch.empty_like(last.q), None
+    assert plan.host.matrix_items > 0 and plan.host.narrow_items > 0
+    scratch = torch.empty(plan.scratch_floats, device=DEV)
+    positions = last.positions.clone()
+    last.positions -= 70
+    call = lambda: kernels.attention_shared_prefix(last.q, last.k, last.v, last.block_table, last.positions, plan, out, status, scratch)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for behind in (70, 69, 41, 0, 13):
+        last.positions.copy_(positions - behind)
+        out.fill_(float("nan"))
+        graph.replay()
+        want, tol = last.exact()
+        assert bool(((out.double() - want).abs() <= tol).all()), behind
+    assert int(status.item()) == 0
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,page", LATER[:4])
+@pytest.mark.parametrize("off", [-1, 129])
+def test_a_step_that_the_plan_does_not_serve(heads, kv_heads, dim, dtype, page, off, status):
+    """Further back than the plan's own, or beyond its stretch: a status bit, and the other requests' rows are as they should be."""
+    own = [300, 310, 320]
+    step = Step(heads, kv_heads, dim, dtype, page, [0, 0, 0], [40], own, [1, 1, 1], seed=3, table_pad=-(-200 // page))
+    plan = earlier_plan(step, [100, 129 if off > 0 else 0, 128], 128)
+    if off < 0:
+        step.positions[1] -= 1
+    out = step.run(status, plan=plan)
+    assert int(status.item()) == 16
+    want, tol = step.exact()
+    keep = torch.tensor([0, 2], device=DEV)
+    assert bool(((out.double() - want).abs() <= tol)[keep].all()) and bool(torch.isfinite(out).all())

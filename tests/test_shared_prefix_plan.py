@@ -60,6 +60,36 @@ def test_every_key_once(seed):
                 assert keys == [(k, int(tables[request, k // page])) for k in range(plan.seen[place])]
 
 
+@pytest.mark.parametrize("seed", range(20))
+def test_every_key_once_in_later_steps(seed):
+    """A plan for steps whose requests are each up to ``stretch`` positions further: open items end with their member's first token."""
+    rng = random.Random(100 + seed)
+    page, group, kv_heads, stretch = rng.choice([1, 4, 8, 32]), rng.choice([1, 3, 7]), rng.choice([1, 2]), rng.choice([1, 17, 128, 1024])
+    tables, q_start, contexts = batch(rng, rng.randint(1, 12), page, [rng.randint(1, 30) for _ in range(3)], rng.choice([[1], [1, 2, 5], [1, 16, 17, 40]]), 60)
+    room = np.full((len(tables), -(-stretch // page)), -1, dtype=np.int32)
+    ahead = np.array([rng.choice([0, stretch, rng.randint(0, stretch)]) for _ in contexts])
+    for tensor_cores in (True, False):
+        plan = HostPlan(tables, q_start, contexts, page, group * kv_heads, kv_heads, tensor_cores, rng.choice([1, 8, 60, 600]), rng.choice([0, 1, 148]), stretch=stretch)
+        own = HostPlan(tables, q_start, contexts, page, group * kv_heads, kv_heads, tensor_cores, 60, 0)
+        assert plan.pages * page >= contexts.max() + stretch and plan.pages <= tables.shape[1] + room.shape[1]
+        assert (plan.order == own.order).all() and (plan.seen == own.seen).all() and (plan.extra == own.extra).all()
+        assert not plan.items[:plan.matrix_items, 7].any()
+        keys = np.zeros((plan.tokens, group), dtype=np.int64)
+        for table, key_begin, key_end, token_begin, row_begin, rows, _, is_open in plan.items.tolist():
+            if is_open:                # as csrc/attention_prefix.cuh has it: to the member's first token
+                first = plan.seen[token_begin] + ahead[plan.table_of[token_begin]]
+                assert key_begin < plan.seen[token_begin] <= first <= key_end
+                key_end = first
+            keys[token_begin:].reshape(-1)[row_begin:row_begin + rows] += key_end - key_begin
+        assert (keys == (plan.seen + ahead[plan.table_of])[:, None]).all()
+
+
+@pytest.mark.parametrize("stretch", [-1, 1025, 2.0, True, None])
+def test_stretch_is_checked(stretch):
+    with pytest.raises(PlanError, match="stretch"):
+        HostPlan([[0, 1]], [0, 1], [5], 8, 4, 1, True, 60, stretch=stretch)
+
+
 def test_a_shared_prefix_is_read_once():
     requests, page, prefix = 50, 16, 1600
     tables = np.arange(requests * 110, dtype=np.int32).reshape(requests, 110)
