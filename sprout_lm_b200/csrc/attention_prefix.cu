@@ -415,9 +415,14 @@ attention_prefix_merge_kernel(const Params p) {
   const int head = (int)(row % p.heads), place = (int)(row / p.heads), token = p.order[place], g = head / group;
   const int first = p.part_start[place], end = p.part_start[place + 1];
   // how far the step is behind the plan's own; outside what the plan serves it is another step's
-  const int all_extra = p.extra[place], ahead = p.positions[token] - (p.seen[place] + all_extra - 1), extra = share == 0 ? all_extra : 0;
-  const int seen = p.seen[place] + min(max(ahead, 0), p.stretch);
-  if (share == 0 && head == 0 && lane == 0 && (ahead < 0 || ahead > p.stretch)) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);
+  const int extra = share == 0 ? p.extra[place] : 0;
+  int seen = p.seen[place];
+  if (share == 0 && head == 0 && lane == 0) {
+    const int ahead = p.positions[token] - (seen + extra - 1);
+    if (ahead < 0 || ahead > p.stretch) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);        // a step that the plan does not serve
+  }
+  // where the member's further keys begin in this step
+  if (p.stretch > 0 && extra > 0) seen += min(max(p.positions[token] - (seen + extra - 1), 0), p.stretch);
   float m = -INFINITY, l = 0.f, sum[PAIRS][2];
 #pragma unroll
   for (int k = 0; k < PAIRS; k++) sum[k][0] = sum[k][1] = 0.f;

@@ -58,7 +58,7 @@ __device__ __forceinline__ void end_items(const Params& p) { if (!p.first) pdl_w
 // positions say.
 __device__ __forceinline__ Item item_at(const Params& p, int index) {
   Item item = p.items[index];
-  if (item.open) item.key_end = max(item.key_begin + 1, min(item.key_end, p.positions[p.order[item.token_begin]] + 1));
+  if (p.stretch > 0 && item.open) item.key_end = max(item.key_begin + 1, min(item.key_end, p.positions[p.order[item.token_begin]] + 1));
   return item;
 }
 // An item's row i, 0 <= i < rows: its place in the plan's order, and its query head.

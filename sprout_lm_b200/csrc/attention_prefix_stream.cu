@@ -44,7 +44,9 @@ __device__ __forceinline__ bool compute_barrier_and(bool mine) {
   return all != 0;
 }
 
-template <int HD>
+// LATER: the plan serves later steps too (Params::stretch).  Looking whether an item is open costs 0.3 to 0.9 us a launch: few items 7.0 us
+// without and 7.4 with, a long walk 47.0 and 47.9.
+template <int HD, bool LATER>
 __global__ void __launch_bounds__(THREADS, Layout<HD>::CTAS)
 attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p, const int pairs, const int box_rows) {
   using L = Layout<HD>;
@@ -78,6 +80,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     const long long index = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     return index < pairs ? (int)index : -1;
   };
+  auto item_of = [&](int at) { return LATER ? item_at(p, at) : p.items[at]; };
   auto gave_up = [&]() { *abort_flag = 1; atomicOr(p.status, SPROUT_STATUS_WAIT_TIMEOUT); };
   int steps = 0;                                       // whose copies were issued (the copying warp), or that were computed
   if (warp == 4) {
@@ -86,7 +89,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     const uint32_t stages = smem_u32(smem);
     const int boxes = KEYS / box_rows;
     int round = 0, pair = pair_of(0), next_pair = pair_of(1);
-    Item item = item_at(p, pair / p.kv_heads), next_item = item_at(p, max(next_pair, 0) / p.kv_heads);
+    Item item = item_of(pair / p.kv_heads), next_item = item_of(max(next_pair, 0) / p.kv_heads);
     int base = item.key_begin;
     auto box_key = [&]() {
       const int key = base + lane * box_rows;
@@ -107,7 +110,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
         item = next_item;
         base = item.key_begin;
         next_pair = pair_of(round + 1);
-        next_item = item_at(p, max(next_pair, 0) / p.kv_heads);
+        next_item = item_of(max(next_pair, 0) / p.kv_heads);
       }
       key = box_key();
       page = page_of(key);
@@ -152,7 +155,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     }
   };
   int pair = pair_of(0);                               // the grid has at most as many CTAs as there are pairs
-  Item item = item_at(p, pair / p.kv_heads);
+  Item item = item_of(pair / p.kv_heads);
   uint4 q[EACH];
   query(item, pair % p.kv_heads, q);
   bool ok = true;
@@ -169,7 +172,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     for (int k = 0; k < EACH; k++) { const int idx = tid + k * COMPUTE; *(uint4*)(sQ + idx / PIECES * L::Q_STRIDE + idx % PIECES * 8) = q[k]; }
     compute_barrier();
     const int next_pair = pair_of(round + 1);
-    const Item next_item = item_at(p, max(next_pair, 0) / p.kv_heads);
+    const Item next_item = item_of(max(next_pair, 0) / p.kv_heads);
     if (next_pair >= 0) query(next_item, next_pair % p.kv_heads, q);
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[2 * MINE][4];
 #pragma unroll
@@ -289,13 +292,13 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
   end_items(p);
 }
 
-template <int HD>
+template <int HD, bool LATER>
 int launch(const CUtensorMap& map_k, const CUtensorMap& map_v, const Params& p, int items, int ctas, int box_rows, cudaStream_t stream) {
   using L = Layout<HD>;
-  if (reserve_shared<attention_prefix_stream_kernel<HD>>(L::SMEM, "attention_shared_prefix (few rows)")) return 1;
+  if (reserve_shared<attention_prefix_stream_kernel<HD, LATER>>(L::SMEM, "attention_shared_prefix (few rows)")) return 1;
   const long long pairs = (long long)items * p.kv_heads, most = (long long)L::CTAS * sprout_sm_count(), slots = ctas < most ? ctas : most;
   SPROUT_REQUIRE(pairs <= 0x7fffffffLL, "attention_shared_prefix: too many items");
-  sprout_launch(attention_prefix_stream_kernel<HD>, dim3((unsigned)(pairs < slots ? pairs : slots)), dim3(THREADS), L::SMEM, stream, map_k, map_v, p, (int)pairs, box_rows);
+  sprout_launch(attention_prefix_stream_kernel<HD, LATER>, dim3((unsigned)(pairs < slots ? pairs : slots)), dim3(THREADS), L::SMEM, stream, map_k, map_v, p, (int)pairs, box_rows);
   return sprout_check_launch("attention_shared_prefix (few rows)");
 }
 
@@ -309,5 +312,6 @@ int sprout_attention_prefix_stream(const Params& p, int items, int ctas, cudaStr
   CUtensorMap map_k, map_v;
   if (tensor_map(p.k_cache, (int)cache_rows, p.head_dim, p.head_dim, box_rows, &map_k)) return 1;
   if (tensor_map(p.v_cache, (int)cache_rows, p.head_dim, p.head_dim, box_rows, &map_v)) return 1;
-  return p.head_dim == 64 ? launch<64>(map_k, map_v, p, items, ctas, box_rows, stream) : launch<128>(map_k, map_v, p, items, ctas, box_rows, stream);
+  if (p.head_dim == 64) return p.stretch > 0 ? launch<64, true>(map_k, map_v, p, items, ctas, box_rows, stream) : launch<64, false>(map_k, map_v, p, items, ctas, box_rows, stream);
+  return p.stretch > 0 ? launch<128, true>(map_k, map_v, p, items, ctas, box_rows, stream) : launch<128, false>(map_k, map_v, p, items, ctas, box_rows, stream);
 }
