@@ -1052,7 +1052,8 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     of the plan's type; ``block_table`` int32 [requests, pages] holds what the plan was made of; ``positions`` int32 [tokens]: a token
     sees the keys up to its own, and a position that the plan does not serve sets a status bit (another step's plan).  float32 runs on CUDA
     cores with 32-bit products, bfloat16 on tensor cores for head sizes up to 128 in steps of 16.  ``scratch``: float32 memory of
-    ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own."""
+    ``plan.scratch_floats``, taken here when not given; calls that run at the same time need their own.  A capture of this call reads the
+    plan's arrays when it is replayed: the plan lives as long."""
     pages, index, dtype = k_cache.shape, q.get_device(), plan.dtype
     q_stride, out_stride, table_stride, table = q.stride(), out.stride(), block_table.stride(), block_table.shape
     if not (0 <= index == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == positions.get_device() == plan.device_index

@@ -200,7 +200,10 @@ class HostPlan:
 
     def __init__(self, tables, q_start, contexts, page_tokens: int, heads: int, kv_heads: int, tensor_cores: bool, slots: int, matrix_slots: int = 0, narrow_slots: int | None = None, head_dim: int = 64,
                  stretch: int = 0):
-        tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
+        try:
+            tables, q_start, contexts = (np.asarray(a) for a in (tables, q_start, contexts))
+        except (TypeError, ValueError) as error:             # ragged rows, or tensors of a device
+            raise PlanError(f"tables, starts and contexts are arrays on the host ({error})") from None
         if tables.ndim != 2 or q_start.ndim != 1 or contexts.ndim != 1 or len(contexts) == 0 or len(q_start) != len(contexts) + 1 or len(tables) < len(contexts):
             raise PlanError("a block table row and a context per request, and where each request's tokens start")
         if any(a.dtype.kind not in "iu" for a in (tables, q_start, contexts)):

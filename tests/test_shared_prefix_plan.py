@@ -231,3 +231,8 @@ def test_overlap_check():
     rows = torch.zeros(4, 10)
     assert kernels._overlap(rows[:, :3], rows[:, 5:]) and not kernels._overlap(rows[:2, 5:], rows[2:, :3])      # from the first to the last element
     assert not kernels._overlap(whole[3:3], whole)
+
+
+def test_ragged_tables_are_refused():
+    with pytest.raises(PlanError, match="arrays on the host"):
+        HostPlan([[1, 2], [3]], [0, 1, 2], [5, 5], 8, 4, 1, True, 60)

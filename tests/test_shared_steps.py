@@ -4,6 +4,7 @@ import random
 import numpy as np
 import pytest
 
+from sprout_lm_b200.engine import shared
 from sprout_lm_b200.engine.shared import shared_keys
 from sprout_lm_b200.sampling import uniform_for, verify_uniforms
 
@@ -43,6 +44,37 @@ def test_numbers_follow_the_output_index_alone():
     assert (accept[2:], draw[2:]) == verify_uniforms(5, "a", 12, 2)
     assert draw == [uniform_for(5, "a", 10 + i) for i in range(4)] and accept != draw
     assert all(0.0 <= u < 1.0 for u in accept + draw)
+
+
+class Request:
+    length, tables = 100, [[1, 2, 3]]
+
+
+class Entry:
+    def __init__(self, seq):
+        self.seq, self.tokens, self.want = seq, [5], [0]
+
+
+def test_when_a_capture_is_thought_of(monkeypatch):
+    """At 8, 16, 32 .. decode steps of the same requests; behind one's last step at once; a step launched ahead makes way for it."""
+    steps = shared.SharedPrefixSteps.__new__(shared.SharedPrefixSteps)
+    steps.sizes, steps.after, steps._seqs, steps._same, steps._graph, steps._base = {(4, 1, 64): 1}, 8, [], 0, None, []
+    asked = []
+    monkeypatch.setattr(steps, "_capture", lambda entries: asked.append(steps._same), raising=False)
+    entries = [Entry(Request()), Entry(Request())]
+    for _ in range(40):
+        ahead = steps.due(entries, behind=1)
+        assert steps.decode_graph(entries, True) is None
+        assert ahead == (asked[-1:] == [steps._same])
+    assert asked == [8, 16, 32]
+    assert steps.decode_graph(entries[::-1], True) is None and steps._same == 1          # their order is the plan's
+    steps._graph, steps._base = "captured", [100, 100]
+    assert steps.decode_graph(entries[::-1], True) == "captured" and steps.captured(entries, 0) is None
+    assert steps.captured(entries[::-1], shared.STRETCH) == "captured" and steps.captured(entries[::-1], shared.STRETCH + 1) is None
+    entries[0].seq.length = 99
+    assert steps.decode_graph(entries[::-1], False) is None and asked == [8, 16, 32]     # launched ahead: nothing is made
+    assert steps.decode_graph(entries[::-1], True) is None and asked == [8, 16, 32, steps._same]
+    assert steps.decode_graph(entries[:1], True) is None and steps._graph is None and not steps.due(entries[:1], behind=7)
 
 
 def test_engine_option_is_a_boolean():
