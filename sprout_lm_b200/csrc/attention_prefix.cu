@@ -59,8 +59,9 @@ attention_prefix_simple_kernel(const Params p) {
   float* s_m = sP + SIMPLE_ROWS * (SIMPLE_KEYS + 4);   // [16] maxima, sums, what a pass multiplies the outputs by
   float* s_l = s_m + SIMPLE_ROWS;
   float* s_a = s_l + SIMPLE_ROWS;
+  const Item planned = p.items[blockIdx.x];
   begin_items(p);
-  const Item item = item_at(p, blockIdx.x);
+  const Item item = in_step(p, planned);
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
   // a thread keeps its four columns and walks down the rows
@@ -215,8 +216,9 @@ attention_prefix_mma_kernel(const Params p) {
   __nv_bfloat16* sQ = (__nv_bfloat16*)(rows + 2 * KEYS);           // [ROWS][STRIDE]
   __nv_bfloat16* sK = sQ + L::ROWS * STRIDE;           // [KEYS][STRIDE]
   __nv_bfloat16* sV = sK + KEYS * STRIDE;
+  const Item planned = p.items[blockIdx.x];
   begin_items(p);
-  const Item item = item_at(p, blockIdx.x);
+  const Item item = in_step(p, planned);
   const int g = blockIdx.y, group = p.heads / p.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
   auto look_up = [&](int base) { return tid < KEYS && base + tid < item.key_end ? key_row(p, table, base + tid, g) : -1ll; };
@@ -412,7 +414,7 @@ attention_prefix_merge_kernel(const Params p) {
   __shared__ float s_max[MERGE_THREADS / 32];
   __shared__ float s_sum[WARPS > 1 ? WARPS : 1][PAIRS * 64 + 1];
   pdl_launch_dependents();
-  pdl_wait();
+  // What the items do not write is read before they are waited for: the stream's earlier kernels were done when the first of them began.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WARPS, group = p.heads / p.kv_heads;
   const long long row = (long long)blockIdx.x * ROWS + warp / WARPS;
   if (row >= (long long)p.tokens * p.heads) return;    // whole blocks where warps share a row
@@ -430,7 +432,6 @@ attention_prefix_merge_kernel(const Params p) {
   float m = -INFINITY, l = 0.f, sum[PAIRS][2];
 #pragma unroll
   for (int k = 0; k < PAIRS; k++) sum[k][0] = sum[k][1] = 0.f;
-  for (int part = first + lane; part < end; part += 32) m = fmaxf(m, __ldcg(&p.part_sum[(size_t)part * p.heads + head]).x);
   float score = -INFINITY;                             // of this lane's extra key
   long long at = -1;
   if (extra > 0) {
@@ -449,6 +450,26 @@ attention_prefix_merge_kernel(const Params p) {
       if (lane == j) score = dot * p.scale_log2;
     }
   }
+  pdl_wait();
+  // the warp's parts, every WARPS-th: a lane the sums of one in every 32, and the outputs of the first AHEAD, all on their way at a time
+  constexpr int AHEAD = 8 / PAIRS;
+  const int mine = (end - first - share + WARPS - 1) / WARPS;
+  auto sums_of = [&](int i) { return i < mine ? __ldcg(&p.part_sum[(size_t)(first + share + i * WARPS) * p.heads + head]) : make_float2(-INFINITY, 0.f); };
+  const float* from = p.part_out + ((size_t)(first + share) * p.heads + head) * p.head_dim;
+  float2 t[AHEAD][PAIRS];
+  auto fetch = [&](int part) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++)
+#pragma unroll
+      for (int k = 0; k < PAIRS; k++) {
+        const int c = k * 64 + lane * 2;
+        t[i][k] = part + i < mine && c < p.head_dim ? __ldcg((const float2*)(from + (size_t)(part + i) * WARPS * p.heads * p.head_dim + c)) : make_float2(0.f, 0.f);
+      }
+  };
+  float2 held = sums_of(lane);
+  fetch(0);
+  m = held.x;
+  for (int i = 32 + lane; i < mine; i += 32) m = fmaxf(m, sums_of(i).x);
   m = warp_max(fmaxf(m, score));
   if (WARPS > 1) {                                     // the extra keys' may be the largest
     if (lane == 0) s_max[warp] = m;
@@ -456,30 +477,16 @@ attention_prefix_merge_kernel(const Params p) {
 #pragma unroll
     for (int w = 0; w < WARPS; w++) m = fmaxf(m, s_max[w]);
   }
-  // 32 of the warp's parts at a time, a lane a part's factor; their outputs AHEAD at a time on their way
-  constexpr int AHEAD = 8 / PAIRS;
-  for (int base = first + share; base < end; base += 32 * WARPS) {
-    const int count = min(32, (end - base + WARPS - 1) / WARPS);
-    float factor = 0.f;
-    if (lane < count) {
-      const float2 ml = __ldcg(&p.part_sum[(size_t)(base + lane * WARPS) * p.heads + head]);
-      factor = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m);
-      l = fmaf(ml.y, factor, l);
-    }
-    const float* from = p.part_out + ((size_t)base * p.heads + head) * p.head_dim;
-    for (int part = 0; part < count; part += AHEAD) {
-      float2 t[AHEAD][PAIRS];
-#pragma unroll
-      for (int i = 0; i < AHEAD; i++)
-#pragma unroll
-        for (int k = 0; k < PAIRS; k++) {
-          const int c = k * 64 + lane * 2;
-          t[i][k] = part + i < count && c < p.head_dim ? __ldcg((const float2*)(from + (size_t)(part + i) * WARPS * p.heads * p.head_dim + c)) : make_float2(0.f, 0.f);
-        }
+  for (int base = 0; base < mine; base += 32) {        // 32 parts at a time, a lane a part's factor
+    if (base > 0) held = sums_of(base + lane);
+    const float factor = held.x == -INFINITY ? 0.f : exp2f(held.x - m);
+    l = fmaf(held.y, factor, l);
+    for (int part = base; part < min(base + 32, mine); part += AHEAD) {
+      if (part > 0) fetch(part);
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
         const float f = __shfl_sync(0xffffffffu, factor, (part + i) & 31);
-        if (part + i < count)
+        if (part + i < mine)
 #pragma unroll
           for (int k = 0; k < PAIRS; k++) { sum[k][0] = fmaf(t[i][k].x, f, sum[k][0]); sum[k][1] = fmaf(t[i][k].y, f, sum[k][1]); }
       }

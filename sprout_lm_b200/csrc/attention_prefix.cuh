@@ -55,9 +55,9 @@ __device__ __forceinline__ void begin_items(const Params& p) {
 __device__ __forceinline__ void end_items(const Params& p) { if (!p.first) pdl_wait(); }
 
 // An item as it is in this step: an open range ends with the member's first token, within the plan's bounds and never empty, whatever the
-// positions say.
-__device__ __forceinline__ Item item_at(const Params& p, int index) {
-  Item item = p.items[index];
+// positions say.  (The plan itself was there before the call; what a step's kernels write, positions, queries, block tables and the cache, is
+// read behind begin_items.)
+__device__ __forceinline__ Item in_step(const Params& p, Item item) {
   if (p.stretch > 0 && item.open) item.key_end = max(item.key_begin + 1, min(item.key_end, p.positions[p.order[item.token_begin]] + 1));
   return item;
 }

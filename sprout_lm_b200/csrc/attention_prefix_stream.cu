@@ -75,14 +75,23 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  begin_items(p);
-  __syncthreads();
   // pairs come longest first; a CTA takes one of every round, forwards and backwards in turn
   auto pair_of = [&](int round) {
     const long long index = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     return index < pairs ? (int)index : -1;
   };
-  auto item_of = [&](int at) { return LATER ? item_at(p, at) : p.items[at]; };
+  int pair = pair_of(0), next_pair = pair_of(1);       // the grid has at most as many CTAs as there are pairs
+  Item item = p.items[pair / p.kv_heads], next_item = p.items[max(next_pair, 0) / p.kv_heads];
+  begin_items(p);
+  if (LATER) {
+    item = in_step(p, item);
+    next_item = in_step(p, next_item);
+  }
+  __syncthreads();
+  auto item_of = [&](int pair) {
+    const Item planned = p.items[max(pair, 0) / p.kv_heads];
+    return LATER ? in_step(p, planned) : planned;
+  };
   auto gave_up = [&]() { *abort_flag = 1; atomicOr(p.status, SPROUT_STATUS_WAIT_TIMEOUT); };
   int steps = 0;                                       // whose copies were issued (the copying warp), or that were computed
   if (warp == 4) {
@@ -90,8 +99,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     // the step before waits and is copied.
     const uint32_t stages = smem_u32(smem);
     const int boxes = KEYS / box_rows;
-    int round = 0, pair = pair_of(0), next_pair = pair_of(1);
-    Item item = item_of(pair / p.kv_heads), next_item = item_of(max(next_pair, 0) / p.kv_heads);
+    int round = 0;
     int base = item.key_begin;
     auto box_key = [&]() {
       const int key = base + lane * box_rows;
@@ -112,7 +120,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
         item = next_item;
         base = item.key_begin;
         next_pair = pair_of(round + 1);
-        next_item = item_of(max(next_pair, 0) / p.kv_heads);
+        next_item = item_of(next_pair);
       }
       key = box_key();
       page = page_of(key);
@@ -156,8 +164,6 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
         q[k] = *(const uint4*)((const __nv_bfloat16*)p.q + (size_t)p.order[place_of_row(item, i, group)] * p.q_stride + (size_t)head_of_row(item, i, group, g) * HD + idx % PIECES * 8);
     }
   };
-  int pair = pair_of(0);                               // the grid has at most as many CTAs as there are pairs
-  Item item = item_of(pair / p.kv_heads);
   uint4 q[EACH];
   query(item, pair % p.kv_heads, q);
   bool ok = true;
@@ -173,8 +179,10 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
 #pragma unroll
     for (int k = 0; k < EACH; k++) { const int idx = tid + k * COMPUTE; *(uint4*)(sQ + idx / PIECES * L::Q_STRIDE + idx % PIECES * 8) = q[k]; }
     compute_barrier();
-    const int next_pair = pair_of(round + 1);
-    const Item next_item = item_of(max(next_pair, 0) / p.kv_heads);
+    if (round > 0) {
+      next_pair = pair_of(round + 1);
+      next_item = item_of(next_pair);
+    }
     if (next_pair >= 0) query(next_item, next_pair % p.kv_heads, q);
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[2 * MINE][4];
 #pragma unroll

@@ -89,8 +89,6 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   // rows of a stage that no copy fills must hold finite numbers: their probabilities are zero, and zero times a NaN is not
   for (int i = tid; i < NS * L::KV_BYTES / 16; i += THREADS) ((uint4*)sV)[i] = make_uint4(0, 0, 0, 0);
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
-  begin_items(p);
-
   const Item item = p.items[blockIdx.x];               // whole pages: never open
   const int g = blockIdx.y, group = p.heads / p.kv_heads;
   const int* table = p.block_table + (size_t)item.table * p.table_stride;
@@ -110,6 +108,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  begin_items(p);
   __syncthreads();
   int issued = 0;                                     // tiles whose copies were issued (copy warps)
   auto gave_up = [&]() { *abort_flag = 1; atomicOr(p.status, SPROUT_STATUS_WAIT_TIMEOUT); };
