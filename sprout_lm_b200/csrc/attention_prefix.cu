@@ -452,7 +452,7 @@ attention_prefix_merge_kernel(const Params p) {
   }
   pdl_wait();
   // the warp's parts, every WARPS-th: a lane the sums of one in every 32, and the outputs of the first AHEAD, all on their way at a time
-  constexpr int AHEAD = 8 / PAIRS;
+  constexpr int AHEAD = PAIRS <= 2 ? 8 : 4;
   const int mine = (end - first - share + WARPS - 1) / WARPS;
   auto sums_of = [&](int i) { return i < mine ? __ldcg(&p.part_sum[(size_t)(first + share + i * WARPS) * p.heads + head]) : make_float2(-INFINITY, 0.f); };
   const float* from = p.part_out + ((size_t)(first + share) * p.heads + head) * p.head_dim;

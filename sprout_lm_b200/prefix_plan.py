@@ -18,6 +18,14 @@ KEY_STEP = 128              # keys that a CTA takes at a time: ranges are whole 
 NARROW_ROWS, WIDE_ROWS, SIMPLE_ROWS, MATRIX_ROWS = 16, 64, 16, 256      # rows of an item of each kind
 MATRIX_FROM = 48            # rows of a segment
 MATRIX_US, MATRIX_STEP_US, NARROW_STEP_US = 8.0, 2.0, 2.0      # of items beside one another: a matrix item's start and step, a step of few rows
+# Microseconds on a B200 by kind (0: matrix, 2: 64 rows), at head sizes up to 64 and above: an item's start and its step of 128 keys, what a
+# launch takes beside; the step of a walk over items of few rows; a row's partial result, written and put together, and the chain of
+# reads that a part of a row adds.  Fitted to launches of 60 batches in ten forms each (kinds, ranges of 1 to 12 steps); over 35 others the
+# form that they choose takes 1 to 2 % more than the best of the ten.
+KIND_US = {0: ((0.6, 2.2), (2.5, 2.6)), 2: ((0.0, 5.0), (0.0, 7.5))}
+BESIDE_US = {0: (2.0, 0.5), 2: (1.0, 1.0)}
+WALK_US = 2.2
+PART_US, DEPTH_US = 2.6e-4, 0.05
 ITEM_STEPS = 0.5            # what an item of few rows costs beside its steps
 MAX_RANGES = 64             # of a segment
 MAX_STRETCH = 1024          # positions that a plan's steps may be behind its own: its items are sized for its own
@@ -99,10 +107,9 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
 def choose_kinds(rows, steps, whole, kv_heads: int, head_dim: int, slots: int, matrix_slots: int, narrow_slots: int) -> np.ndarray:
     """The kind of every segment: 0 where ``whole`` allows it (tiles of 256 rows on tcgen05), 1 (tiles of 16 rows) or 2 (of 64).  Segments of
     up to 16 rows are 1; of the four ways for the rest (0 or not where it may be, and 1 or 2 for all others) the one that a rough model of
-    the launches finds shortest.  Its constants are microseconds on a B200 at head size 64 and 128: a CTA's time for a step of 128 keys,
-    what it takes beside, and the partial results' way through memory.  Measured, head size 128: 20 requests over 16,384 keys
-    (28 heads over 4) as 0, 1, 2: 23.1, 48.4, 40.3 us; 24 of 4 tokens over 2,000: 26.4, 40.3, 33.4; 6 over 30,000 (40 over 8): -, 42.8,
-    56.0; head size 64 (14 over 2): 64 over 1,024: 12.0, 9.7, 11.3; 90 pairs of tokens over 1,000: 20.4, 17.6, 16.8."""
+    the launches finds shortest.  Measured, head size 128 as 0, 2, 1: 24 requests of up to 6 tokens over 2,000 keys (28 heads over 4) 21.7, 28.5,
+    36.5 us; 14 of 2 over two prompts of 5,000 (40 over 8) 18.8, 18.5, 20.9; 42 over six of 6,800 50, 61, 54; head size 64 (14 over 2): 64
+    over 4,096 15.3, 18.5, 19.7; 90 of 2 over six of 5,000 20.1, 24.0, 30.7; 10 of 5 over 230 12.9, 9.6, 8.4."""
     few = rows <= NARROW_ROWS
     if few.all():
         return np.ones(len(rows), dtype=np.int64)
@@ -113,53 +120,52 @@ def choose_kinds(rows, steps, whole, kv_heads: int, head_dim: int, slots: int, m
             kind = np.where(few, 1, others)
             if matrix:
                 kind[whole] = 0
-            cost = 0.0
-            for which, tile, places, beside, step in ((0, MATRIX_ROWS, matrix_slots, 6.5 if wide_head else 7.5, 2.0 if wide_head else 1.4), (2, WIDE_ROWS, slots, 3.5, 7.5 if wide_head else 3.5),
-                                                      (1, NARROW_ROWS, narrow_slots, 2.0, 2.7 if wide_head else 2.2)):
+            cost, walk = 0.0, walk_us(rows, steps, kind, kv_heads, narrow_slots)
+            for which, tile, places in ((0, MATRIX_ROWS, matrix_slots), (2, WIDE_ROWS, slots)):
                 of = kind == which
-                if not of.any():
-                    continue
-                tiles = -(-rows[of] // tile) * kv_heads
-                share = float((tiles * steps[of]).sum()) / places
-                length = max(1.0, share)
-                time = beside + step * (length + 0.75 if which == 1 else np.ceil(length))      # items of few rows are walked: some CTA has more
-                if which == 0:
-                    ctas = float((tiles * -(-steps[of] // np.ceil(length))).sum())
-                    alone, free = time, max(0.0, 1.0 - ctas / places)
-                elif matrix and free > 0:                # on the SMs that the matrix items leave, or behind them
-                    time = min(time, max(0.0, beside + step * (max(1.0, share / free) + 0.75) - alone))
-                cost += 1.0 + time
-                cost += float((rows[of] * -(-steps[of] // np.ceil(length))).sum()) * kv_heads * head_dim * 8 / 6e6
+                if of.any():
+                    time = divide(-(-rows[of] // tile), steps[of], rows[of], kv_heads, places, *KIND_US[which][wide_head], walk if which == 0 else None)[1]
+                    if which == 0:
+                        walk = None                          # beside or behind the matrix items, and counted with them
+                    elif walk is not None:                   # among the others
+                        time += max(0.0, walk[0] - 0.5 * time)
+                        walk = None
+                    cost += BESIDE_US[which][wide_head] + time
+            if walk is not None:
+                cost += walk[0]
             if best is None or cost < best[0]:
                 best = cost, kind
     return best[1]
 
 
-def divide(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int, start: float, step: float) -> np.ndarray:
-    """Into how many ranges each segment's keys go (``steps`` key steps, ``tiles`` tiles of rows), on a device that runs ``slots`` items at
-    once, an item of n steps taking ``start + n * step``: ranges of the length that makes the fewest full rounds of items the shortest."""
+def walk_us(rows, steps, kind, kv_heads: int, narrow_slots: int):
+    """What the items of few rows take with the device to themselves, and a function of the share of it that they have; None without any."""
+    of = kind == 1
+    if not of.any():
+        return None
+    share = float((-(-rows[of] // NARROW_ROWS) * kv_heads * steps[of]).sum()) / narrow_slots
+    parts = float((rows[of] * -(-steps[of] // np.ceil(max(1.0, share)))).sum()) * kv_heads * PART_US
+    time = lambda free: WALK_US * np.maximum(1.5, share / free + 1.25) + parts       # some CTA has more than its share
+    return time(1.0), time
+
+
+def divide(tiles: np.ndarray, steps: np.ndarray, rows: np.ndarray, kv_heads: int, slots: int, start: float, step: float, walk=None):
+    """Into how many ranges each segment's keys go (``steps`` key steps, ``tiles`` tiles of ``rows`` rows), on a device that runs ``slots`` items
+    at once, an item of n steps taking ``start + n * step``, and the time that takes: the rounds of items, what their partial results cost,
+    and what ``walk`` (``walk_us``) takes behind them, or beside them where they leave room."""
     if not len(tiles):
-        return steps
-    items = lambda n: int((tiles * np.minimum(-(-steps // n), MAX_RANGES)).sum()) * kv_heads
-    best = None
-    for rounds in range(1, 9):
-        low, high = 1, int(steps.max())                  # the shortest ranges whose items fit that many rounds
-        if items(high) > rounds * slots:
-            continue
-        while low < high:
-            middle = (low + high) // 2
-            if items(middle) <= rounds * slots:
-                high = middle
-            else:
-                low = middle + 1
-        cost = -(-items(low) // slots) * (start + low * step)
-        if best is None or cost < best[0]:
-            best = cost, low
-        if low == 1:
-            break
-    # more segments than eight rounds hold: an even share of the steps
-    length = best[1] if best is not None else max(1, -(-int((tiles * steps).sum()) * kv_heads // (8 * slots)))
-    return np.minimum(-(-steps // length), MAX_RANGES)
+        return steps, 0.0
+    most = int(steps.max())
+    lengths = np.unique(-(-most // np.arange(1, min(most, MAX_RANGES) + 1)))[:, None]
+    ranges = np.minimum(-(-steps // lengths), MAX_RANGES)
+    items = (tiles * ranges).sum(1) * kv_heads
+    time = -(-items // slots) * (start + step * (-(-steps // ranges)).max(1))
+    total = time + (rows * ranges).sum(1) * kv_heads * PART_US + np.minimum(ranges.max(1), 24) * DEPTH_US
+    if walk is not None:
+        free = np.maximum(1e-9, 1.0 - items / slots)
+        total += np.minimum(walk[0], np.maximum(0.0, walk[1](free) - time))
+    best = int(total.argmin())
+    return ranges[best], float(total[best])
 
 
 def spread(tiles: np.ndarray, steps: np.ndarray, kv_heads: int, slots: int) -> np.ndarray:
@@ -237,10 +243,11 @@ class HostPlan:
         tiles, steps = -(-rows // tile_rows), -(-(end - begin) // KEY_STEP)
         ranges = np.empty(len(segments), dtype=np.int64)
         matrix = kind == 0
-        ranges[matrix] = divide(tiles[matrix], steps[matrix], kv_heads, max(1, matrix_slots), 7.0, 2.4)
         if tensor_cores:
+            ranges[matrix] = divide(tiles[matrix], steps[matrix], rows[matrix], kv_heads, max(1, matrix_slots), *KIND_US[0][head_dim > 64],
+                                    walk_us(rows, steps, kind, kv_heads, narrow_slots or slots))[0]
             wide, narrow = kind == 2, kind == 1
-            ranges[wide] = divide(tiles[wide], steps[wide], kv_heads, slots, 4.0, 1.5)
+            ranges[wide] = divide(tiles[wide], steps[wide], rows[wide], kv_heads, slots, *KIND_US[2][head_dim > 64])[0]
             self.narrow_ctas = narrow_slots or slots
             ranges[narrow], most = spread(tiles[narrow], steps[narrow], kv_heads, self.narrow_ctas)
             ctas = int((tiles[matrix] * ranges[matrix]).sum()) * kv_heads
@@ -252,7 +259,7 @@ class HostPlan:
                 if max(alone_us, there * NARROW_STEP_US) < alone_us + most * NARROW_STEP_US:
                     ranges[narrow], self.narrow_ctas = apart, beside
         else:
-            ranges[:] = divide(tiles, steps, kv_heads, slots, 4.0, 1.5)
+            ranges[:] = divide(tiles, steps, rows, kv_heads, slots, 4.0, 1.5)[0]
         per_range = -(-steps // ranges)                  # steps of a range
         ranges = -(-steps // per_range)
         parts = np.zeros(self.tokens, dtype=np.int64)    # of each place
