@@ -403,9 +403,9 @@ attention_prefix_mma_kernel(const Params p) {
 // member's own tokens that the items leave out, a lane a key.  One warp for a row of few parts; a row of 35 parts in one warp is a chain
 // of five waits for memory.  What bounds it is those waits, and for many rows the parts' way out of L2: 128 tokens of 28 heads of 128 in 10
 // parts 9.6 us behind the items.
-// MERGE_FROM: parts a row, on average.  35 parts (64 tokens of 14 heads of 64): 20.5 us a call with four warps, 21.5 with one; 14 parts (135
-// tokens): 27.4 and 24.4; 10 parts (90 tokens of 28 heads of 128): 33.2 and 29.7.
-constexpr int MERGE_THREADS = 128, MERGE_SPLIT = 4, MERGE_FROM = 24;
+// MERGE_FROM: parts a row, on average.  13 parts (64 tokens of 14 heads of 64): 16.7 us a call with four warps, 15.4 with one; 23 (29 tokens
+// of 28 heads of 128): 20.3 and 23.2; 29 (11 tokens of 14 of 64): 9.0 and 10.3.
+constexpr int MERGE_THREADS = 128, MERGE_SPLIT = 4, MERGE_FROM = 20;
 
 template <typename T, int PAIRS, int WARPS>
 __global__ void __launch_bounds__(MERGE_THREADS)
