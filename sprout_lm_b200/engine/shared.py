@@ -21,14 +21,14 @@ from ..prefix_plan import MEMBER_TOKENS
 
 BYTES_PER_US = 6.4e6               # what attention streams keys and values at
 # A plan, for each request of it, and a layer's launches one by one beside a replay of them (measured: 64 requests of the 0.5B shape over
-# 4,096 shared keys take 1.55 ms a step as a replay and 4.3 with a plan of its own; over 32,768, 4.3 and 4.5)
+# 4,096 shared keys take 1.55 ms a step as a replay and 4.6 with a plan of its own; over 32,768, 4.4 and 4.5)
 PLAN_US, PLAN_REQUEST_US, EAGER_LAYER_US = 600.0, 10.0, 130.0
 # What of the reads' time is saved (the shared keys still meet every request's queries), and what a layer's attention takes longer otherwise.
-# Replayed steps of 64 requests without and with a plan: the 0.5B shape, 24 layers, over 1,024, 4,096 and 32,768 shared keys 1.14 and 1.15 ms,
-# 1.55 and 1.39, 4.35 and 1.94; of 8 over 4,096 and 16,384 0.74 and 0.81, 0.92 and 0.88; the 7B shape, 4 layers, 64 over 1,024 and 8,192
-# 0.84 and 0.80, 1.25 and 0.87.
-SAVED, REPLAY_LAYER_US = 0.6, 5.0
-CAPTURE_US, CAPTURE_LAYER_US = 1500.0, 300.0         # a capture beside its plan (the first step of the above: 8 to 25 ms)
+# Replayed steps of 64 requests without and with a plan: the 0.5B shape, 24 layers, over 1,024, 4,096 and 32,768 shared keys 1.14 and 1.11 ms,
+# 1.55 and 1.23, 4.36 and 1.65; of 8 over 4,096 and 16,384 0.74 and 0.77, 0.91 and 0.84; the 7B shape, 4 layers, 64 over 1,024 and 8,192
+# 0.84 and 0.79, 1.25 and 0.84.
+SAVED, REPLAY_LAYER_US = 0.7, 3.0
+CAPTURE_US, CAPTURE_LAYER_US = 1500.0, 300.0         # a capture beside its plan (the first step of the above: 10 to 30 ms)
 STRETCH = 128                      # steps that a captured one's plan serves behind its first
 
 
