@@ -287,6 +287,26 @@ def test_captured_generation_with_shared_prompts(model_dirs, monkeypatch):
         assert len(result["output"]) == 40 and nearly_greedy(model, model_dirs["B"], prompt, result["output"], "bfloat16")
 
 
+def test_captured_generation_in_a_pool_too_small(model_dirs, monkeypatch):
+    """Requests come, end and are thrown out and readmitted with other pages while captures over the shared ones are made and dropped."""
+    from sprout_lm_b200 import EngineOptions, generate, load_model, make_engine
+    from sprout_lm_b200.engine import shared
+    monkeypatch.setattr(shared, "STRETCH", 5)
+    model = load_model(model_dirs["B"], dtype="bfloat16")
+    rng = np.random.default_rng(61)
+    prefix = helpers.random_tokens(rng, 80, 509)
+    prompts = [prefix + helpers.random_tokens(rng, n, 509) for n in (1, 20, 9, 33, 14, 5, 27)]
+    engine = make_engine(model, EngineOptions(block_size=8, num_blocks=34, max_sequences=5, max_batch_tokens=64, prefill_chunk_size=48, shared_prefix=True))
+    steps = engine.runner.shared_prefix
+    steps.always, steps.after = True, 2
+    generate(model, prompts[:1], max_new_tokens=1, ignore_eos=True, engine=engine)      # publishes the prefix
+    results = generate(model, prompts, max_new_tokens=30, ignore_eos=True, engine=engine)
+    assert steps.steps > 0 and any(e["type"] == "preempted" for e in engine.trace)
+    for prompt, result in zip(prompts, results):
+        assert len(result["output"]) == 30 and nearly_greedy(model, model_dirs["B"], prompt, result["output"], "bfloat16")
+    engine.runner.check_status()
+
+
 def test_plans_are_taken_where_they_pay(model_dirs):
     """Without ``always``: not for a tiny model's short prompt."""
     from sprout_lm_b200 import load_model
