@@ -88,6 +88,7 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
   }
   // rows of a stage that no copy fills must hold finite numbers: their probabilities are zero, and zero times a NaN is not
   for (int i = tid; i < NS * L::KV_BYTES / 16; i += THREADS) ((uint4*)sV)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();                                 // before the copies that the barrier below lets go
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
   const Item item = p.items[blockIdx.x];               // whole pages: never open
   const int g = blockIdx.y, group = p.heads / p.kv_heads;
