@@ -72,7 +72,9 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
     def branch(members, start, depth, parent):
         groups = {}
         for member in members:
-            groups.setdefault(int(tables[request[member], depth]) if whole[member] > depth else -1 - int(member), []).append(member)
+            page = int(tables[request[member], depth]) if whole[member] > depth else -1
+            # by itself, under a key that is no page: it has no full page here, or one outside the pool (which the kernels skip and flag)
+            groups.setdefault(page if page >= 0 else -1 - int(member), []).append(member)
         left.extend((group, start, depth, parent) for group in reversed(groups.values()))
 
     branch(np.arange(len(request)), 0, 0, -1)
@@ -90,7 +92,7 @@ def find_segments(tables: np.ndarray, q_start: np.ndarray, contexts: np.ndarray,
         else:
             members = np.asarray(members)
             rows = tables[request[members], depth:int(whole[members].min())]
-            same = (rows == rows[0]).all(axis=0)
+            same = (rows == rows[0]).all(axis=0) & (rows[0] >= 0)
             end = depth + (int(same.argmin()) if not same.all() else rows.shape[1])
             if (len(members) - 1) * (end - start) * page_tokens >= max(MIN_SAVED_KEYS, PART_KEYS * group * int(tokens[members].sum())):
                 segments.append(Segment(int(request[members[0]]), start * page_tokens, end * page_tokens, placed))

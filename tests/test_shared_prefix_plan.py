@@ -236,3 +236,35 @@ def test_overlap_check():
 def test_ragged_tables_are_refused():
     with pytest.raises(PlanError, match="arrays on the host"):
         HostPlan([[1, 2], [3]], [0, 1, 2], [5, 5], 8, 4, 1, True, 60)
+
+
+@pytest.mark.timeout(60)
+@pytest.mark.parametrize("seed", range(12))
+def test_pages_outside_the_pool(seed):
+    """Negative pages inside contexts, beside requests of every length: the plan ends, and has every key once (the kernels skip and flag such
+    pages).  They are nobody's in common: runs end before them."""
+    rng = random.Random(seed)
+    page, group, kv_heads = rng.choice([1, 4, 16]), rng.choice([1, 4]), rng.choice([1, 2])
+    tables, q_start, contexts = batch(rng, rng.randint(2, 14), page, [rng.randint(1, 30) for _ in range(3)], rng.choice([[1], [1, 2, 5], [1, 17]]), 60)
+    for row, context in zip(tables, contexts):
+        for at in range(-(-int(context) // page)):
+            if rng.random() < (0.5 if at == 0 else 0.1):
+                row[at] = -rng.randint(1, 2 * len(tables))
+    if seed % 3 == 0:
+        tables[:, 1:2] = -1                               # all of them, in the same place
+    for tensor_cores in (True, False):
+        plan = HostPlan(tables, q_start, contexts, page, group * kv_heads, kv_heads, tensor_cores, 60, 148)
+        pairs = covered(plan, tables, group)
+        for place in range(plan.tokens):
+            request = int(plan.table_of[place])
+            for head in range(group):
+                keys = sorted((k, int(tables[table, k // page])) for _, begin, end, table in pairs[place, head] for k in range(begin, end))
+                assert keys == [(k, int(tables[request, k // page])) for k in range(plan.seen[place])]
+        for s in plan.segments:
+            assert s.own or (tables[s.table, s.key_begin // page:s.key_end // page] >= 0).all()
+
+
+@pytest.mark.timeout(60)
+def test_a_short_request_beside_a_negative_page():
+    plan = HostPlan([[5, 6, 7, 8], [-1, 9, 10, 11], [3, 4, 5, 6]], [0, 1, 2, 3], [3, 40, 40], 16, 8, 2, True, 60)
+    assert len(plan.segments) == 3 and plan.read_keys == 83
