@@ -86,9 +86,6 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
     end_items(p);
     return;
   }
-  // rows of a stage that no copy fills must hold finite numbers: their probabilities are zero, and zero times a NaN is not
-  for (int i = tid; i < NS * L::KV_BYTES / 16; i += THREADS) ((uint4*)sV)[i] = make_uint4(0, 0, 0, 0);
-  fence_proxy_async();                                 // before the copies that the barrier below lets go
   if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
   const Item item = p.items[blockIdx.x];               // whole pages: never open
   const int g = blockIdx.y, group = p.heads / p.kv_heads;
@@ -321,6 +318,21 @@ attention_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __gr
       tmem_store16(s_addr + half * (HALF / 2), packed);
       l2 = add2(l2, add2(sums[0], sums[1]));
       tmem_store_wait();
+      // V rows that no copy filled (behind the range's end, or of a page outside the pool) hold what lay there before, an infinity or a NaN
+      // of the ring's tile before among it: their probabilities are zero, but zero times those is not.  They are cleared once the copies
+      // have landed, by each Q tile before it signals its P; four threads a row.
+      if (there + half * HALF < KEYS || marks != 0) {
+        const int s = j % NS, key = row & (KEYS - 1), share = half * 2 + (row >> 6);
+        if (*abort_flag || !mbar_wait(&v_full[s], (j / NS) & 1, abort_flag)) gave_up();
+        if (key >= there + half * HALF || (marks >> (key / box_rows) & 1)) {
+#pragma unroll
+          for (int k = 0; k < DIM / 32; k++) {
+            const int c = share * (DIM / 32) + k;
+            *(uint4*)(sV + s * L::KV_BYTES + (c >> 3) * KV_ATOM + key * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async();
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[q * 2 + (j & 1)]);

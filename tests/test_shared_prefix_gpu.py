@@ -185,6 +185,31 @@ def test_nan_in_a_seen_key_is_not_lost(status):
     assert bool(out[3, :7, 9].isnan().all()) and int(out.isnan().sum()) == 7
 
 
+@pytest.mark.parametrize("page", [8, 16, 32])
+@pytest.mark.parametrize("dtype,ways", [(BF16, (0, 1)), (BF16, (2, 2)), (BF16, (1, 1)), (F32, (1, 1))])
+def test_an_infinite_value_stays_one(page, dtype, ways, monkeypatch, status):
+    """An infinity among the values that a row sees makes the column infinite, as the definition has it, where a range ends inside a tile and
+    where a page lies outside the pool: what an earlier tile left in shared memory there does not come into it."""
+    import sprout_lm_b200.prefix_plan as prefix_plan
+    monkeypatch.setattr(prefix_plan, "choose_kinds", lambda rows, steps, whole, *rest: np.where(rows <= 16, 1, np.where(whole, *ways)))
+    monkeypatch.setattr(prefix_plan, "divide", lambda tiles, steps, *rest: (np.ones_like(steps), 0.0))       # one range: ten tiles of 64 keys
+    step = Step(28, 4, 128, dtype, page, [0] * 24, [(9 * 64 + page) // page], [30] * 24, [1] * 24, seed=19)
+    if dtype == BF16:
+        assert (step.plan().host.matrix_items > 0) == (ways[0] == 0)
+    for tile in range(9):
+        for g, sign in ((1, 1.0), (2, -1.0)):
+            key = tile * 64 + 63                          # a row that no copy fills in the last tile
+            step.v[step.pages[0][key // page], g, key % page, 40 + g] = sign * float("inf")
+    out, (want, tol) = step.run(status).double(), step.exact()
+    infinite = want.isinf()
+    assert int(infinite.sum()) == 24 * 7 * 2 and bool((out[infinite] == want[infinite]).all())
+    assert bool(((out - want).abs()[~infinite] <= tol[~infinite]).all()) and int(status.item()) == 0
+    step.tables[:, (6 * 64 + 63) // page] = step.k.shape[0]
+    step.block_table.copy_(torch.from_numpy(step.tables))
+    out = step.run(status).double()
+    assert bool((out[infinite] == want[infinite]).all()) and bool(out[~infinite].isfinite().all()) and int(status.item()) == 1
+
+
 def test_large_scores(status):
     """Scores of hundreds either way: the running maximum carries them."""
     step = Step(14, 2, 64, BF16, 16, [0] * 6, [40], [5, 9, 0, 30, 200, 77], [1] * 6, seed=8, sharp=60.0)
