@@ -48,6 +48,8 @@ def shared_keys(table: np.ndarray, whole: np.ndarray, page_tokens: int) -> int:
 class SharedPrefixSteps:
     """Decides for a runner's steps; ``always`` takes a plan whenever pages are shared (tests)."""
 
+    _width = float("inf")                  # of the captured step's block tables, in pages
+
     def __init__(self, runner):
         self.runner = runner
         self.always = False
@@ -101,8 +103,10 @@ class SharedPrefixSteps:
         return len(entries) == len(self._seqs) and all(e.seq is s for e, s in zip(entries, self._seqs))
 
     def captured(self, entries, shift: int = 0):
-        """The step captured over these requests' shared pages if it serves them ``shift`` tokens on, else None."""
-        if self._graph is not None and self._are(entries) and all(0 <= e.seq.length + shift - n <= STRETCH for e, n in zip(entries, self._base)):
+        """The step captured over these requests' shared pages if it serves them ``shift`` tokens on, else None: their lengths are within its
+        plan's, and their block tables (a caller may have reserved far ahead meanwhile) within its width."""
+        if self._graph is not None and self._are(entries) and all(0 <= e.seq.length + shift - n <= STRETCH for e, n in zip(entries, self._base)) \
+                and all(len(t) <= self._width for e in entries for t in e.seq.tables):
             return self._graph
         return None
 
@@ -138,7 +142,7 @@ class SharedPrefixSteps:
         multiple = runner.graphs.page_multiple
         width = -(-max(-(-longest // page_tokens), *(len(t) for e in entries for t in e.seq.tables)) // multiple) * multiple
         plans = self._plans(table, np.arange(len(entries) + 1), contexts, STRETCH)
-        self._base = [e.seq.length for e in entries]
+        self._base, self._width = [e.seq.length for e in entries], width
         self._graph = DecodeGraph(runner, len(entries), width, min(width * page_tokens, -(-longest // 128) * 128), plans)
         return self._graph
 

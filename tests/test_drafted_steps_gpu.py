@@ -267,6 +267,40 @@ def test_captured_steps_over_a_shared_prompt(model_dirs, name, monkeypatch):
     runner.check_status()
 
 
+@pytest.mark.parametrize("ahead", [False, True])
+def test_pages_reserved_beyond_a_captured_step(model_dirs, ahead):
+    """Between two decode steps over a capture the caller reserves more pages than the capture's tables hold: the steps go on, over a capture
+    made for them."""
+    from sprout_lm_b200 import load_model
+    from sprout_lm_b200.engine.batch import StepEntry
+    directory = model_dirs["wide"]
+    model = load_model(directory, dtype="bfloat16")
+    page, vocab = 8, model.spec.vocab_size
+    rng = np.random.default_rng(67)
+    prefix = helpers.random_tokens(rng, 11 * page + 3, vocab)
+    tails = [helpers.random_tokens(rng, n, vocab) for n in (1, 9, 30)]
+    runner, seqs = started(model, prefix, tails, page)
+    steps = runner.shared_prefix
+    steps.after = 2
+    histories, graphs = [prefix + tail for tail in tails], []
+    new = [int(t) for t in rng.integers(vocab, size=3)]
+    for i in range(8):
+        if i == 4:
+            assert runner.reserve(seqs[1], steps._graph.table_pages * page + 1)
+        then = ([StepEntry(seq, [0], [0]) for seq in seqs], [0.0] * 3, [0.0] * 3, [0, 1, 2]) if ahead else None
+        sampled = runner.step_and_sample([StepEntry(seq, [t], [0]) for seq, t in zip(seqs, new)], [0.0] * 3, [0.0] * 3, then=then)
+        for history, t in zip(histories, new):
+            history.append(t)
+        new = sampled
+        graphs.append(steps._graph)
+    assert graphs[2] is graphs[3] is not None and graphs[5] is not graphs[3] and graphs[5] is graphs[7] is not None
+    assert runner.ahead_used > 0 or not ahead
+    for tail, history in zip(tails, histories):
+        at = len(prefix) + len(tail) + 1                  # what the model said behind each of its tokens
+        assert nearly_greedy(model, directory, history[:at], history[at:], "bfloat16")
+    runner.check_status()
+
+
 def test_captured_generation_with_shared_prompts(model_dirs, monkeypatch):
     """The same through the scheduler, whose steps are launched ahead."""
     from sprout_lm_b200 import EngineOptions, generate, load_model, make_engine

@@ -82,3 +82,19 @@ def test_engine_option_is_a_boolean():
     EngineOptions(shared_prefix=True).validate()
     with pytest.raises(ValueError, match="shared_prefix must be a boolean"):
         EngineOptions(shared_prefix=1).validate()
+
+
+def test_a_capture_serves_tables_within_its_width(monkeypatch):
+    """A caller may reserve pages far ahead (a device-side loop does): the captured step, whose tables have a fixed width, is not taken then, now
+    or ahead, and the next is thought of at once."""
+    steps = shared.SharedPrefixSteps.__new__(shared.SharedPrefixSteps)
+    steps.sizes, steps.after, steps._seqs, steps._same, steps._base, steps._width = {(4, 1, 64): 1}, 8, [], 0, [100, 100], 4
+    monkeypatch.setattr(steps, "_capture", lambda entries: "another", raising=False)
+    entries = [Entry(Request()), Entry(Request())]
+    steps._seqs, steps._graph = [e.seq for e in entries], "captured"
+    assert steps.captured(entries) == steps.captured(entries, 1) == "captured"
+    entries[1].seq.tables = [[1, 2, 3, 4]]
+    assert steps.captured(entries) == "captured"
+    entries[1].seq.tables = [[1, 2, 3, 4, 5]]
+    assert steps.captured(entries) is None and steps.captured(entries, 1) is None
+    assert steps.due(entries, behind=1) and steps.decode_graph(entries, True) == "another"
