@@ -11,6 +11,7 @@
 // bfloat16 and head sizes up to 128, from attention_prefix_mma_kernel (mma.sync), for few rows of most caches from
 // attention_prefix_stream.cu and for many rows over whole pages from attention_prefix_tcgen05.cu; one launch adds them up.
 #include <algorithm>
+#include <atomic>
 
 #include "attention_bf16.cuh"
 #include "attention_prefix.cuh"
@@ -416,7 +417,7 @@ attention_prefix_merge_kernel(const Params p) {
   __shared__ float s_max[MERGE_THREADS / 32];
   __shared__ float s_sum[WARPS > 1 ? WARPS : 1][PAIRS * 64 + 1];
   pdl_launch_dependents();
-  // What the items do not write is read before they are waited for: the stream's earlier kernels were done when the first of them began.
+  // What the items do not write is read before they are waited for: behind the gate, and the plan before it.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % WARPS, group = p.heads / p.kv_heads;
   const long long row = (long long)blockIdx.x * ROWS + warp / WARPS;
   if (row >= (long long)p.tokens * p.heads) return;    // whole blocks where warps share a row
@@ -425,6 +426,7 @@ attention_prefix_merge_kernel(const Params p) {
   // how far the step is behind the plan's own; outside what the plan serves it is another step's
   const int extra = share == 0 ? p.extra[place] : 0;
   int seen = p.seen[place];
+  pass_gate(p);
   if (share == 0 && head == 0 && lane == 0) {
     const int ahead = p.positions[token] - (seen + extra - 1);
     if (ahead < 0 || ahead > p.stretch) atomicOr(p.status, SPROUT_STATUS_BAD_POSITION);        // a step that the plan does not serve
@@ -453,6 +455,7 @@ attention_prefix_merge_kernel(const Params p) {
     }
   }
   pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.gate = 0;
   // the warp's parts, every WARPS-th: a lane the sums of one in every 32, and the outputs of the first AHEAD, all on their way at a time
   constexpr int AHEAD = PAIRS <= 2 ? 8 : 4;
   const int mine = (end - first - share + WARPS - 1) / WARPS;
@@ -604,20 +607,21 @@ struct PrefixPlan {
 };
 static_assert(sizeof(PrefixPlan) == 6 * 8 + 14 * 4, "as ctypes lays it out");
 
-// part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads.
+// part_out holds parts * heads * head_dim floats, part_sum as many pairs as parts * heads; gate is a word of 64 bits, whatever is in it.
 SPROUT_API int sprout_attention_prefix(const PrefixPlan* plan, const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* block_table, int table_stride,
-                                       const int* positions, float* part_out, float* part_sum, void* out, long long out_stride, int num_pages, int* status, cudaStream_t stream) {
+                                       const int* positions, float* part_out, float* part_sum, unsigned long long* gate, void* out, long long out_stride, int num_pages, int* status, cudaStream_t stream) {
   SPROUT_REQUIRE(plan && q && k_cache && v_cache && block_table && positions && plan->items && plan->order && plan->part_start && plan->seen && plan->extra && plan->table_of && part_out &&
-                 part_sum && out && status, "attention_shared_prefix: null pointer");
+                 part_sum && gate && out && status, "attention_shared_prefix: null pointer");
   const int simple_items = plan->simple_items, matrix_items = plan->matrix_items, narrow_items = plan->narrow_items, narrow_ctas = plan->narrow_ctas, wide_items = plan->wide_items;
   const int dtype = plan->dtype, tokens = plan->tokens, parts = plan->parts, heads = plan->heads, kv_heads = plan->kv_heads, head_dim = plan->head_dim, page_tokens = plan->page_tokens;
   SPROUT_REQUIRE(tokens > 0 && parts > 0 && plan->stretch >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0 && page_tokens > 0 && num_pages > 0,
                  "attention_shared_prefix: bad sizes tokens=%d heads=%d/%d head_dim=%d page=%d", tokens, heads, kv_heads, head_dim, page_tokens);
   SPROUT_REQUIRE(simple_items >= 0 && matrix_items >= 0 && narrow_items >= 0 && wide_items >= 0 && (narrow_items == 0 || narrow_ctas > 0) && (simple_items > 0) != (matrix_items + narrow_items + wide_items > 0), "attention_shared_prefix: bad item counts");
   SPROUT_REQUIRE(dtype == SPROUT_F32 || dtype == SPROUT_BF16, "attention_shared_prefix: bad dtype %d", dtype);
-  SPROUT_REQUIRE(((uintptr_t)part_out & 15) == 0 && ((uintptr_t)part_sum & 7) == 0, "attention_shared_prefix: the partial results must start on 16- and 8-byte boundaries");
+  SPROUT_REQUIRE(((uintptr_t)part_out & 15) == 0 && ((uintptr_t)part_sum & 7) == 0 && ((uintptr_t)gate & 7) == 0, "attention_shared_prefix: the partial results must start on 16- and 8-byte boundaries");
+  static std::atomic<uint32_t> calls{0};
   Params p{q, q_stride, k_cache, v_cache, block_table, table_stride, positions, plan->items, plan->order, plan->part_start, plan->seen, plan->extra, plan->table_of, part_out, (float2*)part_sum, out, out_stride,
-           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, plan->stretch, 1};
+           tokens, heads, kv_heads, head_dim, page_tokens, num_pages, 1.4426950408889634f / sqrtf((float)head_dim), status, plan->stretch, 1, gate, 0x7fd5acedull << 32 | calls.fetch_add(1, std::memory_order_relaxed)};
   if (simple_items > 0) {
     // rows that are whole fours on their boundaries
     const int row = dtype == SPROUT_F32 ? 16 : 8;

@@ -98,6 +98,7 @@ attention_prefix_stream_kernel(const __grid_constant__ CUtensorMap map_k, const 
     // lane b copies box b of a step, keys and values; lane 0 waits for the stage and posts the bytes.  The page of a step is looked up while
     // the step before waits and is copied.
     const uint32_t stages = smem_u32(smem);
+    asm volatile("fence.proxy.async.global;" ::: "memory");        // the gate told ordinary accesses of the cache's writes, the copies go another way
     const int boxes = KEYS / box_rows;
     int round = 0;
     int base = item.key_begin;

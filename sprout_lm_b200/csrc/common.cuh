@@ -39,7 +39,9 @@ extern "C" int sprout_sm_count();
 // loads of weights and tables) and calls pdl_wait() before it reads or writes anything an
 // earlier kernel may have written.  pdl_wait() returns once all earlier kernels have completed
 // and their writes are visible; every block executes it, so a kernel never completes before its
-// predecessors.  sprout_set_pdl(0) turns the launch attribute off (the calls then do nothing).
+// predecessors.  That a kernel starts after some earlier one has ended makes nothing visible to it: the launches of
+// attention_prefix.cuh, which start so, hand on what the first of them waited for by a release and an acquire of their own.
+// sprout_set_pdl(0) turns the launch attribute off (the calls then do nothing).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

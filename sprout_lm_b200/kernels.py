@@ -41,7 +41,7 @@ _SIGNATURES = {
     "sprout_attention_tile": [_P, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "sprout_sample": [_P, _I, _P, _P, _P, _P, _I, _I, _P, _P],
     "sprout_attention_prefix_tc_supported": [_I, _I],
-    "sprout_attention_prefix": [_P, _P, _L, _P, _P, _P, _I, _P, _P, _P, _P, _L, _I, _P, _P],
+    "sprout_attention_prefix": [_P, _P, _L, _P, _P, _P, _I, _P, _P, _P, _P, _P, _L, _I, _P, _P],
     "sprout_attention_prefix_mma_supported": [_I],
     "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
@@ -982,8 +982,9 @@ class SharedPrefixPlan:
         self.arguments = _PrefixPlan(*(base + 4 * at for at, _ in host.offsets), host.simple_items, host.matrix_items, host.narrow_items, host.narrow_ctas,
                                      host.wide_items, _dtype_code(dtype), host.tokens, host.parts, heads, kv_heads, head_dim, page_tokens, host.stretch, 0)
         self.address, self.device_index = ctypes.addressof(self.arguments), buffer.get_device()
-        self.scratch_floats = host.parts * heads * (head_dim + 2)          # the partial results, then their maxima and sums
-        self.sums_at = 4 * host.parts * heads * head_dim                   # bytes
+        # the partial results, then their maxima and sums, then the gate between a call's launches (csrc/attention_prefix.cuh); places in bytes
+        self.scratch_floats = host.parts * heads * (head_dim + 2) + 2
+        self.sums_at, self.gate_at = 4 * host.parts * heads * head_dim, 4 * host.parts * heads * (head_dim + 2)
         # what a call's tensors have to be
         self.rows, self.page, self.token_shape, self.item_bytes = (host.tokens, heads * head_dim), (kv_heads, page_tokens, head_dim), (host.tokens,), dtype.itemsize
 
@@ -1075,7 +1076,7 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
         raise KernelError(f"attention_shared_prefix: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
     at = scratch.data_ptr()
     _run("sprout_attention_prefix", plan.address, q_at, q_stride[0], k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), table_stride[0],
-         positions.data_ptr(), at, at + plan.sums_at, out_at, out_stride[0], pages[0], status.data_ptr(), _stream())
+         positions.data_ptr(), at, at + plan.sums_at, at + plan.gate_at, out_at, out_stride[0], pages[0], status.data_ptr(), _stream())
 
 
 def sample(logits, out, status, temperature=None, uniform=None):

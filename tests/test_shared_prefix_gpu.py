@@ -296,6 +296,34 @@ def test_launches_one_behind_the_other(status):
     step.check(status)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_chain_of_calls_each_reading_the_one_before(dtype, status):
+    """Each call's queries are the outputs of the call before, in scratch that all of them share, whatever was in it: the same bits as launches
+    that follow one another.  The gate between a call's launches is shut behind each."""
+    from sprout_lm_b200 import kernels
+    step = Step(14, 2, 64, dtype, 16, [0] * 30, [200], list(range(0, 600, 20)), [1, 2, 3] * 10, seed=20)
+    plan = step.plan()
+    assert dtype == F32 or plan.host.matrix_items > 0 and plan.host.narrow_items > 0
+    scratch = torch.full((plan.scratch_floats,), float("nan"), device=DEV)
+
+    def chain():
+        outs, q = [torch.empty_like(step.q) for _ in range(25)], step.q
+        for out in outs:
+            kernels.attention_shared_prefix(q, step.k, step.v, step.block_table, step.positions, plan, out, status, scratch)
+            q = out
+        return outs
+
+    try:
+        kernels.set_pdl(False)
+        want = chain()
+    finally:
+        kernels.set_pdl(True)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(chain(), want))
+        assert scratch[-2:].tolist() == [0.0, 0.0]
+    assert int(status.item()) == 0
+
+
 def test_two_calls_at_once(status):
     """Calls of one plan on two streams, each with scratch of its own, while a third runs on the current one."""
     step = Step(28, 4, 128, BF16, 16, [0] * 20, [300], list(range(0, 400, 20)), [1] * 20, seed=16)
