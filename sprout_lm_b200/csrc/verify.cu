@@ -118,6 +118,7 @@ struct Args {
   Chosen* chosen; Sums* sums;                          // [requests], [requests, runs]
   int rows, draft_rows, requests, vocab, per_row, runs;            // pieces and runs of a row
   int items;                                           // pieces that a warp of the first kernel takes
+  int fill;                                            // out holds nothing yet: -1 where no request writes
 };
 
 // The temperature of the request that row `row` (a draft row from p.rows on) belongs to: the last whose rows (draft rows: one fewer
@@ -145,6 +146,7 @@ verify_rows_kernel(const Args p) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (p.fill) for (long long i = (long long)blockIdx.x * THREADS + threadIdx.x; i < p.rows; i += (long long)gridDim.x * THREADS) p.out[i] = -1;
   const long long all = (long long)(p.rows + p.draft_rows) * p.per_row, first = ((long long)blockIdx.x * WARPS + warp) * p.items;
   if (first >= all) return;
   const int items = (int)min((long long)p.items, all - first);
@@ -527,10 +529,11 @@ SPROUT_API long long sprout_verify_scratch_bytes(int rows, int requests, int voc
 }
 
 // Request r's rows are row_start[r] .. row_start[r + 1] - 1 of `logits` [rows, vocab], at least one; its draft rows, one fewer, begin at
-// row_start[r] - r of `draft_logits` (null with draft_rows 0: the drafts have no distribution).  temperature, accept and draw may be null
+// row_start[r] - r of `draft_logits` (null with draft_rows 0: the drafts have no distribution).  Rows of `out` that are no request's, or of one
+// that is flagged for its rows, become -1 with `fill` and stay as they are without.  temperature, accept and draw may be null
 // together (all requests greedy).  Row i of `drafts` is the token drafted after row i's place; a request's last is not read.
 SPROUT_API int sprout_verify(const float* logits, long long ld, const float* draft_logits, long long draft_ld, const int* drafts, const int* row_start,
-                             const float* temperature, const float* accept, const float* draw, int* out, int* accepted, void* scratch,
+                             const float* temperature, const float* accept, const float* draw, int* out, int fill, int* accepted, void* scratch,
                              int rows, int draft_rows, int requests, int vocab, int* status, cudaStream_t stream) {
   SPROUT_REQUIRE(rows > 0 && requests > 0 && requests <= rows && vocab > 0 && vocab <= 1 << 30 && ld >= 0, "verify: bad sizes rows=%d requests=%d vocab=%d ld=%lld", rows, requests, vocab, ld);
   SPROUT_REQUIRE(draft_rows == 0 || (draft_rows == rows - requests && draft_logits && draft_ld >= 0), "verify: a draft row per drafted token");
@@ -540,7 +543,7 @@ SPROUT_API int sprout_verify(const float* logits, long long ld, const float* dra
   const long long per_row = pieces_of(vocab), runs = runs_of(vocab), all = per_row * (rows + (long long)draft_rows);
   SPROUT_REQUIRE(rows + (long long)draft_rows <= 0x7fffffffLL && runs * requests <= 0x7fffffffLL, "verify: too many rows");
   Args p{logits, draft_logits, ld, draft_ld, row_start, temperature, drafts, accept, draw, out, accepted, status, nullptr, nullptr, nullptr,
-         rows, draft_rows, requests, vocab, (int)per_row, (int)runs, 0};
+         rows, draft_rows, requests, vocab, (int)per_row, (int)runs, 0, fill};
   uint8_t* at = (uint8_t*)scratch;
   p.pieces = (PieceSum*)at;
   at += aligned16(all * (long long)sizeof(PieceSum));

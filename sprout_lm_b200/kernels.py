@@ -43,7 +43,7 @@ _SIGNATURES = {
     "sprout_attention_prefix_tc_supported": [_I, _I],
     "sprout_attention_prefix": [_P, _P, _L, _P, _P, _P, _I, _P, _P, _P, _P, _P, _L, _I, _P, _P],
     "sprout_attention_prefix_mma_supported": [_I],
-    "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
+    "sprout_verify": [_P, _L, _P, _L, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _P, _P],
     "sprout_advance_decode": [_P, _P, _P, _P, _P, _P, _I, _I, _P],
     "sprout_feed_tokens": [_P, _P, _P, _I, _I, _I, _P],
     "sprout_attention_decode": [_P, _I, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
@@ -1167,7 +1167,9 @@ def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperat
     ties), then the argmax follows.
 
     ``out`` (int32 [rows]): the drafts that stand, the token after them, and -1 in the rest of the request's rows; ``accepted`` (int32
-    [requests]): how many stand; both are made here unless given.  A row that is reached and holds a non-finite logit, or a draft outside
+    [requests]): how many stand; both are made here unless given.  A request whose rows lie outside the step's sets a status bit and has -1
+    accepted; its rows of ``out``, and those that are no request's, are -1 where ``out`` is made here and stay as they were where it is
+    given.  A row that is reached and holds a non-finite logit, or a draft outside
     the vocabulary, sets a status bit and leaves -1 from there on; rows behind the first draft that falls are not looked at."""
     rows, requests, index, shape, strides = drafts.numel(), row_start.numel() - 1, logits.get_device(), logits.shape, logits.stride()
     draws, per_row, per_request = temperatures is not None, (rows,), (requests,)
@@ -1185,14 +1187,15 @@ def verify_drafts(logits, drafts, row_start, status, draft_logits=None, temperat
         _check_verify(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw, out, accepted)
     vocab = shape[1]
     draft_rows = rows - requests if draft_logits is not None else 0          # none where nobody drafted anything
-    if out is None:
+    fill = out is None
+    if fill:
         out = drafts.new_empty(rows)
     if accepted is None:
         accepted = drafts.new_empty(requests)
     scratch = logits.new_empty((_lib or load_library()).sprout_verify_scratch_bytes(rows + draft_rows, requests, vocab), dtype=torch.uint8)
     _run("sprout_verify", logits.data_ptr(), strides[0], draft_logits.data_ptr() if draft_rows else None,
          draft_logits.stride(0) if draft_rows else 0, drafts.data_ptr(), row_start.data_ptr(), temperatures.data_ptr() if draws else None,
-         accept.data_ptr() if draws else None, draw.data_ptr() if draws else None, out.data_ptr(), accepted.data_ptr(),
+         accept.data_ptr() if draws else None, draw.data_ptr() if draws else None, out.data_ptr(), fill, accepted.data_ptr(),
          scratch.data_ptr(), rows, draft_rows, requests, vocab, status.data_ptr(), _stream())
     return out, accepted
 

@@ -298,6 +298,42 @@ def test_rows_of_nobody_stay(status):
         status.zero_()
 
 
+@pytest.mark.parametrize("greedy", [False, True])
+def test_no_row_of_the_result_is_left_unwritten(greedy, status):
+    """Rows that are no request's, or of a request whose rows lie outside the step's, are -1 in tokens that the call makes: memory that held
+    something else before shows nothing of it."""
+    from sprout_lm_b200 import sampling
+    c = case([2, 1, 3, 0, 4], 3000, seed=3, model=False)
+    args, more = on_device(c)
+    more = {} if greedy else {name: t for name, t in more.items() if t is not None}
+    whole, _ = sampling.verify(*args, status, **more)
+    whole, starts = whole.tolist(), args[2].tolist()
+    rows = args[1].numel()
+    for change in (lambda s: s[:4], lambda s: s[1:], lambda s: [*s[:5], rows + 1], lambda s: [-1, *s[1:]], lambda s: [*s[:2], s[1], *s[3:]]):
+        start = change(list(starts))
+        requests = len(start) - 1
+        torch.cuda.synchronize()
+        for n in (rows, requests):                        # what the call is likely to be given by the allocator
+            torch.full((n,), 1234567, dtype=torch.int32, device=DEV)
+        status.zero_()
+        per_request = {name: t[:requests].contiguous() if name == "temperatures" else t for name, t in more.items()}
+        if start[0] == starts[1] and not greedy:
+            per_request["temperatures"] = more["temperatures"][1:].contiguous()
+        tokens, accepted = sampling.verify(args[0], args[1], torch.tensor(start, dtype=torch.int32, device=DEV), status, **per_request)
+        want, flagged = [-1] * rows, 0
+        for r, (a, b) in enumerate(zip(start, start[1:])):
+            if 0 <= a < b <= rows:
+                if a in starts and b in starts and starts.index(b) == starts.index(a) + 1:
+                    want[a:b] = whole[a:b]
+                else:
+                    want[a:b] = tokens[a:b].tolist()      # rows of two requests taken as one's: written, whatever the answer
+                    assert 1234567 not in want[a:b]
+            else:
+                flagged = 64
+                assert int(accepted[r]) == -1
+        assert tokens.tolist() == want and int(status.item()) & 64 == flagged
+
+
 def test_distribution_of_the_first_token(status):
     """Whatever the draft model, the first emitted token is distributed as the target's: 40,000 requests, each frequency within five
     standard deviations (the binomial's)."""
