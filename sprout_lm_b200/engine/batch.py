@@ -45,7 +45,13 @@ class StepContext:
     # captured graph, that of the steps it is replayed for (0: max_context)
     planned_context: int = 0
     context_total: int = 0          # the requests' contexts together, as the step was staged (0: not known)
-    shared: dict | None = None      # plans of the requests' shared pages by attention sizes (``engine.shared``), for parts that take them
+    shared: dict | None = None      # ``engine.shared.Plans`` of the requests' shared pages, for parts that take them (``shared_plan``)
+
+    def shared_plan(self, sizes, block_table):
+        """The plan for attention of these sizes whose pages are ``block_table``'s (one of ``block_tables``), or None."""
+        if self.shared is None or block_table is not self.block_tables[self.shared.group]:
+            return None
+        return self.shared.get(sizes)
 
     @property
     def all_decode(self) -> bool:

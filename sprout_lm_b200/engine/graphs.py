@@ -67,7 +67,7 @@ class DecodeGraph:
     RING = 3            # pinned buffers per graph: more launches than two are never in flight
 
     def __init__(self, runner, requests: int, table_pages: int, planned_context: int = 0, shared=None):
-        """``shared``: plans of shared pages by attention sizes, for all steps that the capture is replayed for (``engine.shared``)."""
+        """``shared``: plans of shared pages (``engine.shared.Plans``) for all steps that the capture is replayed for."""
         self.runner = runner
         self.requests = R = requests
         self.table_pages = table_pages

@@ -45,6 +45,14 @@ def shared_keys(table: np.ndarray, whole: np.ndarray, page_tokens: int) -> int:
     return saved
 
 
+class Plans(dict):
+    """{(query heads, key/value heads, head size): plan} for the layers whose pages are those of page group ``group``."""
+
+    def __init__(self, group: int, plans):
+        super().__init__(plans)
+        self.group = group
+
+
 class SharedPrefixSteps:
     """Decides for a runner's steps; ``always`` takes a plan whenever pages are shared (tests)."""
 
@@ -95,8 +103,8 @@ class SharedPrefixSteps:
         return sum(n * kv_heads * head_dim * 4 for (_, kv_heads, head_dim), n in self.sizes.items())
 
     def _plans(self, table, q_start, contexts, stretch: int = 0):
-        return {sizes: kernels.shared_prefix_plan(table, q_start, contexts, self.runner.page_tokens, *sizes, torch.bfloat16, self.runner.runtime.device, stretch)
-                for sizes in self.sizes}
+        return Plans(self.group, {sizes: kernels.shared_prefix_plan(table, q_start, contexts, self.runner.page_tokens, *sizes, torch.bfloat16, self.runner.runtime.device, stretch)
+                                  for sizes in self.sizes})
 
     # ------------------------------------------------------------------ captured decode steps
     def _are(self, entries) -> bool:

@@ -119,13 +119,14 @@ class PagedGQAttention(Part):
     def _decodes_fused(self, tokens, ctx, cache) -> bool:
         """One token per request, the projection's tail inside the attention kernel: then that kernel
         can also apply the norm's scale, and the q/k/v product takes the rows as they are."""
-        return tokens <= self.SPLIT_TOKENS and ctx.max_q_len == 1 and cache.write and ctx.shared is None and \
+        return tokens <= self.SPLIT_TOKENS and ctx.max_q_len == 1 and cache.write and ctx.shared_plan(self.shared_prefix_sizes(), cache.block_table) is None and \
             kernels.decode_fusable(tokens, self.heads, self.kv_heads, self.head_dim, cache.block_table.shape[1] * cache.page_tokens)
 
     def forward(self, h, x, ctx, cache: CacheView, state=None, norm=None):
         cos, sin = self.tables if self.tables is not None else (None, None)
         tokens = x.shape[0]
         dtype = self.qkv.weight.dtype
+        shared = ctx.shared_plan(self.shared_prefix_sizes(), cache.block_table)
         if dtype == torch.bfloat16 and tokens <= self.SPLIT_TOKENS:
             # few tokens: the product is a stream of weights, and a CTA streams only about 1/148 of
             # the memory bandwidth; split K so that every SM streams a share, accumulate in float32
@@ -138,7 +139,7 @@ class PagedGQAttention(Part):
                 self.qkv.accumulate(h if h is not None else norm.forward(x), acc)
             attended = torch.empty((tokens, self.heads * self.head_dim), dtype=dtype, device=x.device)
             max_keys = cache.block_table.shape[1] * cache.page_tokens
-            if ctx.max_q_len == 1 and cache.write and ctx.shared is None and kernels.decode_fusable(tokens, self.heads, self.kv_heads,
+            if ctx.max_q_len == 1 and cache.write and shared is None and kernels.decode_fusable(tokens, self.heads, self.kv_heads,
                                                                              self.head_dim, max_keys):
                 # one token per request: bias, rotation and the cache append happen inside the attention kernel
                 planned = ctx.planned_context or ctx.max_context
@@ -169,9 +170,8 @@ class PagedGQAttention(Part):
                                 self.runtime.status, interleaved=self.interleaved)
         q = qkv[:, :self.heads * self.head_dim]
         attended = torch.empty((tokens, self.heads * self.head_dim), dtype=qkv.dtype, device=qkv.device)
-        plan = ctx.shared.get(self.shared_prefix_sizes()) if ctx.shared is not None else None
-        if plan is not None:
-            kernels.attention_shared_prefix(q, cache.k, cache.v, cache.block_table, ctx.positions, plan, attended, self.runtime.status)
+        if shared is not None:
+            kernels.attention_shared_prefix(q, cache.k, cache.v, cache.block_table, ctx.positions, shared, attended, self.runtime.status)
         else:
             kernels.paged_attention(q, cache, ctx, attended, self.heads, self.kv_heads, self.head_dim,
                                     self.runtime.status)

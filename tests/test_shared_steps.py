@@ -98,3 +98,32 @@ def test_a_capture_serves_tables_within_its_width(monkeypatch):
     entries[1].seq.tables = [[1, 2, 3, 4, 5]]
     assert steps.captured(entries) is None and steps.captured(entries, 1) is None
     assert steps.due(entries, behind=1) and steps.decode_graph(entries, True) == "another"
+
+
+def context_of(groups, group, plans):
+    import torch
+    from sprout_lm_b200.engine.batch import StepContext
+    tables = [torch.full((2, 3), g, dtype=torch.int32) for g in range(groups)]
+    none = torch.zeros(0, dtype=torch.int32)
+    ctx = StepContext(num_tokens=2, num_seqs=2, max_q_len=1, max_context=9, token_ids=none, positions=none, seq_of_token=none, q_start=none,
+                      context_lens=none, state_slots=none, logits_rows=none, block_tables=tables, page_tokens=16)
+    ctx.shared = plans and shared.Plans(group, plans)
+    return ctx
+
+
+def test_a_plan_is_its_page_groups_alone(monkeypatch):
+    """Layers of another page group have pages of their own, whatever their sizes: they take no plan of the first's, and keep the kernels that
+    they have without one."""
+    from types import SimpleNamespace
+    from sprout_lm_b200.parts import attention
+    monkeypatch.setattr(attention.kernels, "decode_fusable", lambda *sizes: True)
+    mixer = attention.PagedGQAttention.__new__(attention.PagedGQAttention)
+    mixer.heads, mixer.kv_heads, mixer.head_dim = 4, 2, 16
+    view = lambda table: SimpleNamespace(block_table=table, page_tokens=16, write=True)
+    for group in (0, 1):
+        ctx = context_of(2, group, {(4, 2, 16): "plan"})
+        mine, other = ctx.block_tables[group], ctx.block_tables[1 - group]
+        assert ctx.shared_plan((4, 2, 16), mine) == "plan" and ctx.shared_plan((4, 2, 32), mine) is None and ctx.shared_plan((4, 2, 16), other) is None
+        assert not mixer._decodes_fused(2, ctx, view(mine)) and mixer._decodes_fused(2, ctx, view(other))
+    ctx = context_of(1, 0, None)
+    assert ctx.shared_plan((4, 2, 16), ctx.block_tables[0]) is None and mixer._decodes_fused(2, ctx, view(ctx.block_tables[0]))
