@@ -27,9 +27,19 @@ def uniform_for(seed: int, request_id: str, index: int) -> float:
 
 def verify_uniforms(seed: int, request_id: str, index: int, tokens: int) -> tuple[list, list]:
     """The numbers that check ``tokens`` - 1 drafts from output token ``index`` of a request on: (accept, draw), one each per token of its
-    step.  Functions of (seed, request id, index of the output token) alone; the draws are those of plain sampling (``uniform_for``)."""
+    step.  Functions of (seed, request id, index of the output token) alone; the draws are those of plain sampling (``uniform_for``).
+
+    What comes out is distributed as the target's own tokens only if the drafts were drawn with other numbers than these: under the same
+    seed and id a draft model sampled with ``uniform_for`` has the draws' own, and the token behind a draft that falls would follow from
+    that draft.  ``draft_uniforms`` has numbers for the drafts."""
     return ([uniform_for(seed, f"{request_id}:accept", index + i) for i in range(tokens)],
             [uniform_for(seed, request_id, index + i) for i in range(tokens)])
+
+
+def draft_uniforms(seed: int, request_id: str, index: int, drafts: int) -> list:
+    """The numbers that draw a request's drafts for output tokens ``index`` on (``sample``'s ``uniforms`` on the draft model's logits): functions of
+    (seed, request id, index of the output token) alone, and none of those that check the drafts (``verify_uniforms``)."""
+    return [uniform_for(seed, f"{request_id}:draft", index + i) for i in range(drafts)]
 
 
 def sample(logits: torch.Tensor, status: torch.Tensor, temperatures: torch.Tensor | None = None,
@@ -50,9 +60,10 @@ def verify(logits: torch.Tensor, drafts: torch.Tensor, row_start: torch.Tensor, 
     """Drafted tokens against the target's probabilities: ``(tokens, accepted)``, int32 on the device.
 
     ``tokens`` has a place per row of ``logits``: a request's drafts that stand, the token drawn after them, then -1 (so too in rows that are
-    no request's); ``accepted`` says how many stand.  What is emitted is distributed as if drawn from the target alone; a greedy request (temperature 0, or none given)
+    no request's); ``accepted`` says how many stand.  What is emitted is distributed as if drawn from the target alone, where the drafts were drawn from the draft model's
+    distribution with numbers of their own (``draft_uniforms``), not with ``accept`` or ``draw``; a greedy request (temperature 0, or none given)
     gets the target's argmax at every place.  The arguments are those of ``kernels.verify_drafts`` (csrc/verify.cu), which this launches."""
     return kernels.verify_drafts(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw)
 
 
-__all__ = ["sample", "uniform_for", "verify", "verify_uniforms"]
+__all__ = ["draft_uniforms", "sample", "uniform_for", "verify", "verify_uniforms"]

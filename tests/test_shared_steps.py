@@ -127,3 +127,32 @@ def test_a_plan_is_its_page_groups_alone(monkeypatch):
         assert not mixer._decodes_fused(2, ctx, view(mine)) and mixer._decodes_fused(2, ctx, view(other))
     ctx = context_of(1, 0, None)
     assert ctx.shared_plan((4, 2, 16), ctx.block_tables[0]) is None and mixer._decodes_fused(2, ctx, view(ctx.block_tables[0]))
+
+
+def test_drafts_have_numbers_of_their_own():
+    from sprout_lm_b200.sampling import draft_uniforms
+    drafts = draft_uniforms(5, "a", 10, 4)
+    assert drafts[2:] == draft_uniforms(5, "a", 12, 2) and all(0.0 <= u < 1.0 for u in drafts)
+    accept, draw = verify_uniforms(5, "a", 10, 4)
+    assert not set(drafts) & {*accept, *draw}
+
+
+def test_emitted_tokens_follow_the_target_with_the_drafts_own_numbers():
+    """Drafts drawn with ``draft_uniforms`` and checked with ``verify_uniforms``, the definition in 64 bits, 40,000 requests under one seed: the
+    first token's frequencies are the target's within five standard deviations (the binomial's).  With the draws' own numbers for the
+    drafts they are not."""
+    from sprout_lm_b200.sampling import draft_uniforms
+    rng = np.random.default_rng(0)
+    p, q = (np.exp(1.2 * rng.standard_normal(8)) for _ in range(2))
+    p, q = p / p.sum(), q / q.sum()
+    left = np.maximum(p - q, 0.0)
+    pick = lambda weights, u: int(np.searchsorted(np.cumsum(weights), u * weights.sum(), side="right"))
+    count = 40000
+    seen = {"own": np.zeros(8), "draws": np.zeros(8)}
+    for r in range(count):
+        (u, _), (w, _) = verify_uniforms(3, f"r{r}", 0, 2)
+        for name, number in (("own", draft_uniforms(3, f"r{r}", 0, 1)[0]), ("draws", w)):
+            draft = pick(q, number)
+            seen[name][draft if u * q[draft] < p[draft] else pick(left, w)] += 1 / count
+    off = {name: np.abs(f - p) / np.sqrt(p * (1 - p) / count) for name, f in seen.items()}
+    assert (off["own"] <= 5).all() and off["draws"].max() > 5
