@@ -12,10 +12,15 @@
 // maximum; the token is the first row's argmax that was not drafted.
 //
 // A draw decides between neighbouring tokens by a sum over the vocabulary, and neighbours with probabilities of 1e-6 lie next to one
-// another: float32 exponentials leave the running sum off by 1e-8 and would pick the neighbour once in a few hundred draws.  So the
-// sums a draw is made from are 64-bit sums of 64-bit exponentials (`pow2`: 1e-12).  Those take 33 cycles of an SM's quarter a warp of
-// logits (some 15 64-bit operations, two cycles each), 1.09 T a second, while memory delivers 1.6 T logits a second: only the row that is
-// drawn from takes them.  Whether a draft stands is decided by float32 exponentials, whose sums are good to 1e-8.
+// another: a running sum that is off by 1e-7 would pick the neighbour once in some ten draws.  So the sums a draw is made from are 64-bit
+// sums of 64-bit exponentials (`pow2`: 1e-12).  Those take 33 cycles of an SM's quarter a warp of logits (some 15 64-bit operations, two
+// cycles each), 1.09 T a second, while memory delivers 1.6 T logits a second: only the row that is drawn from takes them.
+//
+// Whether a draft stands is decided by float32 exponentials.  A term 2^((v - max) c) has its difference, c = log2(e) / T and their product
+// rounded, 2^-24 of the exponent each, then the hardware's 2^-22 and up to eight float32 additions: a row's sum is off by at most
+// (3 d + 12) 2^-24 of itself, d the mean of (max - v) / T under the row's own probabilities.  d is 2 to 6 for wide rows, so that is 1 to 2e-6
+// at the most; a model of the roundings gives 1e-8 to 1.3e-7 for 151,936 normal logits at T of 0.5 to 1.7.  A draft whose p and u q are
+// closer than that may be decided either way.
 //
 // Three launches.  verify_rows_kernel: every row in pieces of PIECE logits, a warp each, their maxima and sums of exponentials (greedy:
 // the maximum's first index).  verify_decide_kernel: a block per request merges its rows' pieces, a warp a row, and finds the first row
@@ -23,9 +28,11 @@
 // block to be done also finds the run in which the draw falls and looks through it, else a fourth launch does.
 //
 // The difference in one pass: max(p - q, 0) needs both rows' sums before a single element of it is known.  With a_j, b_j the
-// exponentials and Za, Zb their sums, (p_j - q_j) Zb = a_j rho - b_j, rho = Zb / Za.  The float32 sums give rho to 1e-8, and so the set
-// of tokens where the difference is positive but for those within 1e-8 of zero, which do not matter (1e-8 of them, off by
-// 1e-8): the pass adds up a, b and, over that set, a and b again, from which the exact rho makes the difference's sums.
+// exponentials and Za, Zb their sums, (p_j - q_j) Zb = a_j rho - b_j, rho = Zb / Za.  The float32 sums give rho to the above, and so the set
+// of tokens where the difference is positive but for those within that of zero: the pass adds up a, b and, over that set, a and b again,
+// from which the exact rho makes the difference's sums a run.  They are off by as much of p at the most, and tokens within the run
+// that the draw falls in are told apart exactly.  Where p and q are so close that this is much of the difference, a draft falls as seldom:
+// what is emitted is off by no more than that.
 #include "common.cuh"
 
 namespace {
@@ -206,7 +213,7 @@ verify_rows_kernel(const Args p) {
       }
       index = __reduce_min_sync(0xffffffffu, index);
     } else {
-      // log2(e) / T rounded to a float shifts the sums by 1e-7 at most; infinite, it would make NaN of the maximum
+      // infinite, it would make NaN of the maximum
       const float c = fminf((float)(1.4426950408889634 / (double)own_temp), 3e38f);
       float sums[4] = {0.f, 0.f, 0.f, 0.f};
       if (count == PIECE) {

@@ -198,6 +198,55 @@ def test_equal_distributions(status):
     assert accepted == [4] * 12
 
 
+@pytest.mark.parametrize("counts,vocab", [([1, 3], 5000), ([1] * 40, 12000), ([2], 1100003), ([2] * 3, 1100003)])
+def test_nothing_left_of_the_difference(counts, vocab, status):
+    """Equal rows and numbers of 1, at which the first draft falls all the same: p - q is zero everywhere, and the token is drawn from p.  The
+    last summing block draws for few requests, a launch of its own for many; beyond 256 runs the sums stay in memory."""
+    c = case(counts, vocab, seed=17, noise=0.0)
+    c["accept"][:] = 1.0
+    tokens, accepted = check(c, status)
+    assert accepted == [0] * len(counts) and all(t >= 0 for t in np.array(tokens)[np.cumsum([0] + [n + 1 for n in counts])[:-1]])
+
+
+@pytest.mark.parametrize("noise", [1e-6, 1e-5, 1e-4])
+def test_close_distributions(noise, status):
+    """Draft rows that differ from the target's by little.  The sums that decide are off by at most (3 d + 12) 2^-24 of themselves, d the mean of
+    (max - logit) / T: a draft whose u q / p is further than both rows' from 1 falls or stands as the definition has it, and the token
+    of one that falls has something left of p - q and lies within the two rows' (of p, over what is left in all) of where the exact
+    running sum has the draw."""
+    count, vocab, t = 600, 20000, 0.9
+    rng = np.random.default_rng(5)
+    row = rng.standard_normal(vocab).astype(np.float32)
+    near = (row + (noise * rng.standard_normal(vocab)).astype(np.float32)).astype(np.float32)
+    p, q = softmax64(row, t), softmax64(near, t)
+    rel = sum((3 * float((w * (l.max() - l.astype(np.float64)) / t).sum()) + 12) * 2.0 ** -24 for l, w in ((row, p), (near, q)))
+    # drafts all over p / q, each with numbers on both sides of where it falls
+    by_ratio = np.argsort(p / q)
+    drafts = np.zeros(2 * count, np.int32)
+    drafts[::2] = by_ratio[np.linspace(0, vocab - 1, count).astype(int)]
+    accept = np.zeros(2 * count, np.float32)
+    accept[::2] = np.where(np.arange(count) % 3 == 0, 1 - 2.0 ** -24, (p / q)[drafts[::2]] * (1 + rng.choice([-4, 4], count) * rel))
+    draw = (np.arange(2 * count) / (2.0 * count)).astype(np.float32)
+    c = dict(logits=np.broadcast_to(row, (2 * count, vocab)).copy(), drafts=drafts, counts=[1] * count, draft_logits=np.broadcast_to(near, (count, vocab)).copy(),
+             temperatures=np.full(count, t, np.float32), accept=accept, draw=draw)
+    from sprout_lm_b200 import sampling
+    args, more = on_device(c)
+    tokens, accepted = (x.cpu().numpy() for x in sampling.verify(*args, status, **more))
+    assert int(status.item()) == 0
+    x = drafts[::2]
+    far = accept[::2].astype(np.float64) * q[x] / p[x] - 1.0
+    clear = np.abs(far) > rel
+    assert clear.sum() > count / 4 and (accepted == (far < 0))[clear].all()
+    fell = np.flatnonzero(accepted == 0)
+    left = np.maximum(p - q, 0.0)
+    sums = np.concatenate([[0.0], np.cumsum(left)])
+    assert len(fell) > 50
+    for r in fell:
+        token, target = int(tokens[2 * r]), float(draw[2 * r]) * sums[-1]
+        assert p[token] > q[token]
+        assert sums[token] - 2 * rel <= target <= sums[token + 1] + 2 * rel
+
+
 def test_drafted_token_with_all_the_weight(status):
     """A looked-up draft of probability 1 that falls all the same (a number of 1): drawn from p, the draft itself."""
     vocab = 4100
