@@ -1067,6 +1067,8 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     q_at, out_at = q.data_ptr(), out.data_ptr()
     # the one that starts first ends before the other (its last row is `width` elements)
     tokens, width = plan.rows
+    if out_stride[0] < width and tokens > 1:
+        raise KernelError(f"attention_shared_prefix: out's rows share memory ({out_stride[0]} apart, {width} wide)")
     gap = out_at - q_at
     if (gap if gap >= 0 else -gap) < ((tokens - 1) * (q_stride if gap >= 0 else out_stride)[0] + width) * plan.item_bytes:
         raise KernelError("attention_shared_prefix: q and out share memory")
@@ -1074,6 +1076,8 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
         scratch = q.new_empty(plan.scratch_floats, dtype=torch.float32)
     elif scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < plan.scratch_floats or scratch.data_ptr() % 16:
         raise KernelError(f"attention_shared_prefix: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
+    elif any(_overlap(scratch, t) for t in (q, out, k_cache, v_cache, block_table, positions, status, plan.buffer)):
+        raise KernelError("attention_shared_prefix: scratch shares memory with another argument")
     at = scratch.data_ptr()
     _run("sprout_attention_prefix", plan.address, q_at, q_stride[0], k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), table_stride[0],
          positions.data_ptr(), at, at + plan.sums_at, at + plan.gate_at, out_at, out_stride[0], pages[0], status.data_ptr(), _stream())

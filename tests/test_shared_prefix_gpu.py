@@ -395,6 +395,31 @@ def test_refusals(status):
     assert int(status.item()) == 0
 
 
+def test_memory_that_meets_itself_is_refused(status):
+    """Rows of the output that share memory, and a given scratch inside another argument: nothing is launched."""
+    from sprout_lm_b200 import kernels
+    step = Step(14, 2, 64, F32, 16, [0] * 3, [10], [5, 9, 0], [1, 2, 1], seed=13)
+    plan, width = step.plan(), 14 * 64
+    whole = torch.full((plan.scratch_floats + 8 * width,), 7.0, device=DEV)
+    call = lambda q, out, scratch=None: kernels.attention_shared_prefix(q, step.k, step.v, step.block_table, step.positions, plan, out, status, scratch)
+    for apart in (0, 64, width - 1):
+        with pytest.raises(kernels.KernelError, match="rows share memory"):
+            call(step.q, whole.as_strided((4, width), (apart, 1)))
+    scratch = whole[:plan.scratch_floats]
+    for at in (plan.scratch_floats - 1, 0, plan.scratch_floats // 2):
+        with pytest.raises(kernels.KernelError, match="scratch shares memory"):
+            call(step.q, whole[at:at + 4 * width].view(4, width), scratch)
+        with pytest.raises(kernels.KernelError, match="scratch shares memory"):
+            call(whole[at:at + 4 * width].view(4, width), torch.empty_like(step.q), scratch)
+    with pytest.raises(kernels.KernelError, match="scratch shares memory"):
+        call(step.q, torch.empty_like(step.q), step.k.view(-1)[:plan.scratch_floats])
+    assert bool((whole == 7.0).all()) and int(status.item()) == 0
+    out = whole[plan.scratch_floats:][:4 * width].view(4, width)
+    call(step.q, out, scratch)
+    want, tol = step.exact()
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
 # ---------------------------------------------------------------------------------- plans for later steps
 
 LATER = [(14, 2, 64, BF16, 16), (28, 4, 128, BF16, 16), (14, 2, 64, BF16, 5), (5, 1, 48, BF16, 16), (28, 4, 128, BF16, 128), (6, 3, 40, BF16, 8), (14, 2, 64, F32, 16), (3, 1, 144, BF16, 16)]
