@@ -1070,7 +1070,8 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
     if out_stride[0] < width and tokens > 1:
         raise KernelError(f"attention_shared_prefix: out's rows share memory ({out_stride[0]} apart, {width} wide)")
     gap = out_at - q_at
-    if (gap if gap >= 0 else -gap) < ((tokens - 1) * (q_stride if gap >= 0 else out_stride)[0] + width) * plan.item_bytes:
+    if (gap if gap >= 0 else -gap) < ((tokens - 1) * (q_stride if gap >= 0 else out_stride)[0] + width) * plan.item_bytes \
+            and not _columns_apart(gap // plan.item_bytes, width, tokens, q_stride[0], out_stride[0]):
         raise KernelError("attention_shared_prefix: q and out share memory")
     if scratch is None:
         scratch = q.new_empty(plan.scratch_floats, dtype=torch.float32)
@@ -1120,6 +1121,12 @@ def _overlap(a, b) -> bool:
         return True
     low, gap = (a, b0 - a0) if a0 < b0 else (b, a0 - b0)       # the one that starts first reaches the other's start?
     return gap < (sum((n - 1) * s for n, s in zip(low.shape, low.stride())) + 1) * low.element_size()
+
+
+def _columns_apart(gap, width, rows, a_stride, b_stride) -> bool:
+    """Whether two matrices of `rows` rows of `width` elements, the second `gap` elements behind the first, lie side by side in rows that are
+    as far apart in both: columns of one buffer."""
+    return a_stride == b_stride and rows > 1 and width <= gap % a_stride <= a_stride - width
 
 
 def _check_verify(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw, out, accepted):

@@ -153,6 +153,22 @@ def test_strided_rows(dtype, dim, status):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q_first", [True, False])
+def test_queries_and_outputs_in_columns_of_one_buffer(dtype, q_first, status):
+    from sprout_lm_b200 import kernels
+    step = Step(14, 2, 64, dtype, 16, [0] * 5, [20], [5, 9, 0, 30, 100], [2, 1, 1, 3, 1], seed=6)
+    width = step.q.shape[1]
+    both = torch.full((step.q.shape[0], 2 * width + 64), 7.0, dtype=dtype, device=DEV)
+    mine, out = (both[:, :width], both[:, width:2 * width]) if q_first else (both[:, width:2 * width], both[:, :width])
+    mine.copy_(step.q)
+    step.q = mine
+    step.check(status, out)
+    assert bool((both[:, 2 * width:] == 7.0).all())
+    with pytest.raises(kernels.KernelError, match="q and out share memory"):
+        step.run(status, both[:, 64:64 + width])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_later_tokens_do_not_reach_earlier_ones(dtype, status):
     """Non-finite keys and values of a request's later tokens leave its earlier tokens, and all other requests, as they were."""
     step = Step(14, 2, 64, dtype, 16, [0] * 4, [20], [5, 9, 0, 30], [6, 1, 20, 3], seed=7)

@@ -268,3 +268,18 @@ def test_pages_outside_the_pool(seed):
 def test_a_short_request_beside_a_negative_page():
     plan = HostPlan([[5, 6, 7, 8], [-1, 9, 10, 11], [3, 4, 5, 6]], [0, 1, 2, 3], [3, 40, 40], 16, 8, 2, True, 60)
     assert len(plan.segments) == 3 and plan.read_keys == 83
+
+
+def test_columns_of_one_buffer_do_not_share_memory():
+    """Against the elements themselves."""
+    from sprout_lm_b200 import kernels
+    for stride in (4, 9, 13):
+        for width in range(1, 5):
+            for gap in range(-30, 31):
+                places = lambda start: {start + r * stride + c for r in range(3) for c in range(width)}
+                apart = not places(0) & places(gap)
+                said = kernels._columns_apart(gap, width, 3, stride, stride)
+                assert not said or apart                  # never side by side when they meet
+                if apart and gap % stride:                # and found wherever both keep to columns of their own
+                    assert said == (width <= gap % stride <= stride - width)
+    assert not kernels._columns_apart(5, 4, 3, 9, 10) and not kernels._columns_apart(0, 4, 1, 9, 9)
