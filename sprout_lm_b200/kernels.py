@@ -985,8 +985,16 @@ class SharedPrefixPlan:
         # the partial results, then their maxima and sums, then the gate between a call's launches (csrc/attention_prefix.cuh); places in bytes
         self.scratch_floats = host.parts * heads * (head_dim + 2) + 2
         self.sums_at, self.gate_at = 4 * host.parts * heads * head_dim, 4 * host.parts * heads * (head_dim + 2)
+        self.stream = _stream() if self.device_index >= 0 else None        # the buffer's own: its memory is used again in this one's order
         # what a call's tensors have to be
         self.rows, self.page, self.token_shape, self.item_bytes = (host.tokens, heads * head_dim), (kv_heads, page_tokens, head_dim), (host.tokens,), dtype.itemsize
+
+
+    def used_on_another_stream(self):
+        """A plan that its owner lets go is not overwritten while the current stream still reads it.  (A capture reads it whenever it is replayed,
+        and keeps nothing alive.)"""
+        if not torch.cuda.is_current_stream_capturing():
+            self.buffer.record_stream(torch.cuda.current_stream())
 
 
 def _prefix_slots(head_dim: int, tensor_cores: bool) -> tuple[int, int, int]:
@@ -1079,9 +1087,11 @@ def attention_shared_prefix(q, k_cache, v_cache, block_table, positions, plan: S
         raise KernelError(f"attention_shared_prefix: scratch must be {plan.scratch_floats} contiguous float32 values on a 16-byte boundary")
     elif any(_overlap(scratch, t) for t in (q, out, k_cache, v_cache, block_table, positions, status, plan.buffer)):
         raise KernelError("attention_shared_prefix: scratch shares memory with another argument")
-    at = scratch.data_ptr()
+    at, stream = scratch.data_ptr(), _stream()
+    if stream != plan.stream:
+        plan.used_on_another_stream()
     _run("sprout_attention_prefix", plan.address, q_at, q_stride[0], k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), table_stride[0],
-         positions.data_ptr(), at, at + plan.sums_at, at + plan.gate_at, out_at, out_stride[0], pages[0], status.data_ptr(), _stream())
+         positions.data_ptr(), at, at + plan.sums_at, at + plan.gate_at, out_at, out_stride[0], pages[0], status.data_ptr(), stream)
 
 
 def sample(logits, out, status, temperature=None, uniform=None):

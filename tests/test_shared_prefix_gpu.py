@@ -357,6 +357,26 @@ def test_two_calls_at_once(status):
     assert all(torch.equal(out, want) for out in outs) and int(status.item()) == 0
 
 
+def test_a_plan_let_go_while_another_stream_reads_it(status):
+    """The plan's memory is not given to others before a call on another stream than its own is done, whoever held it last."""
+    step = Step(28, 4, 128, BF16, 16, [0] * 20, [300], list(range(0, 400, 20)), [1] * 20, seed=16)
+    want = step.run(status)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        plan, out = step.plan(), torch.full_like(step.q, float("nan"))
+        size = plan.buffer.numel()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)                # ten milliseconds or so
+            step.run(status, out=out, plan=plan)
+        assert not side.query()
+        del plan
+        held = [torch.zeros(size, dtype=torch.int32, device=DEV) for _ in range(20)]      # what the allocator has to give of that size
+        side.synchronize()
+        assert torch.equal(out, want) and int(status.item()) == 0
+        del held
+
+
 @pytest.mark.parametrize("shape", [(128, 1, 64), (64, 1, 128), (17, 1, 16)])
 def test_many_query_heads_a_key_value_head(shape, status):
     """More query rows a token than an item of few rows holds."""
