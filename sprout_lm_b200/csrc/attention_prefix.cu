@@ -187,13 +187,6 @@ attention_prefix_simple_kernel(const Params p) {
 }
 
 // ------------------------------------------------------------------ mma.sync
-// 2^x, the hardware approximation; results below the normal range are zero
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Keys and values in steps through shared memory (cp.async), three or four CTAs an SM.  The next step's keys are asked for when this
 // step's scores are done, its values when this step's outputs are, so that a buffer of each is always on its way or in use.  NARROW (an
 // item of up to 16 rows): the rows are one tile of the MMA, each of the 4 warps takes 32 of a step's 128 keys, and the warps' results are

@@ -33,11 +33,6 @@ struct Layout {
   static constexpr int SMEM = OFF_BAR + 128;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 // The same; whether all threads say so.
 __device__ __forceinline__ bool compute_barrier_and(bool mine) {

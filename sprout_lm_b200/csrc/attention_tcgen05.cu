@@ -107,13 +107,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for x <= 0 (a probability): the hardware approximation, results below the normal range are zero
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // SPLIT: the launch has fewer 256-row pieces than the GPU has SMs.  The first `split_pieces`
 // pieces of the launch (the longest) then get two CTAs each, which take alternate key tiles.
 // Each leaves its partial result (maximum, sum and accumulators of every row) in global scratch

@@ -84,13 +84,6 @@ __device__ __forceinline__ float4 load_four(const float* row, int at, int end, b
   return make_float4(at < end ? row[at] : -INFINITY, at + 1 < end ? row[at + 1] : -INFINITY, at + 2 < end ? row[at + 2] : -INFINITY,
                      at + 3 < end ? row[at + 3] : -INFINITY);
 }
-// 2^x, the hardware approximation
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // A run's logits of this thread.
 __device__ __forceinline__ void load_run(const float* run, int count, float (&v)[PER_THREAD]) {
   const bool aligned = ((uintptr_t)run & 15) == 0;
