@@ -8,9 +8,10 @@
 //
 // What bounds it is memory where the items are many, up to the walk's end, where the last pairs of some CTAs run alone: 128 requests of 1,500
 // keys of their own (28 heads over 4 of 128) 395 MB in 76 us, 5.2 TB/s, cold.  What is in flight does not: head size 128 has room for two
-// CTAs an SM, each with up to 96 KB on its way, and 44 KB an SM cover a microsecond at the full rate.  A short walk is bound by a step's chain: scores, maximum, barrier,
-// exponentials, barrier, products, 1.1 us.  With the copies issued by the computing warps (cp.async, some twelve instructions a thread and
-// 16 bytes) their instructions bounded it: 4.9 TB/s at three CTAs an SM, 3.7 with a ring of three stages at two.
+// CTAs an SM, each with up to 96 KB on its way, and 44 KB an SM cover a microsecond at the full rate.  A short walk is bound by a step's
+// chain: scores, maximum, barrier, exponentials, barrier, products, 1.1 us.  With the copies issued by the computing warps (cp.async, some
+// twelve instructions a thread and 16 bytes) their instructions bounded it: 4.9 TB/s at three CTAs an SM, 3.7 with a ring of three stages
+// at two.
 //
 // Every mbarrier wait is bounded: on a timeout the CTA sets the status word, waits (bounded) for its copies in flight and returns.
 #include "attention_bf16.cuh"

@@ -252,7 +252,8 @@ class ModelRunner:
 
         ``temperatures``: per entry (0: greedy); ``accept`` and ``draw``: uniform numbers in [0, 1), one per token of the batch, the
         first for whether the draft behind the token stands, the second for the token drawn there (``sampling.verify_uniforms`` makes
-        them; drafts are drawn with others, ``sampling.draft_uniforms``).  ``draft_logits``: the draft model's float32 rows [drafts, vocab] entry by entry, None for drafts that were looked up.
+        them; drafts are drawn with others, ``sampling.draft_uniforms``).  ``draft_logits``: the draft model's float32 rows [drafts, vocab]
+        entry by entry, None for drafts that were looked up.
         A request whose logits are not finite gets -1 (``check_status`` says why).  Models that keep per-request state cannot take
         tokens back: refused."""
         self._take_ahead(None, None, None)

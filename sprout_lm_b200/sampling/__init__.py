@@ -60,8 +60,8 @@ def verify(logits: torch.Tensor, drafts: torch.Tensor, row_start: torch.Tensor, 
     """Drafted tokens against the target's probabilities: ``(tokens, accepted)``, int32 on the device.
 
     ``tokens`` has a place per row of ``logits``: a request's drafts that stand, the token drawn after them, then -1 (so too in rows that are
-    no request's); ``accepted`` says how many stand.  What is emitted is distributed as if drawn from the target alone, where the drafts were drawn from the draft model's
-    distribution with numbers of their own (``draft_uniforms``), not with ``accept`` or ``draw``; a greedy request (temperature 0, or none given)
+    no request's); ``accepted`` says how many stand.  What is emitted is distributed as if drawn from the target alone, where the drafts were
+    drawn from the draft model's distribution with numbers of their own (``draft_uniforms``), not with ``accept`` or ``draw``; a greedy request (temperature 0, or none given)
     gets the target's argmax at every place.  The arguments are those of ``kernels.verify_drafts`` (csrc/verify.cu), which this launches."""
     return kernels.verify_drafts(logits, drafts, row_start, status, draft_logits, temperatures, accept, draw)
 
