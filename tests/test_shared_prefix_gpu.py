@@ -361,17 +361,18 @@ def test_a_plan_let_go_while_another_stream_reads_it(status):
     """The plan's memory is not given to others before a call on another stream than its own is done, whoever held it last."""
     step = Step(28, 4, 128, BF16, 16, [0] * 20, [300], list(range(0, 400, 20)), [1] * 20, seed=16)
     want = step.run(status)
-    side = torch.cuda.Stream()
+    side, scratch = torch.cuda.Stream(), torch.empty(step.plan().scratch_floats, device=DEV)
+    from sprout_lm_b200 import kernels
     for _ in range(3):
         plan, out = step.plan(), torch.full_like(step.q, float("nan"))
-        size = plan.buffer.numel()
+        size, at = plan.buffer.numel(), plan.buffer.data_ptr()
         torch.cuda.synchronize()
         with torch.cuda.stream(side):
-            torch.cuda._sleep(20_000_000)                # ten milliseconds or so
-            step.run(status, out=out, plan=plan)
-        assert not side.query()
+            torch.cuda._sleep(100_000_000)               # fifty milliseconds or so
+            kernels.attention_shared_prefix(step.q, step.k, step.v, step.block_table, step.positions, plan, out, status, scratch)
         del plan
         held = [torch.zeros(size, dtype=torch.int32, device=DEV) for _ in range(20)]      # what the allocator has to give of that size
+        assert side.query() or at not in [t.data_ptr() for t in held]
         side.synchronize()
         assert torch.equal(out, want) and int(status.item()) == 0
         del held
